@@ -12,6 +12,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -20,7 +22,8 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_NAME = "libgemma4_qmm.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 
-SOURCES = ["qmm_runtime.cpp", "q4_layout.hip", "q4_decode.hip", "q4_limbs.hip", "q4_gemm.hip", "q4_gemm_kpair.hip", "q4_lora.hip"]
+SOURCES = ["qmm_runtime.cpp", "q4_layout.hip", "q4_decode.hip", "q4_limbs.hip", "q4_gemm.hip", "q4_gemm_kpair.hip", "q4_lora.hip",
+           "kv_runtime.cpp", "kv_heads.hip", "kv_attention.hip"]
 ARCH = "gfx950"
 # measurement aid for the benchmark (a read-only HBM streaming kernel), its own library
 PROBE_SOURCES = ["hbm_probe.hip"]
@@ -48,8 +51,6 @@ DEVICE_FLAGS = [
 
 def device_asm(source: str) -> str:
     """gfx950 assembly of one source file, compiled with the library's flags."""
-    import tempfile
-
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "out.s")
         cmd = [hipcc()] + DEVICE_FLAGS + ["--offload-device-only", "-S", "-I", os.path.join(ROOT, "include"),
@@ -61,16 +62,7 @@ def device_asm(source: str) -> str:
             return f.read()
 
 
-def _link(sources, path: str, verbose: bool) -> str:
-    os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = path + ".tmp"
-    cmd = [hipcc()] + DEVICE_FLAGS + [
-        "-fPIC",
-        "-shared",
-        "-Wall",
-        "-I", os.path.join(ROOT, "include"),
-        "-o", tmp,
-    ] + [os.path.join(CSRC, s) for s in sources]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -80,6 +72,21 @@ def _link(sources, path: str, verbose: bool) -> str:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{errs}")
     if errs.strip() and verbose:
         print(errs, file=sys.stderr)
+
+
+def _link(sources, path: str, verbose: bool) -> str:
+    """Compiles the sources (a few at a time, each on its own) and links them into `path`."""
+    os.makedirs(LIB_DIR, exist_ok=True)
+    with tempfile.TemporaryDirectory() as d:
+        objects = [os.path.join(d, s + ".o") for s in sources]
+        flags = DEVICE_FLAGS + ["-fPIC", "-Wall", "-I", os.path.join(ROOT, "include")]
+        with ThreadPoolExecutor(max_workers=6) as pool:
+            jobs = [pool.submit(_run, [hipcc()] + flags + ["-x", "hip", "-c", "-o", o, os.path.join(CSRC, s)], verbose)
+                    for s, o in zip(sources, objects)]
+            for job in jobs:
+                job.result()
+        tmp = path + ".tmp"
+        _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", tmp] + objects, verbose)
     os.replace(tmp, path)
     return path
 

@@ -323,6 +323,107 @@ Gemma4Status gemma4_qgeglu_create_device(const Gemma4QLinearDesc* desc, const ui
 Gemma4Status gemma4_qgeglu_forward(const Gemma4QLinear* pair, void* stream, const uint16_t* x_dev, uint32_t rows,
                                    void* h_dev, Gemma4QmmDtype h_dtype);
 
+/* ---- Attention over a paged cache ----
+ * What a layer does between its q|k|v projection and its o projection, for a batch of
+ * requests that each have one new token (decode), a few (a verify block) or many (a
+ * prompt or a chunk of one): the per-head norms and the rotation of queries and keys,
+ * the append of keys and values to the cache, and the attention that reads it.  In the
+ * reference these are MLX's fast::rms_norm, fast::rope and
+ * fast::scaled_dot_product_attention around a cache per request
+ * (native_model.cc:808-881); here the cache is paged and shared by the requests.
+ *
+ * All memory is the caller's; the structs below only describe it and may be built per
+ * call.  Strides are in elements.  Device arrays (positions, starts, lengths, tables) are
+ * read when the call's kernels run, so a captured graph follows their contents.
+ * q, k, v, weights and outputs are bf16; sums, norms, angles and softmax statistics are
+ * 32 bits or more, and results are rounded once, when they are stored. */
+
+typedef enum Gemma4KvDtype {
+    GEMMA4_KV_BF16 = 0,
+    GEMMA4_KV_E4M3 = 1 /* 8-bit floats (4 exponent bits, largest 448) times k_scale or v_scale */
+} Gemma4KvDtype;
+
+/* Page p of KV head h holds its token s at k_dev + p * page_stride + h * head_stride +
+ * s * token_stride, head_dim consecutive elements; v_dev likewise.  Any order of the
+ * three strides works ([pages, heads, page_size, head_dim] reads whole pages in runs).
+ *   page_size   a power of two, 16 to 65536
+ *   head_dim    64, 128, 256 or 512
+ *   k_dev, v_dev, and every stride in bytes: multiples of 16 */
+typedef struct Gemma4KvPages {
+    void* k_dev;
+    void* v_dev;
+    uint64_t page_stride, token_stride, head_stride;
+    uint32_t num_pages, page_size, kv_heads, head_dim;
+    uint32_t dtype; /* Gemma4KvDtype */
+    float k_scale, v_scale; /* finite, > 0; bf16 pages ignore them */
+} Gemma4KvPages;
+
+/* The new tokens of a batch: request r's are rows query_starts[r] .. query_starts[r+1] - 1
+ * of q (k, v, out), its last one at position kv_lens[r] - 1.  Position p of request r lies
+ * in page block_tables[r * table_stride + p / page_size], slot p % page_size.
+ *   query_starts_dev  int32 [requests + 1], nondecreasing from 0; rows past the last are
+ *                     padding: nothing is stored for them and their outputs are zeros
+ *   kv_lens_dev       int32 [requests], the new tokens included
+ *   block_tables_dev  int32 [requests, table_stride], pages_per_request entries used.  An
+ *                     entry outside [0, num_pages) is an absent page: append stores
+ *                     nothing there, attention sees no keys there */
+typedef struct Gemma4KvBatch {
+    const int32_t* query_starts_dev;
+    const int32_t* kv_lens_dev;
+    const int32_t* block_tables_dev;
+    uint32_t requests, tokens, pages_per_request, table_stride;
+} Gemma4KvBatch;
+
+/* Rotation by angle position * inv_freq[i] of elements (i, i + distance) for i < pairs;
+ * distance 1 means adjacent pairs (2i, 2i + 1).  Other elements pass unrotated.  pairs is
+ * a multiple of 8, pairs <= distance, distance a multiple of 8 (or 1) and
+ * distance + pairs <= head_dim (2 * pairs for adjacent ones).  pairs 0: no rotation. */
+typedef struct Gemma4Rope {
+    const float* inv_freq_dev; /* [pairs] */
+    uint32_t pairs, distance;
+} Gemma4Rope;
+
+/* `count` heads of every row: head h of row t at x_dev + t * x_stride + h * head_dim, e.g.
+ * a run of columns of a fused q|k|v output.  norm 1 divides each head by
+ * sqrt(mean of squares + eps) and multiplies by weight_dev (head_dim values; NULL: ones);
+ * norm 0 leaves it.  out_dev/out_stride: where the result goes (it may be x_dev itself
+ * with the same stride); NULL where it goes to the cache. */
+typedef struct Gemma4Heads {
+    const uint16_t* x_dev;
+    uint16_t* out_dev;
+    const uint16_t* weight_dev;
+    uint64_t x_stride, out_stride;
+    uint32_t count;
+    uint32_t norm;
+    float eps;
+} Gemma4Heads;
+
+/* Norm and rotation of q's and k's heads (k may be NULL) in one launch; positions_dev is
+ * int32 [rows].  rope NULL: norms only. */
+Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Rope* rope,
+                                 const int32_t* positions_dev, uint32_t rows, uint32_t head_dim, void* stream);
+
+/* Stores the batch's k (normed, rotated) and v (normed if v->norm, never rotated) into its
+ * pages, and, with q not NULL, norms and rotates q into q->out_dev in the same launch.
+ * k and v may read the same columns.  E4M3 pages hold value / scale, saturated at 448. */
+Gemma4Status gemma4_kv_append(const Gemma4KvPages* pages, const Gemma4KvBatch* batch, const Gemma4Heads* q,
+                              const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream);
+
+/* out[t, h] = softmax(scale * q[t, h] . K) V over the keys that row t's position p sees:
+ * positions 0..p, or with window > 0 the last `window` of those, in present pages.  Query
+ * heads share KV heads in equal consecutive groups (q_heads a multiple of kv_heads).  The
+ * batch's own tokens must be in the cache (gemma4_kv_append).  A row that sees no key
+ * gives zeros and lse -inf.  Whatever lies in hidden places (a page's unused slots
+ * included) is never part of a result, infinities and NaN included.
+ *   q_dev [tokens, q_heads, head_dim] with q_stride between rows, 16-byte aligned
+ *   out_dev the same shape with out_stride
+ *   lse_dev float [tokens, q_heads], log of the softmax's sum; NULL to skip
+ * Pages that no row's window reaches are not read.  Long key ranges of small batches are
+ * split over the card and joined by a second launch, in the stream's scratch memory. */
+Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch* batch, const uint16_t* q_dev,
+                                 uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
+                                 uint64_t out_stride, float* lse_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
