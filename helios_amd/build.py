@@ -23,7 +23,7 @@ LIB_NAME = "libgemma4_qmm.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 
 SOURCES = ["qmm_runtime.cpp", "q4_layout.hip", "q4_decode.hip", "q4_limbs.hip", "q4_gemm.hip", "q4_gemm_kpair.hip", "q4_lora.hip",
-           "kv_runtime.cpp", "kv_heads.hip", "kv_attention.hip"]
+           "kv_runtime.cpp", "kv_heads.hip", "kv_attention.hip", "kv_tile.hip"]
 ARCH = "gfx950"
 # measurement aid for the benchmark (a read-only HBM streaming kernel), its own library
 PROBE_SOURCES = ["hbm_probe.hip"]
@@ -43,17 +43,23 @@ DEVICE_FLAGS = [
     "-O3",
     "-std=c++17",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # MFMA results in arch VGPRs: the GEMM's fp32 accumulators are updated by
-    # VALU FMAs every group, which cannot read AGPRs
-    "-mllvm", "-amdgpu-mfma-vgpr-form",
 ]
+# MFMA results in arch VGPRs: the GEMM's fp32 accumulators are updated by VALU FMAs every
+# group, which cannot read AGPRs
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+# the 128-row attention tile keeps up to 256 accumulators that the VALU seldom touches
+AGPR_SOURCES = ()
+
+
+def device_flags(source: str) -> list:
+    return DEVICE_FLAGS + ([] if source in AGPR_SOURCES else VGPR_FORM)
 
 
 def device_asm(source: str) -> str:
     """gfx950 assembly of one source file, compiled with the library's flags."""
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "out.s")
-        cmd = [hipcc()] + DEVICE_FLAGS + ["--offload-device-only", "-S", "-I", os.path.join(ROOT, "include"),
+        cmd = [hipcc()] + device_flags(source) + ["--offload-device-only", "-S", "-I", os.path.join(ROOT, "include"),
                                           "-o", out, os.path.join(CSRC, source)]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
@@ -79,9 +85,9 @@ def _link(sources, path: str, verbose: bool) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     with tempfile.TemporaryDirectory() as d:
         objects = [os.path.join(d, s + ".o") for s in sources]
-        flags = DEVICE_FLAGS + ["-fPIC", "-Wall", "-I", os.path.join(ROOT, "include")]
+        flags = ["-fPIC", "-Wall", "-I", os.path.join(ROOT, "include")]
         with ThreadPoolExecutor(max_workers=6) as pool:
-            jobs = [pool.submit(_run, [hipcc()] + flags + ["-x", "hip", "-c", "-o", o, os.path.join(CSRC, s)], verbose)
+            jobs = [pool.submit(_run, [hipcc()] + device_flags(s) + flags + ["-x", "hip", "-c", "-o", o, os.path.join(CSRC, s)], verbose)
                     for s, o in zip(sources, objects)]
             for job in jobs:
                 job.result()

@@ -25,166 +25,12 @@
 // infinity or NaN in a hidden value would still be NaN: values of such groups that are
 // not finite are taken as zero in the product, and what of them is visible is added to
 // the outputs at the end (fix_nonfinite; only workgroups that met one run it).
-#include "kv_index.h"
-#include "kv_kernels.h"
-#include "q4_common.h"
+#include "kv_device.h"
 
 namespace kv {
 namespace {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kWaves = 4;
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kNegInf = -__builtin_huge_valf();
-
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Maximum and sum over the four lanes l % 16, + 16, + 32, + 48.
-__device__ __forceinline__ float col_max(float v) {
-    u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
-    p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
-}
-__device__ __forceinline__ float col_sum(float v) {
-    u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(p.x) + __uint_as_float(p.y);
-    p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(p.x) + __uint_as_float(p.y);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    return (uint32_t)q4::f32_to_bf16(a) | ((uint32_t)q4::f32_to_bf16(b) << 16);
-}
-
-// Two e4m3 of a word as two bf16 (exact).
-template <bool HI>
-__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
-}
-
-// Zeros the bf16 (or e4m3) values of a word that are infinite or NaN.
-template <bool FP8>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-    uint32_t keep = 0;
-    if (FP8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (((w >> (8 * i)) & 0x7Fu) != 0x7Fu) keep |= 0xFFu << (8 * i);
-    } else {
-        if ((w & 0x7F80u) != 0x7F80u) keep |= 0xFFFFu;
-        if ((w & 0x7F800000u) != 0x7F800000u) keep |= 0xFFFF0000u;
-    }
-    return w & keep;
-}
-template <bool FP8>
-__device__ __forceinline__ bool any_nonfinite(uint32_t w) {
-    if (FP8) {
-        // a byte is NaN as its low seven bits are all ones: adding one then carries into bit 7
-        return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
-    }
-    return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-}
-
-// A query tile: `n` consecutive rows of q from `row0`, at positions pos0.. of `request`.
-struct Tile {
-    int request, row0, n, pos0, kv_len;
-};
-
-// Tile number `tile` of the batch when every request's rows are cut into runs of `tokens`;
-// n = 0 past the last.  All lanes of a wave take part; the result is the same in all.
-__device__ __forceinline__ Tile find_tile(const Batch& b, int tile, int tokens, int lane) {
-    int before = 0;
-    for (int base = 0; base <= b.requests; base += 64) {
-        const int r = base + lane;
-        int s = 0, e = 0, len = 0;
-        if (r <= b.requests) {
-            s = run_bound(b.starts, r, b.requests, b.tokens);
-            e = run_bound(b.starts, r + 1, b.requests, b.tokens);
-            len = r < b.requests ? b.kv_lens[r] : 0;
-        }
-        const int rows = e > s ? e - s : 0;
-        const int tiles = (rows + tokens - 1) / tokens;
-        int sum = tiles;  // inclusive sum over the lanes
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(sum, d);
-            sum += lane >= d ? o : 0;
-        }
-        const unsigned long long past = __ballot(before + sum > tile);
-        if (past != 0) {
-            const int at = __ffsll(past) - 1;
-            Tile t;
-            t.request = base + at;
-            const int first = before + __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at);
-            const int start = __builtin_amdgcn_readlane(s, at), count = __builtin_amdgcn_readlane(rows, at);
-            const int skip = (tile - first) * tokens;
-            t.row0 = start + skip;
-            t.n = count - skip < tokens ? count - skip : tokens;
-            const int kv = __builtin_amdgcn_readlane(len, at);
-            t.pos0 = kv - count + skip;
-            t.kv_len = kv;
-            return t;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-    }
-    return Tile{0, 0, 0, 0, 0};
-}
-
-// Tokens x heads of a query tile of ROWS rows: all of a KV head's query heads if they fit
-// (row = token * heads + head), else runs of ROWS of them.
-struct Shape {
-    int heads, chunks, tokens;
-};
-__host__ __device__ inline Shape tile_shape(int rows, int group) {
-    Shape s;
-    s.heads = group < rows ? group : rows;
-    s.chunks = ceil_div(group, s.heads);
-    s.tokens = rows / s.heads;
-    return s;
-}
-
-// Adds the infinities and NaN of groups that some row does not see to the outputs of the
-// rows that do see them.  `put(row, dim, v)` adds v to that output.  Keys [lo, hi), from
-// a multiple of 16.
-template <int D, bool FP8, class Put>
-__device__ void fix_nonfinite(const AttnArgs& a, const Tile& t, const Shape& sh, int kv_head, int lo, int hi, int threads,
-                              Put put) {
-    const int* table = a.batch.tables + (int64_t)t.request * a.batch.stride;
-    const Pages& pg = a.pages;
-    for (int key = lo; key < hi; ++key) {
-        const int base = key & ~(kGroupKeys - 1);
-        if (all_visible(base, kGroupKeys, t.pos0, t.n, a.window)) continue;
-        const int page = page_at(table, key >> pg.page_shift, a.batch.width, pg.num_pages);
-        if (page < 0) continue;
-        const int64_t off = (int64_t)page * pg.page_stride + (int64_t)kv_head * pg.head_stride +
-                            (int64_t)(key & ((1 << pg.page_shift) - 1)) * pg.token_stride;
-        for (int d = (int)threadIdx.x; d < D; d += threads) {
-            float v;
-            if (FP8) {
-                const uint32_t b = (uint8_t)pg.v[off + d];
-                if ((b & 0x7Fu) != 0x7Fu) continue;
-                v = __uint_as_float(0x7FC00000u);
-            } else {
-                const uint32_t b = reinterpret_cast<const uint16_t*>(pg.v)[off + d];
-                if ((b & 0x7F80u) != 0x7F80u) continue;
-                v = __uint_as_float(b << 16);
-            }
-            for (int i = 0; i < t.n; ++i) {
-                const int pos = t.pos0 + i;
-                if (key > pos || (a.window > 0 && key <= pos - a.window)) continue;
-                for (int h = 0; h < sh.heads; ++h) put(i, h, d, v);
-            }
-        }
-    }
-}
-
 template <int D, bool FP8>
 struct Rows16 {
     static constexpr int kElt = FP8 ? 1 : 2;
@@ -216,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     const int part = (int)blockIdx.x - tile_no * per_tile;
     const int kv_head = part / sh.chunks, chunk = part - kv_head * sh.chunks;
 
-    const Tile t = find_tile(a.batch, tile_no, sh.tokens, lane);
+    const Tile t = find_tile(a.batch, tile_no, sh.tokens, 1, a.tile_from - 1, lane);
     if (t.n <= 0) return;
     const int kv_len = clampi(t.kv_len, 0, a.batch.width << a.pages.page_shift);
 
@@ -472,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     if (fix) {
         const int from = lo + range.first * kTileKeys;
         const int upto = lo + range.last * kTileKeys < keys.hi ? lo + range.last * kTileKeys : keys.hi;
-        fix_nonfinite<D, FP8>(a, t, sh, kv_head, from, upto, 64 * kWaves, [&](int i, int h, int d, float v) {
+        fix_nonfinite<D, FP8>(a, t, sh, kv_head, from, upto, kGroupKeys, 64 * kWaves, [&](int i, int h, int d, float v) {
             const int ig = chunk * sh.heads + h;
             if (ig >= group) return;
             const int64_t rr = t.row0 + i;
@@ -519,28 +365,71 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, float v_scale) {
 }
 
 template <int D, bool FP8>
-hipError_t launch(const AttnArgs& a, hipStream_t stream) {
+hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
     const Shape sh = tile_shape(16, a.q_heads / a.pages.kv_heads);
-    const unsigned tiles = (unsigned)(a.batch.tokens / sh.tokens + a.batch.requests + 1);
+    // requests of tile_from rows or more are not this kernel's
+    const int64_t all = a.batch.tokens / sh.tokens + a.batch.requests + 1;
+    const int64_t small = (int64_t)(a.batch.requests + 1) * ceil_div(a.tile_from - 1, sh.tokens);
+    const unsigned tiles = (unsigned)(all < small ? all : small);
     rows16_kernel<D, FP8><<<dim3(tiles * (unsigned)(a.pages.kv_heads * sh.chunks), (unsigned)a.splits), 64 * kWaves, 0, stream>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
+    return hipGetLastError();
+}
+
+hipError_t launch_rows16(const AttnArgs& a, hipStream_t stream) {
+    switch (a.pages.head_dim * 2 + a.pages.fp8) {
+        case 128: return launch_rows<64, false>(a, stream);
+        case 129: return launch_rows<64, true>(a, stream);
+        case 256: return launch_rows<128, false>(a, stream);
+        case 257: return launch_rows<128, true>(a, stream);
+        case 512: return launch_rows<256, false>(a, stream);
+        case 513: return launch_rows<256, true>(a, stream);
+        case 1024: return launch_rows<512, false>(a, stream);
+        case 1025: return launch_rows<512, true>(a, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <int D>
+hipError_t launch_join_of(const AttnArgs& a, hipStream_t stream) {
     const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
     constexpr int per = 256 / (D / 4);
-    join_kernel<D><<<(unsigned)((rows + per - 1) / per), 256, 0, stream>>>(a, FP8 ? a.pages.v_scale : 1.0f);
+    join_kernel<D><<<(unsigned)((rows + per - 1) / per), 256, 0, stream>>>(a, a.pages.fp8 ? a.pages.v_scale : 1.0f);
     return hipGetLastError();
+}
+hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
+    switch (a.pages.head_dim) {
+        case 64: return launch_join_of<64>(a, stream);
+        case 128: return launch_join_of<128>(a, stream);
+        case 256: return launch_join_of<256>(a, stream);
+        case 512: return launch_join_of<512>(a, stream);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 AttnPlan plan_attention(const AttnArgs& a) {
-    AttnPlan p{16, 1, 0, 0};
-    const Shape sh = tile_shape(16, a.q_heads / a.pages.kv_heads);
-    const int64_t wgs = ((int64_t)a.batch.tokens / sh.tokens + a.batch.requests) * a.pages.kv_heads * sh.chunks;
+    AttnPlan p{};
+    const int group = a.q_heads / a.pages.kv_heads;
+    const int64_t tokens = a.batch.tokens, requests = a.batch.requests;
+    const Shape wide = tile_shape(128, group), thin = tile_shape(16, group);
+    // A request goes to the 128-row tiles if it fills half of one.
+    const int from = ceil_div(64, wide.heads);
+    // One request: its kernel is known.  Several with a row each at least: none reaches
+    // `from` rows if the sum stays under this (were some of them empty, the 16-row kernel
+    // would still be right).
+    if (requests == 1)
+        p.tile_from = tokens >= from ? 1 : kNoTiles;
+    else
+        p.tile_from = tokens >= from + requests - 1 ? from : kNoTiles;
+    p.rows = p.tile_from > 1;
+    p.tiles = p.tile_from != kNoTiles;
+    const Shape& sh = p.tiles ? wide : thin;
+    const int64_t wgs = (tokens / sh.tokens + requests) * a.pages.kv_heads * sh.chunks;
     int64_t keys = (int64_t)a.batch.width << a.pages.page_shift;
     if (a.window > 0 && keys > a.window + sh.tokens) keys = a.window + sh.tokens;
-    // splits until the card has two workgroups per CU, each with 256 keys or more
-    int64_t splits = wgs > 0 ? 512 / wgs : 1;
+    // splits until the card has two workgroups per CU (of 128 rows: one), each with 256 keys or more
+    int64_t splits = wgs > 0 ? (p.tiles ? 256 : 512) / wgs : 1;
     if (splits > keys / 256) splits = keys / 256;
     if (splits > 128) splits = 128;
     if (splits < 1) splits = 1;
@@ -554,18 +443,11 @@ AttnPlan plan_attention(const AttnArgs& a) {
 }
 
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
-    (void)plan;
-    switch (a.pages.head_dim * 2 + a.pages.fp8) {
-        case 128: return launch<64, false>(a, stream);
-        case 129: return launch<64, true>(a, stream);
-        case 256: return launch<128, false>(a, stream);
-        case 257: return launch<128, true>(a, stream);
-        case 512: return launch<256, false>(a, stream);
-        case 513: return launch<256, true>(a, stream);
-        case 1024: return launch<512, false>(a, stream);
-        case 1025: return launch<512, true>(a, stream);
-    }
-    return hipErrorInvalidValue;
+    hipError_t e = hipSuccess;
+    if (plan.tiles) e = launch_tiles(a, stream);
+    if (e == hipSuccess && plan.rows) e = launch_rows16(a, stream);
+    if (e == hipSuccess && a.splits > 1) e = launch_join(a, stream);
+    return e;
 }
 
 }  // namespace kv

@@ -60,6 +60,7 @@ struct AttnArgs {
     Batch batch;
     int q_heads, window;
     float scale;
+    int tile_from;  // requests of this many rows or more go to the 128-row tiles, the rest to rows16
     // scratch of a split launch: [splits][tokens][q_heads] rows of head_dim, and their
     // running maximum and sum
     float* part_o;
@@ -67,14 +68,16 @@ struct AttnArgs {
     int splits;
 };
 
-// How a call is run: rows of a query tile (tokens x heads that share a KV head) and
-// splits of its key range.
+// How a call is run: which kernels, and splits of the key range.
+constexpr int kNoTiles = 0x40000000;  // more rows than any request has
 struct AttnPlan {
-    int rows;
+    bool tiles, rows;  // 128-row tiles; 16-row tiles
+    int tile_from;     // AttnArgs::tile_from
     int splits;
     size_t o_bytes, ml_bytes;
 };
 AttnPlan plan_attention(const AttnArgs& a);
+hipError_t launch_tiles(const AttnArgs& a, hipStream_t stream);  // kv_tile.hip
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream);
 
 }  // namespace kv

@@ -216,6 +216,7 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
             return unsupported(name, "tokens * q_heads exceeds 2^31");
         const kv::AttnPlan plan = kv::plan_attention(a);
         a.splits = plan.splits;
+        a.tile_from = plan.tile_from;
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
         hipError_t e = hipGetDevice(&sc.device);

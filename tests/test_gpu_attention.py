@@ -248,6 +248,17 @@ def test_prefill_tiles(gpu_lib, d, hq, hk, kind, q_len, kv_len, window):
     attend_case(np.random.default_rng(q_len), d, hq, hk, [q_len], [kv_len], 64, kind, window=window)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("d,hq,hk", [(64, 8, 2), (128, 12, 4), (256, 16, 8), (512, 16, 1)])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_chunks_far_into_their_contexts(gpu_lib, d, hq, hk, kind, window):
+    """Chunks whose keys take many tiles and several rounds of table entries, beside single
+    tokens; and one request alone."""
+    rng = np.random.default_rng(d + window)
+    attend_case(rng, d, hq, hk, [70, 1, 0, 9, 1], [3100, 2500, 7, 2049, 1], 16, kind, window=window, padding=1)
+    attend_case(rng, d, hq, hk, [67], [4500], 32, kind, window=window, spread=4.0)
+
+
 @pytest.mark.parametrize("page", [16, 64, 256, 1024])
 @pytest.mark.parametrize("layout", ["phsd", "pshd"])
 def test_pages(gpu_lib, page, layout):
