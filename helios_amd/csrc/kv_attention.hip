@@ -31,6 +31,10 @@ namespace kv {
 namespace {
 
 constexpr int kWaves = 4;
+
+// Workgroups of rows16 that run at once: one per CU at head_dim 512 (registers), else two.
+int rows_fill(const AttnArgs& a) { return a.pages.head_dim == 512 ? 256 : 512; }
+
 template <int D, bool FP8>
 struct Rows16 {
     static constexpr int kElt = FP8 ? 1 : 2;
@@ -43,7 +47,7 @@ struct Rows16 {
 };
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(AttnArgs a, Items it) {
     using C = Rows16<D, FP8>;
     constexpr int NG = C::kGroups;
     constexpr int kTileKeys = NG * kGroupKeys;
@@ -55,14 +59,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int group = a.q_heads / a.pages.kv_heads;
-    const Shape sh = tile_shape(16, group);
-    const int per_tile = a.pages.kv_heads * sh.chunks;
-    const int split = (int)blockIdx.y;
-    const int tile_no = (int)blockIdx.x / per_tile;
-    const int part = (int)blockIdx.x - tile_no * per_tile;
+    const Shape sh = tile_shape(kThinRows, group);
+    const int item = (int)blockIdx.x / it.parts;
+    const int part = (int)blockIdx.x - item * it.parts;
     const int kv_head = part / sh.chunks, chunk = part - kv_head * sh.chunks;
 
-    const Tile t = find_tile(a.batch, tile_no, sh.tokens, 1, a.tile_from - 1, lane);
+    const Tile t = find_item<false>(a.batch, a.pages.page_shift, rows_cuts(a, it, sh), item, lane);
     if (t.n <= 0) return;
     const int kv_len = clampi(t.kv_len, 0, a.batch.width << a.pages.page_shift);
 
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     const KeyRange keys = visible_keys(t.pos0, t.n, kv_len, a.window);
     const int lo = keys.lo & ~(kGroupKeys - 1);
     const int tiles = keys.hi > lo ? ceil_div(keys.hi - lo, kTileKeys) : 0;
-    const TileRange range = split_tiles(tiles, split, a.splits, kWaves);
+    const TileRange range = split_tiles(tiles, t.split, t.splits, 1);
     const int* table = a.batch.tables + (int64_t)t.request * a.batch.stride;
     const float c = a.scale * (FP8 ? a.pages.k_scale : 1.0f) * kLog2e;
     const uint32_t row_bytes = (uint32_t)a.pages.token_stride * C::kElt;
@@ -275,11 +277,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     if (wave == 1) put(0);
     __syncthreads();
     const int64_t out_row = (int64_t)row * a.q_heads + q_head;
-    const int64_t part_row = (int64_t)split * a.batch.tokens * a.q_heads;
+    const int64_t slot = (int64_t)blockIdx.x * kThinRows;  // rows of this item's partial sums
     if (wave == 0) {
         add(0);
         if (live) {
-            if (a.splits == 1) {
+            if (t.splits == 1) {
                 const float norm = total > 0.0f || total != total ? (FP8 ? a.pages.v_scale : 1.0f) / total : 0.0f;
                 uint16_t* op = a.out + (int64_t)row * a.out_stride + (int64_t)q_head * D;
 #pragma unroll
@@ -295,9 +297,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
                         }
                 if (a.lse != nullptr && g == 0) a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
             } else {
-                if (g == 0) a.part_ml[part_row + out_row] = make_float2(top, total);
+                if (g == 0) it.part_ml[slot + n] = make_float2(top, total);
                 if (top != kNegInf || total != 0.0f) {
-                    float* op = a.part_o + (part_row + out_row) * D;
+                    float* op = it.part_o + (slot + n) * D;
 #pragma unroll
                     for (int b = 0; b < C::kBlocks; ++b)
 #pragma unroll
@@ -323,87 +325,133 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
             if (ig >= group) return;
             const int64_t rr = t.row0 + i;
             const int qh = kv_head * group + ig;
-            if (a.splits == 1) {
+            if (t.splits == 1) {
                 uint16_t* op = a.out + rr * a.out_stride + (int64_t)qh * D + d;
                 *op = q4::f32_to_bf16(__uint_as_float((uint32_t)*op << 16) + v);
             } else {
-                float* op = a.part_o + (part_row + rr * a.q_heads + qh) * D + d;
+                float* op = it.part_o + (slot + i * sh.heads + h) * D + d;
                 *op += v;
             }
         });
     }
 }
 
-// Joins the splits of each output row, in split order: one wave per row and 64 D/64 lanes.
+// Joins the items of each tile that has several.  A workgroup takes rows of a tile in slices
+// of 128 dims (all of a smaller head): 32 lanes (D / 4) of four dims each, a group of lanes
+// per item, the groups' sums meeting in LDS; always in the same order.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, float v_scale) {
-    constexpr int kLanes = D / 4;  // four values each
-    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
-    const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + (int)threadIdx.x / kLanes;
-    const int d = 4 * ((int)threadIdx.x % kLanes);
-    if (row >= rows) return;
-    float top = kNegInf;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * rows + row].x);
-    const float base = top == kNegInf ? 0.0f : top;
-    float total = 0.0f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * rows + row];
-        if (ml.x == kNegInf && ml.y == 0.0f) continue;
-        const float w = exp2_hw(ml.x - base);
-        total += ml.y * w;
-        o += *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * D + d) * w;
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cuts, int rows) {
+    constexpr int kSlice = D < 128 ? D : 128, kLanes = kSlice / 4, kSets = 256 / kLanes;
+    __shared__ f32x4 sums[kSets][kLanes];
+    __shared__ float totals[kSets];
+    const int lane = (int)threadIdx.x & 63;
+    const int set = (int)threadIdx.x / kLanes, d4 = 4 * ((int)threadIdx.x % kLanes);
+    const int group = a.q_heads / a.pages.kv_heads;
+    const Shape sh = tile_shape(rows, group);
+    const int tile_no = (int)blockIdx.x / it.parts;
+    const int part = (int)blockIdx.x - tile_no * it.parts;
+    const int kv_head = part / sh.chunks, chunk = part - kv_head * sh.chunks;
+    const Tile t = find_item<true>(a.batch, a.pages.page_shift, cuts, tile_no, lane);
+    if (t.n <= 0 || t.splits < 2 || t.first_item < 0 || t.first_item + t.splits > it.items) return;
+    const float v_scale = a.pages.fp8 ? a.pages.v_scale : 1.0f;
+    const int64_t step = (int64_t)it.parts * rows;  // partial rows from one item to the next
+    for (int w = (int)blockIdx.y; w < t.n * sh.heads * (D / kSlice); w += (int)gridDim.y) {
+        const int r = w / (D / kSlice), d = (w % (D / kSlice)) * kSlice + d4;
+        const int tok = r / sh.heads, in_group = chunk * sh.heads + r - tok * sh.heads;
+        if (in_group >= group) continue;
+        const int64_t first = ((int64_t)t.first_item * it.parts + part) * rows + r;
+        float top = kNegInf;
+        for (int s = lane; s < t.splits; s += 64) top = fmaxf(top, it.part_ml[first + s * step].x);
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float base = top == kNegInf ? 0.0f : top;
+        float total = 0.0f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = set; s < t.splits; s += kSets) {
+            const float2 ml = it.part_ml[first + s * step];
+            const f32x4 v = *reinterpret_cast<const f32x4*>(it.part_o + (first + s * step) * D + d);
+            const bool any = ml.x != kNegInf || ml.y != 0.0f;  // else the item left nothing there
+            const float e = __builtin_amdgcn_exp2f(ml.x - base);
+            total += any ? ml.y * e : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += any ? v[i] * e : 0.0f;
+        }
+        __syncthreads();  // the sums of the row before are read
+        sums[set][d4 / 4] = o;
+        if (d4 == 0) totals[set] = total;
+        __syncthreads();
+        if (set == 0) {
+            for (int s = 1; s < kSets; ++s) {
+                o += sums[s][d4 / 4];
+                total += totals[s];
+            }
+            const float norm = total > 0.0f || total != total ? v_scale / total : 0.0f;
+            const int64_t row = t.row0 + tok;
+            const int head = kv_head * group + in_group;
+            *reinterpret_cast<u32x2*>(a.out + row * a.out_stride + (int64_t)head * D + d) =
+                u32x2{pack_bf16(o[0] * norm, o[1] * norm), pack_bf16(o[2] * norm, o[3] * norm)};
+            if (a.lse != nullptr && d == 0) a.lse[row * a.q_heads + head] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+        }
     }
-    const float norm = total > 0.0f || total != total ? v_scale / total : 0.0f;
-    const int64_t tok = row / a.q_heads;
-    const int head = (int)(row - tok * a.q_heads);
-    u32x2 w;
-    w.x = pack_bf16(o[0] * norm, o[1] * norm);
-    w.y = pack_bf16(o[2] * norm, o[3] * norm);
-    *reinterpret_cast<u32x2*>(a.out + tok * a.out_stride + (int64_t)head * D + d) = w;
-    if (a.lse != nullptr && d == 0) a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 template <int D, bool FP8>
-hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
-    const Shape sh = tile_shape(16, a.q_heads / a.pages.kv_heads);
-    // requests of tile_from rows or more are not this kernel's
-    const int64_t all = a.batch.tokens / sh.tokens + a.batch.requests + 1;
-    const int64_t small = (int64_t)(a.batch.requests + 1) * ceil_div(a.tile_from - 1, sh.tokens);
-    const unsigned tiles = (unsigned)(all < small ? all : small);
-    rows16_kernel<D, FP8><<<dim3(tiles * (unsigned)(a.pages.kv_heads * sh.chunks), (unsigned)a.splits), 64 * kWaves, 0, stream>>>(a);
+hipError_t launch_rows(const AttnArgs& a, const Items& it, hipStream_t stream) {
+    rows16_kernel<D, FP8><<<(unsigned)it.items * (unsigned)it.parts, 64 * kWaves, 0, stream>>>(a, it);
     return hipGetLastError();
 }
 
-hipError_t launch_rows16(const AttnArgs& a, hipStream_t stream) {
+hipError_t launch_rows16(const AttnArgs& a, const Items& it, hipStream_t stream) {
     switch (a.pages.head_dim * 2 + a.pages.fp8) {
-        case 128: return launch_rows<64, false>(a, stream);
-        case 129: return launch_rows<64, true>(a, stream);
-        case 256: return launch_rows<128, false>(a, stream);
-        case 257: return launch_rows<128, true>(a, stream);
-        case 512: return launch_rows<256, false>(a, stream);
-        case 513: return launch_rows<256, true>(a, stream);
-        case 1024: return launch_rows<512, false>(a, stream);
-        case 1025: return launch_rows<512, true>(a, stream);
+        case 128: return launch_rows<64, false>(a, it, stream);
+        case 129: return launch_rows<64, true>(a, it, stream);
+        case 256: return launch_rows<128, false>(a, it, stream);
+        case 257: return launch_rows<128, true>(a, it, stream);
+        case 512: return launch_rows<256, false>(a, it, stream);
+        case 513: return launch_rows<256, true>(a, it, stream);
+        case 1024: return launch_rows<512, false>(a, it, stream);
+        case 1025: return launch_rows<512, true>(a, it, stream);
     }
     return hipErrorInvalidValue;
 }
 
-template <int D>
-hipError_t launch_join_of(const AttnArgs& a, hipStream_t stream) {
-    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
-    constexpr int per = 256 / (D / 4);
-    join_kernel<D><<<(unsigned)((rows + per - 1) / per), 256, 0, stream>>>(a, a.pages.fp8 ? a.pages.v_scale : 1.0f);
+hipError_t launch_join(const AttnArgs& a, const Items& it, const Cuts& cuts, int rows, hipStream_t stream) {
+    if (it.slots == 0) return hipSuccess;
+    const int tiles = (it.items - it.slots) * it.parts;
+    const int work = rows * (a.pages.head_dim > 128 ? a.pages.head_dim / 128 : 1);
+    int y = ceil_div(2048, tiles);
+    y = y > work ? work : y;
+    const dim3 grid((unsigned)tiles, (unsigned)y);
+    switch (a.pages.head_dim) {
+        case 64: join_kernel<64><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
+        case 128: join_kernel<128><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
+        case 256: join_kernel<256><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
+        case 512: join_kernel<512><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
+        default: return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
-hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
-    switch (a.pages.head_dim) {
-        case 64: return launch_join_of<64>(a, stream);
-        case 128: return launch_join_of<128>(a, stream);
-        case 256: return launch_join_of<256>(a, stream);
-        case 512: return launch_join_of<512>(a, stream);
-    }
-    return hipErrorInvalidValue;
+
+// The most tiles of `tokens` rows that runs of least..most rows can make (the padding is a run too).
+int most_tiles(const AttnArgs& a, int tokens, int least, int most) {
+    const int64_t runs = (int64_t)a.batch.requests + 1, fit = a.batch.tokens / least;
+    const int64_t by_rows = a.batch.tokens / tokens + (fit < runs ? fit : runs);
+    const int64_t by_runs = runs * ((most < a.batch.tokens ? most : a.batch.tokens) / tokens + 1);
+    return (int)(by_rows < by_runs ? by_rows : by_runs);
+}
+
+// Items of a kernel's rows: `fill` workgroups fill the card.  No cuts where the tiles alone
+// fill it, or where no tile has keys for two items of `least_keys`.
+Items plan_items(const AttnArgs& a, const Shape& sh, int tiles, int fill, int least_keys) {
+    Items it{};
+    it.parts = a.pages.kv_heads * sh.chunks;
+    int64_t keys = (int64_t)a.batch.width << a.pages.page_shift;
+    if (a.window > 0 && keys > a.window + sh.tokens) keys = a.window + sh.tokens;
+    const int slots = fill / it.parts;
+    it.slots = tiles < slots && keys >= 2 * least_keys ? slots : 0;
+    it.items = it.slots + tiles;
+    return it;
 }
 
 }  // namespace
@@ -412,7 +460,7 @@ AttnPlan plan_attention(const AttnArgs& a) {
     AttnPlan p{};
     const int group = a.q_heads / a.pages.kv_heads;
     const int64_t tokens = a.batch.tokens, requests = a.batch.requests;
-    const Shape wide = tile_shape(128, group), thin = tile_shape(16, group);
+    const Shape wide = tile_shape(kWideRows, group), thin = tile_shape(kThinRows, group);
     // A request goes to the 128-row tiles if it fills half of one.
     const int from = ceil_div(64, wide.heads);
     // One request: its kernel is known.  Several with a row each at least: none reaches
@@ -422,31 +470,22 @@ AttnPlan plan_attention(const AttnArgs& a) {
         p.tile_from = tokens >= from ? 1 : kNoTiles;
     else
         p.tile_from = tokens >= from + requests - 1 ? from : kNoTiles;
-    p.rows = p.tile_from > 1;
-    p.tiles = p.tile_from != kNoTiles;
-    const Shape& sh = p.tiles ? wide : thin;
-    const int64_t wgs = (tokens / sh.tokens + requests) * a.pages.kv_heads * sh.chunks;
-    int64_t keys = (int64_t)a.batch.width << a.pages.page_shift;
-    if (a.window > 0 && keys > a.window + sh.tokens) keys = a.window + sh.tokens;
-    // splits until the card has two workgroups per CU (of 128 rows: one), each with 256 keys or more
-    int64_t splits = wgs > 0 ? (p.tiles ? 256 : 512) / wgs : 1;
-    if (splits > keys / 256) splits = keys / 256;
-    if (splits > 128) splits = 128;
-    if (splits < 1) splits = 1;
-    p.splits = (int)splits;
-    if (p.splits > 1) {
-        const size_t rows = (size_t)p.splits * a.batch.tokens * a.q_heads;
-        p.o_bytes = rows * a.pages.head_dim * 4;
-        p.ml_bytes = rows * sizeof(float2);
-    }
+    p.use_rows = p.tile_from > 1;
+    p.use_tiles = p.tile_from != kNoTiles;
+    if (p.use_tiles) p.tiles = plan_items(a, wide, most_tiles(a, wide.tokens, p.tile_from, kNoTiles), kTileFill, kTileLeast);
+    if (p.use_rows) p.rows = plan_items(a, thin, most_tiles(a, thin.tokens, 1, p.tile_from - 1), rows_fill(a), kRowsLeast);
     return p;
 }
 
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
+    const int group = a.q_heads / a.pages.kv_heads;
     hipError_t e = hipSuccess;
-    if (plan.tiles) e = launch_tiles(a, stream);
-    if (e == hipSuccess && plan.rows) e = launch_rows16(a, stream);
-    if (e == hipSuccess && a.splits > 1) e = launch_join(a, stream);
+    if (plan.use_tiles) e = launch_tiles(a, plan.tiles, stream);
+    if (plan.use_rows && e == hipSuccess) e = launch_rows16(a, plan.rows, stream);
+    if (plan.use_tiles && e == hipSuccess)
+        e = launch_join(a, plan.tiles, tile_cuts(a, plan.tiles, tile_shape(kWideRows, group)), kWideRows, stream);
+    if (plan.use_rows && e == hipSuccess)
+        e = launch_join(a, plan.rows, rows_cuts(a, plan.rows, tile_shape(kThinRows, group)), kThinRows, stream);
     return e;
 }
 

@@ -68,50 +68,135 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
     return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
 }
 
-// A query tile: `n` consecutive rows of q from `row0`, at positions pos0.. of `request`.
+// Inclusive sum over the lanes of a wave (row shifts of 1, 2, 4, 8, then the rows' last
+// lanes to the rows after them).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+template <int DPP, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), DPP, ROWS, 0xf, ROWS == 0xf));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
+    v = dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ int wave_max(int v) {
+    const auto at_least = [](int a, int b) { return a > b ? a : b; };
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));
+    v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// A query tile: `n` consecutive rows of q from `row0`, at positions pos0.. of `request`; its
+// keys are cut into `splits` parts, of which this is `split`; part s is item first_item + s.
 struct Tile {
     int request, row0, n, pos0, kv_len;
+    int split, splits, first_item;
 };
 
-// Tile number `tile` of the batch when the rows of every request that has from `least` to
-// `most` of them are cut into runs of `tokens`; n = 0 past the last.  All lanes of a wave
-// take part; the result is the same in all.
-__device__ __forceinline__ Tile find_tile(const Batch& b, int tile, int tokens, int least, int most, int lane) {
-    int before = 0;
-    for (int base = 0; base <= b.requests; base += 64) {
+// What the tiles of a launch are: the requests that have from `least` to `most` rows, cut
+// into runs of `tokens`; their key ranges counted in units of `unit` keys, and cut so that
+// there are about `slots` items (at most slots + the number of tiles; 0: no cuts).
+struct Cuts {
+    int tokens, least, most, unit, slots, min_units, window;
+};
+
+// Item number `index` of the launch, or (BY_TILE) its tile number `index` as split 0; n = 0
+// past the last.  The lengths are on the device only, so every workgroup finds the cuts
+// anew: C units to an item, from the sum and the maximum of the requests' units.  All lanes
+// of a wave take part; the result is the same in all.
+template <bool BY_TILE>
+__device__ __forceinline__ Tile find_item(const Batch& b, int page_shift, const Cuts& cuts, int index, int lane) {
+    struct Run {
+        int start, rows, len, tiles, units;
+    };
+    const auto load = [&](int base) {
         const int r = base + lane;
-        int s = 0, e = 0, len = 0;
+        Run run{0, 0, 0, 0, 0};
         if (r <= b.requests) {
-            s = run_bound(b.starts, r, b.requests, b.tokens);
-            e = run_bound(b.starts, r + 1, b.requests, b.tokens);
-            len = r < b.requests ? b.kv_lens[r] : 0;
+            run.start = run_bound(b.starts, r, b.requests, b.tokens);
+            const int end = run_bound(b.starts, r + 1, b.requests, b.tokens);
+            run.len = r < b.requests ? b.kv_lens[r] : 0;
+            run.rows = end - run.start >= cuts.least && end - run.start <= cuts.most ? end - run.start : 0;
         }
-        const int rows = e - s >= least && e - s <= most ? e - s : 0;
-        const int tiles = (rows + tokens - 1) / tokens;
-        int sum = tiles;  // inclusive sum over the lanes
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(sum, d);
-            sum += lane >= d ? o : 0;
+        run.tiles = (int)((uint32_t)(run.rows + cuts.tokens - 1) / (uint32_t)cuts.tokens);
+        int keys = clampi(run.len, 0, b.width << page_shift);
+        const int reach = cuts.window + (run.rows < cuts.tokens ? run.rows : cuts.tokens);
+        if (cuts.window > 0 && keys > reach) keys = reach;
+        run.units = run.rows > 0 ? (int)((uint32_t)(keys + cuts.unit - 1) / (uint32_t)cuts.unit) : 0;
+        if (run.units < 1) run.units = 1;
+        return run;
+    };
+    const auto parts = [](int units, int per) { return (int)((uint32_t)(units + per - 1) / (uint32_t)per); };
+    const Run head = load(0);
+    int per = 0x7fffffff >> 1;  // units of an item
+    if (cuts.slots > 0) {
+        float sum = 0.0f;
+        int tiles = 0, most = 0;
+        for (int base = 0; base <= b.requests; base += 64) {
+            const Run r = base == 0 ? head : load(base);
+            sum += wave_total((float)r.tiles * (float)r.units);
+            tiles += wave_total(r.tiles);
+            const int u = wave_max(r.tiles > 0 ? r.units : 0);
+            most = most > u ? most : u;
         }
-        const unsigned long long past = __ballot(before + sum > tile);
+        // all requests alike: as many parts of each as there are slots for; else an even share
+        const int alike = parts(most, tiles > 0 && tiles < cuts.slots ? cuts.slots / tiles : 1);
+        const int even = (int)fminf(sum * 1.0001f / (float)cuts.slots, 1.0e9f) + 1;
+        int items_alike = 0, items_even = 0;
+        for (int base = 0; base <= b.requests; base += 64) {
+            const Run r = base == 0 ? head : load(base);
+            items_alike += wave_total(r.tiles * parts(r.units, alike));
+            items_even += wave_total(r.tiles * parts(r.units, even));
+        }
+        const float cost_alike = (float)parts(items_alike, cuts.slots) * (float)alike;
+        per = (float)parts(items_even, cuts.slots) * (float)even < cost_alike ? even : alike;
+        if (per < cuts.min_units) per = cuts.min_units;
+    }
+    int before = 0, before_items = 0;
+    for (int base = 0; base <= b.requests; base += 64) {
+        const Run r = base == 0 ? head : load(base);
+        const int splits = parts(r.units, per);
+        const int sum = wave_scan(BY_TILE ? r.tiles : r.tiles * splits);
+        const unsigned long long past = __ballot(before + sum > index);
+        const int items = BY_TILE ? wave_scan(r.tiles * splits) : sum;
         if (past != 0) {
             const int at = __ffsll(past) - 1;
             Tile t;
             t.request = base + at;
-            const int first = before + __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at);
-            const int start = __builtin_amdgcn_readlane(s, at), count = __builtin_amdgcn_readlane(rows, at);
-            const int skip = (tile - first) * tokens;
+            const int tiles = __builtin_amdgcn_readlane(r.tiles, at);
+            t.splits = __builtin_amdgcn_readlane(splits, at);
+            const int own = BY_TILE ? tiles : tiles * t.splits;
+            const int nth = index - (before + __builtin_amdgcn_readlane(sum, at) - own);
+            const int tile = BY_TILE ? nth : (int)((uint32_t)nth / (uint32_t)t.splits);
+            t.split = BY_TILE ? 0 : nth - tile * t.splits;
+            t.first_item = before_items + __builtin_amdgcn_readlane(items, at) - tiles * t.splits + tile * t.splits;
+            if (tile < 0 || tile >= tiles) break;  // starts that are no starts: the sums have overflowed
+            const int start = __builtin_amdgcn_readlane(r.start, at), count = __builtin_amdgcn_readlane(r.rows, at);
+            const int skip = tile * cuts.tokens;
             t.row0 = start + skip;
-            t.n = count - skip < tokens ? count - skip : tokens;
-            const int kv = __builtin_amdgcn_readlane(len, at);
-            t.pos0 = kv - count + skip;
-            t.kv_len = kv;
+            t.n = count - skip < cuts.tokens ? count - skip : cuts.tokens;
+            t.kv_len = __builtin_amdgcn_readlane(r.len, at);
+            t.pos0 = t.kv_len - count + skip;
             return t;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
+        before_items += __builtin_amdgcn_readlane(items, 63);
     }
-    return Tile{0, 0, 0, 0, 0};
+    return Tile{0, 0, 0, 0, 0, 0, 1, 0};
 }
 
 // Tokens x heads of a query tile of ROWS rows: all of a KV head's query heads if they fit
@@ -125,6 +210,16 @@ __host__ __device__ inline Shape tile_shape(int rows, int group) {
     s.chunks = ceil_div(group, s.heads);
     s.tokens = rows / s.heads;
     return s;
+}
+
+// Units are what a workgroup takes in one step; an item is of 256 keys at least.
+constexpr int kRowsUnit = 64, kTileUnit = 32;
+constexpr int kRowsLeast = 256, kTileLeast = 256, kTileFill = 256;
+__host__ __device__ inline Cuts rows_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {
+    return Cuts{sh.tokens, 1, a.tile_from - 1, kRowsUnit, it.slots, kRowsLeast / kRowsUnit, a.window};
+}
+__host__ __device__ inline Cuts tile_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {
+    return Cuts{sh.tokens, a.tile_from, kNoTiles, kTileUnit, it.slots, kTileLeast / kTileUnit, a.window};
 }
 
 // Adds the infinities and NaN of groups that some row does not see to the outputs of the

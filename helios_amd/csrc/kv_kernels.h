@@ -61,23 +61,35 @@ struct AttnArgs {
     int q_heads, window;
     float scale;
     int tile_from;  // requests of this many rows or more go to the 128-row tiles, the rest to rows16
-    // scratch of a split launch: [splits][tokens][q_heads] rows of head_dim, and their
-    // running maximum and sum
-    float* part_o;
-    float2* part_ml;
-    int splits;
 };
 
-// How a call is run: which kernels, and splits of the key range.
+// How the rows of one kernel are cut into items (kv_device.h Cuts): `slots` items fill the
+// card (0: no cuts), `items` is the most there can be, each of `parts` KV heads' workgroups
+// (or runs of heads).  A tile of one item is stored by the kernel itself; the others leave
+// their rows' sums of e^(s - m) v in part_o [items][parts][rows][head_dim] and (m, sum of
+// e^(s - m)) in part_ml, to be joined by a second launch.
+struct Items {
+    int slots, items, parts;
+    float* part_o;
+    float2* part_ml;
+};
+
+// How a call is run: which kernels, and their items.
 constexpr int kNoTiles = 0x40000000;  // more rows than any request has
 struct AttnPlan {
-    bool tiles, rows;  // 128-row tiles; 16-row tiles
-    int tile_from;     // AttnArgs::tile_from
-    int splits;
-    size_t o_bytes, ml_bytes;
+    bool use_tiles, use_rows;  // 128-row tiles; 16-row tiles
+    int tile_from;             // AttnArgs::tile_from
+    Items tiles, rows;
+    size_t o_bytes(const Items& it, int rows_of, int head_dim) const {
+        return it.slots > 0 ? (((size_t)it.items * it.parts * rows_of * head_dim * 4 + 255) & ~(size_t)255) : 0;
+    }
+    size_t ml_bytes(const Items& it, int rows_of) const {
+        return it.slots > 0 ? (((size_t)it.items * it.parts * rows_of * sizeof(float2) + 255) & ~(size_t)255) : 0;
+    }
 };
+constexpr int kThinRows = 16, kWideRows = 128;
 AttnPlan plan_attention(const AttnArgs& a);
-hipError_t launch_tiles(const AttnArgs& a, hipStream_t stream);  // kv_tile.hip
+hipError_t launch_tiles(const AttnArgs& a, const Items& it, hipStream_t stream);  // kv_tile.hip
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream);
 
 }  // namespace kv

@@ -214,20 +214,24 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
         // a launch's workgroups are counted in 31 bits
         if (((uint64_t)batch->tokens + batch->requests + 1) * q_heads > 0x7FFFFFFFull)
             return unsupported(name, "tokens * q_heads exceeds 2^31");
-        const kv::AttnPlan plan = kv::plan_attention(a);
-        a.splits = plan.splits;
+        kv::AttnPlan plan = kv::plan_attention(a);
         a.tile_from = plan.tile_from;
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
         hipError_t e = hipGetDevice(&sc.device);
         if (e != hipSuccess) return hip_fail("gemma4_kv_attention: hipGetDevice", e);
-        const size_t o_bytes = (plan.o_bytes + 255) & ~(size_t)255;
+        const int d = a.pages.head_dim;
+        const size_t wide_o = plan.o_bytes(plan.tiles, kv::kWideRows, d), wide_ml = plan.ml_bytes(plan.tiles, kv::kWideRows);
+        const size_t thin_o = plan.o_bytes(plan.rows, kv::kThinRows, d), thin_ml = plan.ml_bytes(plan.rows, kv::kThinRows);
         void* ws = nullptr;
-        e = sc.take(o_bytes + plan.ml_bytes, &ws);
+        e = sc.take(wide_o + wide_ml + thin_o + thin_ml, &ws);
         if (e != hipSuccess)
             return fail(GEMMA4_ERR_MEMORY_GUARD, name + ": workspace allocation failed: " + hipGetErrorString(e));
-        a.part_o = static_cast<float*>(ws);
-        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + o_bytes);
+        char* at = static_cast<char*>(ws);
+        plan.tiles.part_o = reinterpret_cast<float*>(at);
+        plan.tiles.part_ml = reinterpret_cast<float2*>(at + wide_o);
+        plan.rows.part_o = reinterpret_cast<float*>(at + wide_o + wide_ml);
+        plan.rows.part_ml = reinterpret_cast<float2*>(at + wide_o + wide_ml + thin_o);
         e = kv::launch_attention(a, plan, sc.stream);
         const hipError_t er = sc.release();
         if (e != hipSuccess) return hip_fail("gemma4_kv_attention: launch", e);

@@ -140,7 +140,7 @@ struct TileShared {
 };
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, Items it) {
     using C = TileConf<D, FP8>;
     constexpr int E = C::kE, RG = C::kGroups;
     constexpr int kVBytes = E * C::kElt;
@@ -152,14 +152,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int group = a.q_heads / a.pages.kv_heads;
-    const Shape sh = tile_shape(128, group);
-    const int per_tile = a.pages.kv_heads * sh.chunks;
-    const int split = (int)blockIdx.y;
-    const int tile_no = (int)blockIdx.x / per_tile;
-    const int part = (int)blockIdx.x - tile_no * per_tile;
+    const Shape sh = tile_shape(kWideRows, group);
+    const int item = (int)blockIdx.x / it.parts;
+    const int part = (int)blockIdx.x - item * it.parts;
     const int kv_head = part / sh.chunks, chunk = part - kv_head * sh.chunks;
 
-    const Tile t = find_tile(a.batch, tile_no, sh.tokens, a.tile_from, 0x7fffffff, lane);
+    const Tile t = find_item<false>(a.batch, a.pages.page_shift, tile_cuts(a, it, sh), item, lane);
     if (t.n <= 0) return;
     const int kv_len = clampi(t.kv_len, 0, a.batch.width << a.pages.page_shift);
 
@@ -192,7 +190,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
     const KeyRange keys = visible_keys(t.pos0, t.n, kv_len, a.window);
     const int lo = keys.lo & ~(kTileKeys - 1);
     const int tiles = keys.hi > lo ? ceil_div(keys.hi - lo, kTileKeys) : 0;
-    const TileRange range = split_tiles(tiles, split, a.splits, 8);
+    const TileRange range = split_tiles(tiles, t.split, t.splits, 1);
     const int count = range.last - range.first;
     const int key0 = lo + range.first * kTileKeys;
     const int* table = a.batch.tables + (int64_t)t.request * a.batch.stride;
@@ -464,6 +462,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) mfma_settled(o[rg][e]);
 
+    const int64_t slot = (int64_t)blockIdx.x * kWideRows;  // rows of this item's partial sums
     // every row's maximum and sum, for the waves that hold its outputs
     l = half_sum(l);
     if (h == 0) {
@@ -471,8 +470,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
         sm.l[tile_row] = l;
         if (live) {
             const int64_t out_row = (int64_t)row * a.q_heads + q_head;
-            if (a.splits > 1)
-                a.part_ml[(int64_t)split * a.batch.tokens * a.q_heads + out_row] = make_float2(m, l);
+            if (t.splits > 1)
+                it.part_ml[slot + tile_row] = make_float2(m, l);
             else if (a.lse != nullptr)
                 a.lse[out_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
         }
@@ -480,7 +479,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
     if (lane == 0) sm.found[wave] = nonfinite;
     __syncthreads();
 
-    const int64_t part_row = (int64_t)split * a.batch.tokens * a.q_heads;
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
         const int r = 32 * (rg0 + rg) + n;
@@ -490,7 +488,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
         const int64_t orow = t.row0 + rtok;
         const int ohead = kv_head * group + rig;
         const int d0 = slice * C::kSliceDims + 4 * h * E;
-        if (a.splits == 1) {
+        if (t.splits == 1) {
             const float norm = total > 0.0f || total != total ? (FP8 ? a.pages.v_scale : 1.0f) / total : 0.0f;
             uint16_t* op = a.out + orow * a.out_stride + (int64_t)ohead * D + d0;
 #pragma unroll
@@ -507,7 +505,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
                     *reinterpret_cast<u32x4*>(op + 8 * b * E + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
             }
         } else if (sm.m[r] != kNegInf || total != 0.0f) {
-            float* op = a.part_o + (part_row + orow * a.q_heads + ohead) * D + d0;
+            float* op = it.part_o + (slot + r) * D + d0;
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -534,11 +532,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
             if (ig >= group) return;
             const int64_t rr = t.row0 + i;
             const int qh = kv_head * group + ig;
-            if (a.splits == 1) {
+            if (t.splits == 1) {
                 uint16_t* op = a.out + rr * a.out_stride + (int64_t)qh * D + d;
                 *op = q4::f32_to_bf16(__uint_as_float((uint32_t)*op << 16) + v);
             } else {
-                float* op = a.part_o + (part_row + rr * a.q_heads + qh) * D + d;
+                float* op = it.part_o + (slot + i * sh.heads + hd) * D + d;
                 *op += v;
             }
         });
@@ -546,28 +544,24 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a) {
 }
 
 template <int D, bool FP8>
-hipError_t launch(const AttnArgs& a, hipStream_t stream) {
-    const Shape sh = tile_shape(128, a.q_heads / a.pages.kv_heads);
-    // only requests of `tile_from` rows or more come here
-    const int64_t runs = a.batch.requests + 1, most = a.batch.tokens / a.tile_from;
-    const unsigned tiles = (unsigned)(a.batch.tokens / sh.tokens + (most < runs ? most : runs));
-    if (tiles == 0) return hipSuccess;
-    tile_kernel<D, FP8><<<dim3(tiles * (unsigned)(a.pages.kv_heads * sh.chunks), (unsigned)a.splits), 64 * kTileWaves, 0, stream>>>(a);
+hipError_t launch(const AttnArgs& a, const Items& it, hipStream_t stream) {
+    tile_kernel<D, FP8><<<(unsigned)it.items * (unsigned)it.parts, 64 * kTileWaves, 0, stream>>>(a, it);
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_tiles(const AttnArgs& a, hipStream_t stream) {
+hipError_t launch_tiles(const AttnArgs& a, const Items& it, hipStream_t stream) {
+    if (it.items == 0) return hipSuccess;
     switch (a.pages.head_dim * 2 + a.pages.fp8) {
-        case 128: return launch<64, false>(a, stream);
-        case 129: return launch<64, true>(a, stream);
-        case 256: return launch<128, false>(a, stream);
-        case 257: return launch<128, true>(a, stream);
-        case 512: return launch<256, false>(a, stream);
-        case 513: return launch<256, true>(a, stream);
-        case 1024: return launch<512, false>(a, stream);
-        case 1025: return launch<512, true>(a, stream);
+        case 128: return launch<64, false>(a, it, stream);
+        case 129: return launch<64, true>(a, it, stream);
+        case 256: return launch<128, false>(a, it, stream);
+        case 257: return launch<128, true>(a, it, stream);
+        case 512: return launch<256, false>(a, it, stream);
+        case 513: return launch<256, true>(a, it, stream);
+        case 1024: return launch<512, false>(a, it, stream);
+        case 1025: return launch<512, true>(a, it, stream);
     }
     return hipErrorInvalidValue;
 }

@@ -74,17 +74,21 @@ def attend(q, k_cache, v_cache, batch, scale, window=0):
     group = heads // k_cache.shape[1]
     out, bound = np.zeros_like(q), np.zeros_like(q)
     lse, lse_bound = np.full((rows, heads), -np.inf), np.zeros((rows, heads))
+    held = {}  # a request's present positions, and its keys and values
     for i, r, p in rows_of(batch):
         if r is None:
             continue
-        last = min(p, int(batch["kv_lens"][r]) - 1)
-        first = max(0, p - window + 1) if window else 0
-        where = [w for w in (slot_of(batch, r, j) for j in range(first, last + 1)) if w is not None]
-        if not where:
+        if r not in held:
+            at = [(j, slot_of(batch, r, j)) for j in range(int(batch["kv_lens"][r]))]
+            at = [(j, *w) for j, w in at if w is not None]
+            places, pages, slots = (np.array(w, np.int64) for w in zip(*at)) if at else (np.zeros(0, np.int64),) * 3
+            held[r] = places, [(k_cache[pages, h, slots], v_cache[pages, h, slots]) for h in range(k_cache.shape[1])]
+        places, per_head = held[r]
+        a, e = np.searchsorted(places, [max(0, p - window + 1) if window else 0, p + 1])
+        if a >= e:
             continue
-        pages, slots = (np.array(w) for w in zip(*where))
         for h in range(heads):
-            k, v = k_cache[pages, h // group, slots], v_cache[pages, h // group, slots]
+            k, v = (x[a:e] for x in per_head[h // group])
             s = scale * (k @ q[i, h])
             top = s.max()
             e = np.exp(s - top)

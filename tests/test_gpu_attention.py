@@ -259,6 +259,16 @@ def test_chunks_far_into_their_contexts(gpu_lib, d, hq, hk, kind, window):
     attend_case(rng, d, hq, hk, [67], [4500], 32, kind, window=window, spread=4.0)
 
 
+@pytest.mark.parametrize("d,hq,hk", [(64, 4, 2), (256, 4, 2), (512, 16, 1)])
+def test_many_requests(gpu_lib, d, hq, hk):
+    """More requests than a wave has lanes, of very different lengths and numbers of tokens."""
+    rng = np.random.default_rng(d)
+    q_lens = [int(v) for v in rng.choice([0, 1, 1, 1, 2, 5, 20], 150)] + [130, 1]
+    kv_lens = [a + int(rng.integers(0, 60)) for a in q_lens[:-1]] + [3001]
+    attend_case(rng, d, hq, hk, q_lens, kv_lens, 16, padding=4)
+    attend_case(rng, d, hq, hk, [1] * 70, [int(v) for v in rng.integers(1, 200, 69)] + [2600], 32, "e4m3")
+
+
 @pytest.mark.parametrize("page", [16, 64, 256, 1024])
 @pytest.mark.parametrize("layout", ["phsd", "pshd"])
 def test_pages(gpu_lib, page, layout):
