@@ -27,6 +27,7 @@ Errors surface as :class:`~helios_amd.qmm.Gemma4Error`; there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import qmm
 from .qmm import Gemma4Error, Status
@@ -57,6 +58,12 @@ class _Heads(ctypes.Structure):
                 ("count", _u32), ("norm", _u32), ("eps", ctypes.c_float)]
 
 
+# _Batch and _Heads as bytes: packing takes a quarter of a ctypes structure's time, and these
+# two are made for every call (bytes pass as the pointers the calls declare)
+_pack_batch = struct.Struct("PPPIIII").pack
+_pack_heads = struct.Struct("PPPQQIIf4x").pack
+
+
 def _invalid(message: str):
     return Gemma4Error(Status.INVALID_ARGUMENT, message)
 
@@ -72,33 +79,32 @@ def _int32(t, what: str, dims: int):
 
 
 def _heads_tensor(t, what: str, head_dim: int | None = None):
-    """A [rows, heads, head_dim] bf16 tensor whose heads lie next to each other in a row."""
+    """The shape and row stride of a [rows, heads, head_dim] bf16 tensor whose heads lie next
+    to each other in a row."""
     import torch
 
     if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 3 or not t.is_cuda:
         raise _invalid(f"{what} must be a bfloat16 tensor [rows, heads, head_dim] on the GPU")
-    shape, stride = t.shape, t.stride()
-    if head_dim is not None and shape[2] != head_dim:
-        raise _invalid(f"{what} has head_dim {shape[2]}, expected {head_dim}")
-    if stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
+    shape = t.shape
+    rows, heads, dim = shape
+    row_stride, head_stride, one = t.stride()
+    if head_dim is not None and dim != head_dim:
+        raise _invalid(f"{what} has head_dim {dim}, expected {head_dim}")
+    if one != 1 or (heads > 1 and head_stride != dim):
         raise _invalid(f"{what} must have its heads contiguous within a row")
-    return t
-
-
-def _row_stride(t) -> int:
     # a single row's stride says nothing
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+    return shape, row_stride if rows > 1 else max(row_stride, heads * dim)
 
 
-def _on(device, *tensors):
-    """The stream to use on `device`; every tensor must live there."""
+def _on(index, *tensors):
+    """Every tensor must live on GPU `index`, which must be the current device."""
     import torch
 
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise _invalid("all tensors must be on one device")
-    if torch.cuda.current_device() != device.index:
-        raise _invalid(f"the tensors are on {device}, which is not the current device")
+    if torch.cuda.current_device() != index:
+        raise _invalid(f"the tensors are on cuda:{index}, which is not the current device")
 
 
 class Rope:
@@ -133,7 +139,8 @@ class HeadNorm:
             weight = weight.contiguous()
         self.weight = weight
         self.eps = float(eps)
-        self._ptr = None if weight is None else weight.data_ptr()
+        self.size = 0 if weight is None else weight.numel()
+        self._ptr = 0 if weight is None else weight.data_ptr()
 
 
 class KVBatch:
@@ -155,31 +162,35 @@ class KVBatch:
         if stride < width:
             raise _invalid("block_tables' rows overlap")
         self.requests = n
-        self._fields = (query_starts.data_ptr(), kv_lens.data_ptr(), block_tables.data_ptr(), n, width, stride)
+        self._device = kv_lens.get_device()
+        self._fields = (query_starts.data_ptr(), kv_lens.data_ptr(), block_tables.data_ptr(), n)
+        self._table = (width, stride)
+        self._packed = (-1, b"")
 
     def _struct(self, tokens: int):
-        # a struct per call: two threads may use one batch with different row counts
-        a, b, c, n, width, stride = self._fields
-        return ctypes.byref(_Batch(a, b, c, n, tokens, width, stride))
+        # replaced as a whole: two threads may use one batch with different row counts
+        packed = self._packed
+        if packed[0] != tokens:
+            packed = self._packed = (tokens, _pack_batch(*self._fields, tokens, *self._table))
+        return packed[1]
 
 
-def _heads(t, norm, out):
-    if norm is not None and norm.weight is not None and norm.weight.numel() != t.shape[2]:
-        raise _invalid(f"the norm's weight has {norm.weight.numel()} values, head_dim is {t.shape[2]}")
-    return ctypes.byref(_Heads(t.data_ptr(), None if out is None else out.data_ptr(), None if norm is None else norm._ptr,
-                               _row_stride(t), 0 if out is None else _row_stride(out), t.shape[1],
-                               0 if norm is None else 1, 0.0 if norm is None else norm.eps))
+def _heads(t, shape, stride, norm, out, out_stride):
+    if norm is None:
+        return _pack_heads(t.data_ptr(), out, 0, stride, out_stride, shape[1], 0, 0.0)
+    if norm.weight is not None and norm.size != shape[2]:
+        raise _invalid(f"the norm's weight has {norm.size} values, head_dim is {shape[2]}")
+    return _pack_heads(t.data_ptr(), out, norm._ptr, stride, out_stride, shape[1], 1, norm.eps)
 
 
-def _output(out, like, what: str):
-    import torch
-
+def _output(out, shape, like, what: str):
+    """(tensor, row stride) of an output of `shape`."""
     if out is None:
-        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
-    _heads_tensor(out, what)
-    if out.shape != like.shape:
+        return like.new_empty(shape), shape[1] * shape[2]
+    got, stride = _heads_tensor(out, what)
+    if got != shape:
         raise _invalid(f"{what} has the wrong shape")
-    return out
+    return out, stride
 
 
 def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=None, out_k=None, stream=None):
@@ -187,22 +198,29 @@ def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=Non
     None, of k, in one launch.  ``positions``: int32 [rows].  Returns (q, k) in new
     tensors, or in ``out_q`` and ``out_k`` (which may be q and k themselves)."""
     lib = qmm.load_library()
-    _heads_tensor(q, "q")
-    rows, _, head_dim = q.shape
+    shape, q_stride = _heads_tensor(q, "q")
+    rows, _, head_dim = shape
     if k is not None:
-        _heads_tensor(k, "k", head_dim)
-        if k.shape[0] != rows:
+        k_shape, k_stride = _heads_tensor(k, "k", head_dim)
+        if k_shape[0] != rows:
             raise _invalid("q and k must have the same rows")
     if rope is not None:
         _int32(positions, "positions", 1)
         if positions.shape[0] != rows:
             raise _invalid(f"positions must have {rows} entries")
-    _on(q.device, k, positions if rope is not None else None)
-    out_q = _output(out_q, q, "out_q")
-    out_k = None if k is None else _output(out_k, k, "out_k")
-    status = lib.gemma4_qk_norm_rope(_heads(q, q_norm, out_q), None if k is None else _heads(k, k_norm, out_k),
-                                     None if rope is None else rope._ref,
-                                     positions.data_ptr() if rope is not None else None, rows, head_dim,
+    else:
+        positions = None
+    out_q, out_stride = _output(out_q, shape, q, "out_q")
+    of_q = _heads(q, shape, q_stride, q_norm, out_q.data_ptr(), out_stride)
+    of_k = None
+    if k is not None:
+        out_k, out_stride = _output(out_k, k_shape, k, "out_k")
+        of_k = _heads(k, k_shape, k_stride, k_norm, out_k.data_ptr(), out_stride)
+    else:
+        out_k = None
+    _on(q.get_device(), k, positions, out_q, out_k)
+    status = lib.gemma4_qk_norm_rope(of_q, of_k, None if rope is None else rope._ref,
+                                     None if positions is None else positions.data_ptr(), rows, head_dim,
                                      qmm._stream_ptr(stream))
     if status != 0:
         qmm.check(status, lib)
@@ -234,6 +252,7 @@ class PagedKVCache:
         self.kv_heads, self.page_size, self.head_dim = k.shape[h], k.shape[s], k.shape[3]
         self.num_pages = k.shape[0]
         self.device = k.device
+        self._device = k.get_device()
         self._lib = qmm.load_library()
         # the stride of an axis of one says nothing
         strides = [k.stride(i) if k.shape[i] > 1 else self.head_dim for i in (0, s, h)]
@@ -256,23 +275,27 @@ class PagedKVCache:
         """Stores the batch's k and v [rows, kv_heads, head_dim]: k normed and rotated, v
         normed, each where given.  k and v may be the same tensor.  With q [rows, heads,
         head_dim] the same launch norms and rotates it; returns it (or None)."""
-        _heads_tensor(k, "k", self.head_dim)
-        _heads_tensor(v, "v", self.head_dim)
-        rows = k.shape[0]
-        if v.shape[0] != rows or k.shape[1] != self.kv_heads or v.shape[1] != self.kv_heads:
+        shape, k_stride = _heads_tensor(k, "k", self.head_dim)
+        v_shape, v_stride = (shape, k_stride) if v is k else _heads_tensor(v, "v", self.head_dim)
+        rows = shape[0]
+        if v_shape != shape or shape[1] != self.kv_heads:
             raise _invalid(f"k and v must be [rows, {self.kv_heads}, {self.head_dim}]")
+        of_q = None
         if q is not None:
-            _heads_tensor(q, "q", self.head_dim)
-            if q.shape[0] != rows:
+            q_shape, q_stride = _heads_tensor(q, "q", self.head_dim)
+            if q_shape[0] != rows:
                 raise _invalid("q, k and v must have the same rows")
-            out_q = _output(out_q, q, "out_q")
-        _on(self.device, k, v, q, batch.kv_lens)
-        status = self._lib.gemma4_kv_append(self._ref, batch._struct(rows), None if q is None else _heads(q, q_norm, out_q),
-                                            _heads(k, k_norm, None), _heads(v, v_norm, None),
+            out_q, out_stride = _output(out_q, q_shape, q, "out_q")
+            of_q = _heads(q, q_shape, q_stride, q_norm, out_q.data_ptr(), out_stride)
+        else:
+            out_q = None
+        _on(self._device, k, v, q, out_q, batch.kv_lens)
+        status = self._lib.gemma4_kv_append(self._ref, batch._struct(rows), of_q,
+                                            _heads(k, shape, k_stride, k_norm, 0, 0), _heads(v, v_shape, v_stride, v_norm, 0, 0),
                                             None if rope is None else rope._ref, qmm._stream_ptr(stream))
         if status != 0:
             qmm.check(status, self._lib)
-        return out_q if q is not None else None
+        return out_q
 
     def attend(self, q, batch: KVBatch, scale: float | None = None, window: int = 0, out=None, return_lse: bool = False,
                stream=None):
@@ -282,16 +305,16 @@ class PagedKVCache:
         zeros), and with ``return_lse`` also the log-sum-exp, float32 [rows, heads]."""
         import torch
 
-        _heads_tensor(q, "q", self.head_dim)
-        rows, heads, _ = q.shape
+        shape, q_stride = _heads_tensor(q, "q", self.head_dim)
+        rows, heads, _ = shape
         if window < 0:
             raise _invalid("window must be >= 0 (0: none)")
-        _on(self.device, q, batch.kv_lens)
-        out = _output(out, q, "out")
+        out, out_stride = _output(out, shape, q, "out")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
-        status = self._lib.gemma4_kv_attention(self._ref, batch._struct(rows), q.data_ptr(), _row_stride(q), heads,
+        _on(self._device, q, out, batch.kv_lens)
+        status = self._lib.gemma4_kv_attention(self._ref, batch._struct(rows), q.data_ptr(), q_stride, heads,
                                                self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                               _row_stride(out), None if lse is None else lse.data_ptr(),
+                                               out_stride, None if lse is None else lse.data_ptr(),
                                                qmm._stream_ptr(stream))
         if status != 0:
             qmm.check(status, self._lib)

@@ -47,12 +47,12 @@ DEVICE_FLAGS = [
 # MFMA results in arch VGPRs: the GEMM's fp32 accumulators are updated by VALU FMAs every
 # group, which cannot read AGPRs
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-# the 128-row attention tile keeps up to 256 accumulators that the VALU seldom touches
-AGPR_SOURCES = ()
+# the 128-row attention tile's step is one straight run of code: its loops must all unroll
+UNROLL_SOURCES = ("kv_tile.hip",)
 
 
 def device_flags(source: str) -> list:
-    return DEVICE_FLAGS + ([] if source in AGPR_SOURCES else VGPR_FORM)
+    return DEVICE_FLAGS + VGPR_FORM + (["-mllvm", "-pragma-unroll-threshold=1000000"] if source in UNROLL_SOURCES else [])
 
 
 def device_asm(source: str) -> str:

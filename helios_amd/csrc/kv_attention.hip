@@ -336,16 +336,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     }
 }
 
-// Joins the items of each tile that has several.  A workgroup takes rows of a tile in slices
-// of 128 dims (all of a smaller head): 32 lanes (D / 4) of four dims each, a group of lanes
-// per item, the groups' sums meeting in LDS; always in the same order.
+// Joins the items of each tile that has several; bound by the latency of its loads for few
+// rows and by their bytes for many.  Sixteen lanes of four dims take a slice of 64 dims of a
+// row.  Up to eight items are summed by one such group; more are dealt to the workgroup's
+// sixteen groups, whose sums meet in LDS.  Either way always in the same order.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cuts, int rows) {
-    constexpr int kSlice = D < 128 ? D : 128, kLanes = kSlice / 4, kSets = 256 / kLanes;
-    __shared__ f32x4 sums[kSets][kLanes];
+    constexpr int kSets = 16, kSlices = D / 64;
+    __shared__ f32x4 sums[kSets][16];
     __shared__ float totals[kSets];
     const int lane = (int)threadIdx.x & 63;
-    const int set = (int)threadIdx.x / kLanes, d4 = 4 * ((int)threadIdx.x % kLanes);
+    const int set = (int)threadIdx.x / 16, d4 = 4 * ((int)threadIdx.x % 16);
     const int group = a.q_heads / a.pages.kv_heads;
     const Shape sh = tile_shape(rows, group);
     const int tile_no = (int)blockIdx.x / it.parts;
@@ -355,23 +356,64 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cu
     if (t.n <= 0 || t.splits < 2 || t.first_item < 0 || t.first_item + t.splits > it.items) return;
     const float v_scale = a.pages.fp8 ? a.pages.v_scale : 1.0f;
     const int64_t step = (int64_t)it.parts * rows;  // partial rows from one item to the next
-    for (int w = (int)blockIdx.y; w < t.n * sh.heads * (D / kSlice); w += (int)gridDim.y) {
-        const int r = w / (D / kSlice), d = (w % (D / kSlice)) * kSlice + d4;
-        const int tok = r / sh.heads, in_group = chunk * sh.heads + r - tok * sh.heads;
-        if (in_group >= group) continue;
-        const int64_t first = ((int64_t)t.first_item * it.parts + part) * rows + r;
+    const int work = t.n * sh.heads * kSlices;
+    const int heads_here = group - chunk * sh.heads < sh.heads ? group - chunk * sh.heads : sh.heads;
+    const auto first_of = [&](int r) { return ((int64_t)t.first_item * it.parts + part) * rows + r; };
+    const auto store = [&](int r, int d, f32x4 o, float top, float total) {
+        const float norm = total > 0.0f || total != total ? v_scale / total : 0.0f;
+        const int tok = r / sh.heads;
+        const int64_t row = t.row0 + tok;
+        const int head = kv_head * group + chunk * sh.heads + r - tok * sh.heads;
+        *reinterpret_cast<u32x2*>(a.out + row * a.out_stride + (int64_t)head * D + d) =
+            u32x2{pack_bf16(o[0] * norm, o[1] * norm), pack_bf16(o[2] * norm, o[3] * norm)};
+        if (a.lse != nullptr && d == 0) a.lse[row * a.q_heads + head] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+    };
+
+    if (t.splits <= 8) {
+        for (int w = (int)blockIdx.y * kSets + set; w < work; w += (int)gridDim.y * kSets) {
+            const int r = w / kSlices, d = 64 * (w % kSlices) + d4;
+            if (r % sh.heads >= heads_here) continue;
+            const int64_t first = first_of(r);
+            float2 ml[8];
+            f32x4 v[8];
+            float top = kNegInf;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const int64_t at = first + (s < t.splits ? s : 0) * step;
+                ml[s] = it.part_ml[at];
+                v[s] = *reinterpret_cast<const f32x4*>(it.part_o + at * D + d);
+                top = fmaxf(top, ml[s].x);
+            }
+            const float base = top == kNegInf ? 0.0f : top;
+            float total = 0.0f;
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const bool any = s < t.splits && (ml[s].x != kNegInf || ml[s].y != 0.0f);  // else the item left nothing there
+                const float e = __builtin_amdgcn_exp2f(ml[s].x - base);
+                total += any ? ml[s].y * e : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += any ? v[s][i] * e : 0.0f;
+            }
+            store(r, d, o, top, total);
+        }
+        return;
+    }
+    for (int w = (int)blockIdx.y; w < work; w += (int)gridDim.y) {
+        const int r = w / kSlices, d = 64 * (w % kSlices) + d4;
+        if (r % sh.heads >= heads_here) continue;
+        const int64_t first = first_of(r);
         float top = kNegInf;
         for (int s = lane; s < t.splits; s += 64) top = fmaxf(top, it.part_ml[first + s * step].x);
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        top = wave_max(top);
         const float base = top == kNegInf ? 0.0f : top;
         float total = 0.0f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
         for (int s = set; s < t.splits; s += kSets) {
             const float2 ml = it.part_ml[first + s * step];
             const f32x4 v = *reinterpret_cast<const f32x4*>(it.part_o + (first + s * step) * D + d);
-            const bool any = ml.x != kNegInf || ml.y != 0.0f;  // else the item left nothing there
+            const bool any = ml.x != kNegInf || ml.y != 0.0f;
             const float e = __builtin_amdgcn_exp2f(ml.x - base);
             total += any ? ml.y * e : 0.0f;
 #pragma unroll
@@ -386,12 +428,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cu
                 o += sums[s][d4 / 4];
                 total += totals[s];
             }
-            const float norm = total > 0.0f || total != total ? v_scale / total : 0.0f;
-            const int64_t row = t.row0 + tok;
-            const int head = kv_head * group + in_group;
-            *reinterpret_cast<u32x2*>(a.out + row * a.out_stride + (int64_t)head * D + d) =
-                u32x2{pack_bf16(o[0] * norm, o[1] * norm), pack_bf16(o[2] * norm, o[3] * norm)};
-            if (a.lse != nullptr && d == 0) a.lse[row * a.q_heads + head] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+            store(r, d, o, top, total);
         }
     }
 }
@@ -419,8 +456,8 @@ hipError_t launch_rows16(const AttnArgs& a, const Items& it, hipStream_t stream)
 hipError_t launch_join(const AttnArgs& a, const Items& it, const Cuts& cuts, int rows, hipStream_t stream) {
     if (it.slots == 0) return hipSuccess;
     const int tiles = (it.items - it.slots) * it.parts;
-    const int work = rows * (a.pages.head_dim > 128 ? a.pages.head_dim / 128 : 1);
-    int y = ceil_div(2048, tiles);
+    const int work = rows * (a.pages.head_dim / 64);
+    int y = ceil_div(1024, tiles);  // enough workgroups to hide the loads' latency
     y = y > work ? work : y;
     const dim3 grid((unsigned)tiles, (unsigned)y);
     switch (a.pages.head_dim) {

@@ -36,7 +36,8 @@ __device__ __forceinline__ float col_sum(float v) {
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    return (uint32_t)q4::f32_to_bf16(a) | ((uint32_t)q4::f32_to_bf16(b) << 16);
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));  // one conversion of two
 }
 
 // Two e4m3 of a word as two bf16 (exact).
@@ -98,6 +99,16 @@ __device__ __forceinline__ int wave_max(int v) {
     v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));
     v = at_least(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
     return __builtin_amdgcn_readlane(v, 63);
+}
+
+template <int DPP, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), DPP, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(v))));
+    v = dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // A query tile: `n` consecutive rows of q from `row0`, at positions pos0.. of `request`; its

@@ -16,14 +16,14 @@ using namespace rt;
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-Gemma4Status bad(const std::string& name, const char* what) { return fail(GEMMA4_ERR_INVALID_ARGUMENT, name + ": " + what); }
-Gemma4Status unsupported(const std::string& name, const char* what) {
-    return fail(GEMMA4_ERR_UNSUPPORTED_CONFIG, name + ": " + what);
+Gemma4Status bad(const char* name, const char* what) { return fail(GEMMA4_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); }
+Gemma4Status unsupported(const char* name, const char* what) {
+    return fail(GEMMA4_ERR_UNSUPPORTED_CONFIG, std::string(name) + ": " + what);
 }
 
 bool head_dim_ok(uint32_t d) { return d == 64 || d == 128 || d == 256 || d == 512; }
 
-Gemma4Status check_pages(const Gemma4KvPages* p, const std::string& name, kv::Pages* out) {
+Gemma4Status check_pages(const Gemma4KvPages* p, const char* name, kv::Pages* out) {
     if (p == nullptr) return bad(name, "requires non-null pages");
     if (p->k_dev == nullptr || p->v_dev == nullptr) return bad(name, "requires non-null k and v pages");
     if (!head_dim_ok(p->head_dim)) return unsupported(name, "head_dim must be 64, 128, 256 or 512");
@@ -62,7 +62,7 @@ Gemma4Status check_pages(const Gemma4KvPages* p, const std::string& name, kv::Pa
     return GEMMA4_OK;
 }
 
-Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const std::string& name, kv::Batch* out) {
+Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const char* name, kv::Batch* out) {
     if (b == nullptr) return bad(name, "requires a non-null batch");
     if (b->requests == 0 || b->requests > (1u << 20)) return bad(name, "requests must be 1 to 2^20");
     if (b->tokens > (1u << 24)) return unsupported(name, "tokens exceeds 2^24");
@@ -84,7 +84,7 @@ Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const s
     return GEMMA4_OK;
 }
 
-Gemma4Status check_rope(const Gemma4Rope* r, uint32_t head_dim, const std::string& name, kv::Rope* out) {
+Gemma4Status check_rope(const Gemma4Rope* r, uint32_t head_dim, const char* name, kv::Rope* out) {
     *out = kv::Rope{nullptr, 0, 8};
     if (r == nullptr || r->pairs == 0) return GEMMA4_OK;
     if (r->inv_freq_dev == nullptr || !aligned(r->inv_freq_dev, 4)) return bad(name, "rope needs inv_freq, 4-byte aligned");
@@ -96,23 +96,23 @@ Gemma4Status check_rope(const Gemma4Rope* r, uint32_t head_dim, const std::strin
     return GEMMA4_OK;
 }
 
-Gemma4Status check_heads(const Gemma4Heads* h, uint32_t head_dim, bool has_out, const char* which, const std::string& name,
+Gemma4Status check_heads(const Gemma4Heads* h, uint32_t head_dim, bool has_out, const char* which, const char* name,
                          kv::Heads* out) {
-    const std::string at = name + ": " + which;
+    const auto at = [&](const char* what) { return std::string(name) + ": " + which + what; };
     if (h->x_dev == nullptr || (has_out && h->out_dev == nullptr))
-        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " requires non-null pointers");
+        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" requires non-null pointers"));
     if (!has_out && h->out_dev != nullptr)
-        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " goes to the cache: out_dev must be NULL");
-    if (h->count == 0 || h->count > 65536) return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " count must be 1 to 65536");
+        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" goes to the cache: out_dev must be NULL"));
+    if (h->count == 0 || h->count > 65536) return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" count must be 1 to 65536"));
     if (!aligned(h->x_dev, 16) || !aligned(h->out_dev, 16) || !aligned(h->weight_dev, 16) || h->x_stride % 8 != 0 ||
         h->out_stride % 8 != 0)
-        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " pointers and strides must be multiples of 16 bytes");
+        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" pointers and strides must be multiples of 16 bytes"));
     const uint64_t least = (uint64_t)h->count * head_dim, most = (uint64_t)1 << 32;
     if (h->x_stride < least || (has_out && h->out_stride < least) || h->x_stride > most || h->out_stride > most)
-        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " stride must hold count * head_dim elements (and at most 2^32)");
-    if (h->norm > 1) return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " norm must be 0 or 1");
+        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" stride must hold count * head_dim elements (and at most 2^32)"));
+    if (h->norm > 1) return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" norm must be 0 or 1"));
     if (h->norm == 1 && !(std::isfinite(h->eps) && h->eps >= 0))
-        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at + " eps must be finite and >= 0");
+        return fail(GEMMA4_ERR_INVALID_ARGUMENT, at(" eps must be finite and >= 0"));
     out->x = h->x_dev;
     out->out = has_out ? h->out_dev : nullptr;
     out->weight = h->norm ? h->weight_dev : nullptr;
@@ -131,7 +131,7 @@ extern "C" {
 Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Rope* rope,
                                  const int32_t* positions_dev, uint32_t rows, uint32_t head_dim, void* stream) {
     try {
-        const std::string name("gemma4_qk_norm_rope");
+        const char* const name = "gemma4_qk_norm_rope";
         kv::HeadArgs a{};
         if (q == nullptr) return bad(name, "requires non-null q");
         if (!head_dim_ok(head_dim)) return unsupported(name, "head_dim must be 64, 128, 256 or 512");
@@ -158,7 +158,7 @@ Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, con
 Gemma4Status gemma4_kv_append(const Gemma4KvPages* pages, const Gemma4KvBatch* batch, const Gemma4Heads* q,
                               const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream) {
     try {
-        const std::string name("gemma4_kv_append");
+        const char* const name = "gemma4_kv_append";
         kv::HeadArgs a{};
         Gemma4Status st = check_pages(pages, name, &a.pages);
         if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
@@ -187,7 +187,7 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
                                  uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
                                  uint64_t out_stride, float* lse_dev, void* stream) {
     try {
-        const std::string name("gemma4_kv_attention");
+        const char* const name = "gemma4_kv_attention";
         kv::AttnArgs a{};
         Gemma4Status st = check_pages(pages, name, &a.pages);
         if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
@@ -226,7 +226,7 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
         void* ws = nullptr;
         e = sc.take(wide_o + wide_ml + thin_o + thin_ml, &ws);
         if (e != hipSuccess)
-            return fail(GEMMA4_ERR_MEMORY_GUARD, name + ": workspace allocation failed: " + hipGetErrorString(e));
+            return fail(GEMMA4_ERR_MEMORY_GUARD, std::string(name) + ": workspace allocation failed: " + hipGetErrorString(e));
         char* at = static_cast<char*>(ws);
         plan.tiles.part_o = reinterpret_cast<float*>(at);
         plan.tiles.part_ml = reinterpret_cast<float2*>(at + wide_o);

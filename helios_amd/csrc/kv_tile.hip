@@ -19,9 +19,13 @@
 // every 32 rows: 156 B a cycle at the matrix cores' full rate (head_dim 512), where LDS
 // gives 128; this split asks for 98.
 //
-// One barrier per tile: before it tile i's weights are written and tile i + 1's scores are
-// computed from LDS (the softmax of tile i between their products); after it the DMA of
-// K tile i + 3 starts in the buffer just read, and the waves multiply tile i's weights by V.
+// One wave per SIMD has nobody to fill its waits, so a step mixes three tiles' work, one
+// barrier each: the products of tile i's V, those of tile i + 2's scores, and between every two
+// of them a share of tile i + 1's softmax, of the transposes, of the DMAs of K tile i + 3 and of
+// the loads of V tile i + 1.  (Scores first and V after them, in two blocks: 1095 us at 2048
+// tokens over 16384 keys, 16 heads of 512 over one; in turns of four products 1070; in turns of
+// one 982-1000 us, 1.05 PFLOP/s.)  Loads of V take 16 bytes a lane, two keys at once: the
+// vector memory path moves 64 B a cycle at best, and a wave that waits for it issues no products.
 // The running maximum of a row is raised only when a score exceeds it by 2^8: weights up to
 // 2^8 lose nothing in bf16 or in the fp32 sums, and the outputs (256 registers at head_dim
 // 512) are seldom rescaled.
@@ -64,30 +68,12 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// o[e] += av[e] x p for the E products of a row group, accumulators in AGPRs: with the builtin
-// the compiler keeps accumulators either all in VGPRs or, S among them, all in AGPRs, and
-// neither holds 256 of O beside the rest.  It sees no hazards in asm: the leading wait states
-// cover operands the VALU has just written, and mfma_settled() goes between these products
-// and the next VALU access to o.
-template <int E>
-__device__ __forceinline__ void mfma_acc(f32x16 (&o)[E], const u32x4 (&av)[E], u32x4 p) {
-    static_assert(E == 2 || E == 4, "two or four products");
-    if constexpr (E == 4) {
-        asm("s_nop 1\n\t"
-            "v_mfma_f32_32x32x16_bf16 %0, %4, %8, %0\n\t"
-            "v_mfma_f32_32x32x16_bf16 %1, %5, %8, %1\n\t"
-            "v_mfma_f32_32x32x16_bf16 %2, %6, %8, %2\n\t"
-            "v_mfma_f32_32x32x16_bf16 %3, %7, %8, %3"
-            : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3])
-            : "v"(av[0]), "v"(av[1]), "v"(av[2]), "v"(av[3]), "v"(p));
-    } else {
-        asm("s_nop 1\n\t"
-            "v_mfma_f32_32x32x16_bf16 %0, %2, %4, %0\n\t"
-            "v_mfma_f32_32x32x16_bf16 %1, %3, %4, %1\n\t"
-            "s_nop 1"
-            : "+a"(o[0]), "+a"(o[1])
-            : "v"(av[0]), "v"(av[1]), "v"(p));
-    }
+// o += a x p with the accumulators in AGPRs: with the builtin the compiler keeps accumulators
+// either all in VGPRs or, S among them, all in AGPRs, and neither holds 256 of O beside the
+// rest.  It sees no hazards in asm: the wait states cover operands that the VALU has just
+// written, and mfma_settled() goes between these products and the next VALU access to o.
+__device__ __forceinline__ void mfma_acc(f32x16& o, u32x4 a, u32x4 p) {
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
 }
 __device__ __forceinline__ void mfma_settled(f32x16& o) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o)); }
 
@@ -100,25 +86,51 @@ __device__ __forceinline__ float half_sum(float v) {
     return __uint_as_float(p.x) + __uint_as_float(p.y);
 }
 
-// The E values of one key a lane holds, as words (E * kElt = 2, 4 or 8 bytes).
+// The E values of one key a lane holds (E * kElt = 2, 4 or 8 bytes).
 template <int BYTES>
 struct VWords {
     static constexpr int kCount = BYTES == 8 ? 2 : 1;
     uint32_t w[kCount];
 };
+// A load of 2 BYTES a lane: 16 lanes take all dims of a slice of one key, the next 16 those of
+// another (the address unit takes as long for 8 bytes a lane as for 16).
 template <int BYTES>
-__device__ __forceinline__ VWords<BYTES> load_v(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
-    VWords<BYTES> v;
+struct VRaw {
+    static constexpr int kCount = BYTES == 8 ? 4 : (BYTES == 4 ? 2 : 1);
+    uint32_t w[kCount];
+};
+template <int BYTES>
+__device__ __forceinline__ VRaw<BYTES> load_v(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    VRaw<BYTES> v;
     if constexpr (BYTES == 2) {
-        v.w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)lane_off, (int)off, 0);
-    } else if constexpr (BYTES == 4) {
         v.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane_off, (int)off, 0);
-    } else {
+    } else if constexpr (BYTES == 4) {
         const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane_off, (int)off, 0);
         v.w[0] = t.x;
         v.w[1] = t.y;
+    } else {
+        const u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_off, (int)off, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.w[i] = t[i];
     }
     return v;
+}
+// The two keys of such a load: even rows of 16 lanes keep the first half of the dims of both,
+// odd rows the second.
+template <int BYTES>
+__device__ __forceinline__ void both_keys(const VRaw<BYTES>& raw, VWords<BYTES>& first, VWords<BYTES>& second) {
+    if constexpr (BYTES == 2) {
+        const u32x2 p = __builtin_amdgcn_permlane16_swap(raw.w[0] & 0xFFFFu, raw.w[0] >> 16, false, false);
+        first.w[0] = p.x;
+        second.w[0] = p.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) {
+            const u32x2 p = __builtin_amdgcn_permlane16_swap(raw.w[i], raw.w[BYTES / 4 + i], false, false);
+            first.w[i] = p.x;
+            second.w[i] = p.y;
+        }
+    }
 }
 
 // bf16 pair (dim E of key a, dim E of key b)
@@ -133,8 +145,9 @@ __device__ __forceinline__ uint32_t pair_of(const VWords<BYTES>& a, const VWords
 }
 
 struct TileShared {
-    float alpha[2][128];
-    uint32_t raised[2][kTileWaves];
+    float alpha[4][128];
+    uint32_t raised[4][kTileWaves];
+    int pos[128];
     float m[128], l[128];
     uint32_t found[kTileWaves];
 };
@@ -169,7 +182,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const int row = t.row0 + (live ? tok : 0);
     const int q_head = kv_head * group + (live ? in_group : 0);
     const int pos = live ? t.pos0 + tok : t.pos0;
-    const int above = a.window > 0 ? pos - a.window : -0x7fffffff;  // keys in (above, pos]
+    if (h == 0) sm.pos[tile_row] = pos;  // read by the row's own wave only
 
     // The scale's sign goes into Q, so that the largest product is the largest score.  A scale
     // of zero makes every score zero (or NaN) in Q already.
@@ -196,45 +209,52 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const int* table = a.batch.tables + (int64_t)t.request * a.batch.stride;
     const uint32_t row_bytes = (uint32_t)a.pages.token_stride * C::kElt;
 
-    // Pages of the 16-key groups of 32 tiles, one per lane: chunk j of 64 groups in page_at_[j & 1].
-    const auto fetch_pages = [&](int ch) {
-        const int g = 64 * ch + lane;
-        const int at = (key0 + g * kGroupKeys) >> a.pages.page_shift;
-        return g < 2 * count ? page_at(table, at, a.batch.width, a.pages.num_pages) : -1;
-    };
-    int pages_even = fetch_pages(0), pages_odd = fetch_pages(1);
-    const auto page_of = [&](int g) {
-        const int v = ((g >> 6) & 1) ? pages_odd : pages_even;
-        return __builtin_amdgcn_readlane(v, g & 63);
-    };
-    // bytes from this head's first page to the first of the 16 keys of group g
+    // Where the 16-key groups lie: lane i has group `window` + i's bytes from this head's first
+    // page, and its bit of `present` whether there is a page.  The window moves by 16 tiles; the
+    // pages of the next one are read 16 tiles ahead.
     const uint64_t page_bytes = (uint64_t)a.pages.page_stride * C::kElt;
     const int64_t head_bytes = (int64_t)kv_head * a.pages.head_stride * C::kElt;
     const char* const k_head = a.pages.k + head_bytes;
     const char* const v_head = a.pages.v + head_bytes;
-    const uint32_t slot_mask = (1u << a.pages.page_shift) - 1u;
+    const auto fetch_pages = [&](int first) {
+        const int g = first + lane;
+        return g < 2 * count ? page_at(table, (key0 + g * kGroupKeys) >> a.pages.page_shift, a.batch.width, a.pages.num_pages) : -1;
+    };
+    int window = 0, pages_next = 0;
+    uint64_t offsets = 0;
+    unsigned long long present = 0;
+    const auto move_window = [&](int first, int pages) {
+        window = first;
+        present = __ballot(pages >= 0);
+        const uint32_t slot = (uint32_t)(key0 + (first + lane) * kGroupKeys) & ((1u << a.pages.page_shift) - 1u);
+        offsets = (uint32_t)(pages < 0 ? 0 : pages) * page_bytes + (uint64_t)slot * row_bytes;
+    };
     const auto group_offset = [&](int g) {
-        const int page = page_of(g);
-        return (uint32_t)(page < 0 ? 0 : page) * page_bytes + (uint64_t)((uint32_t)(key0 + g * kGroupKeys) & slot_mask) * row_bytes;
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)offsets, g - window);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(offsets >> 32), g - window);
+        return ((uint64_t)hi << 32) | lo;
     };
 
     const uint32_t group_bytes = 15u * row_bytes + (uint32_t)C::kRowBytes;
-    // K tile `tl` into buffer tl & 1; each DMA brings kDmaKeys whole rows
-    const auto dma_k = [&](int tl) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));  // offsets are cheap to make again and dear to keep
-        const int dma_key = ln / C::kCpr, dma_chunk = ln & (C::kCpr - 1);
-#pragma unroll
-        for (int j = 0; j < (C::kDmas + kTileWaves - 1) / kTileWaves; ++j) {
-            const int d = wave * ((C::kDmas + kTileWaves - 1) / kTileWaves) + j;
-            if (C::kDmas >= kTileWaves || d < C::kDmas) {
-                const int first = d * C::kDmaKeys;  // key within the tile
-                const int g = 2 * tl + first / kGroupKeys;
-                const __amdgpu_buffer_rsrc_t r = q4::make_rsrc(k_head + group_offset(g), group_bytes);
-                const uint32_t voff = (uint32_t)dma_key * row_bytes + 16u * (uint32_t)(dma_chunk ^ swizzle<C::kCpr>(first + dma_key));
-                q4::dma16(r, &kbuf[tl & 1][d * 64], voff, (uint32_t)(first % kGroupKeys) * row_bytes);
-            }
-        }
+    // K tile `tl` into a buffer: each DMA brings kDmaKeys whole rows, a wave's lie in one group of
+    // 16 keys.  Past the last tile the resource is empty (the DMAs bring zeros).
+    constexpr int kWaveDmas = (C::kDmas + kTileWaves - 1) / kTileWaves;
+    const int first_dma = wave * kWaveDmas % C::kDmas, first_key = first_dma * C::kDmaKeys;
+    const auto k_source = [&](int tl) {
+        return q4::make_rsrc(k_head + group_offset(2 * tl + first_key / kGroupKeys), tl < count ? group_bytes : 0u);
+    };
+    const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)&kbuf[0][0];
+    // this lane's row among a DMA's and its chunk there; the DMA's first key adds its own bits
+    // (swizzle(key + i) = swizzle(key) ^ swizzle(i) for i < kDmaKeys)
+    const auto dma_k = [&](__amdgpu_buffer_rsrc_t r, uint32_t buffer, int j, int ln) {
+        const uint32_t dma_row = C::kDmaKeys == 1 ? 0u : ((uint32_t)ln / C::kCpr) * row_bytes;
+        const uint32_t dma_chunk = 16u * (((uint32_t)ln & (C::kCpr - 1)) ^ (C::kDmaKeys == 1 ? 0u : (uint32_t)swizzle<C::kCpr>(ln / C::kCpr)));
+        const int key = first_key + j * C::kDmaKeys;
+        uint32_t to = k_lds + (uint32_t)first_dma * 1024u, swz = 16u * (uint32_t)swizzle<C::kCpr>(first_key);
+        asm volatile("" : "+s"(to), "+s"(swz));  // sums are cheap to make again and dear to keep
+        swz = 16u * (uint32_t)swizzle<C::kCpr>(j * C::kDmaKeys) ^ swz;
+        q4::dma16_at(r, to + buffer * (uint32_t)C::kTileBytes + (uint32_t)j * 1024u, dma_row + (dma_chunk ^ swz),
+                     (uint32_t)(key % kGroupKeys) * row_bytes);
     };
 
     // This lane's reads of K: key n's chunk 2u + h, at its row + 16 ((2u + h) ^ swizzle(n)).  The
@@ -242,11 +262,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     // follow each other, so that few addresses are alive.
     constexpr int kUnits = C::kCpr / 2, kFar = C::kCpr > 16 ? C::kCpr / 16 : 1, kPer = FP8 ? 2 : 1;
     typedef const __attribute__((address_space(3))) u32x4* LdsPtr;
-    const uint32_t k_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)&kbuf[0][0] +
-                            (uint32_t)n * C::kRowBytes + 16u * (uint32_t)(h ^ swizzle<C::kCpr>(n));
+    const auto k_base = [&](int ln) {
+        return k_lds + (uint32_t)(ln & 31) * C::kRowBytes + 16u * (uint32_t)((ln >> 5) ^ swizzle<C::kCpr>(ln & 31));
+    };
     const auto unit_of = [](int i) { return i / kFar + 8 * (i % kFar); };
-    const auto read_k = [&](uint32_t base, int u) {
-        return *((LdsPtr)(uintptr_t)(base ^ (16u * (uint32_t)((2 * u) & 15))) + (2 * u) / 16 * 16);
+    const auto read_k = [&](uint32_t base, int buffer, int u) {
+        return *((LdsPtr)(uintptr_t)(base ^ (16u * (uint32_t)((2 * u) & 15))) + (2 * u) / 16 * 16 + buffer * (C::kTileBytes / 16));
     };
     // s += the products of unit u
     const auto product = [&](f32x16 s, int u, u32x4 raw) {
@@ -261,7 +282,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
 
     const int slice = wave % C::kSlices;
     const int rg0 = wave / C::kSlices * RG;  // first row group of this wave's outputs
-    const uint32_t v_lane = 4u * h * row_bytes + (uint32_t)((slice * C::kSliceDims + n * E) * C::kElt);
+    // lane (h, r = l / 16 % 2, m = l % 16) reads dims 2 E m .. of key 4h + r of a load's
+    const uint32_t v_lane = (uint32_t)(4 * h + ((lane >> 4) & 1)) * row_bytes + (uint32_t)((slice * C::kSliceDims + (lane & 15) * 2 * E) * C::kElt);
 
     f32x16 o[RG][E];
 #pragma unroll
@@ -271,33 +293,35 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     float m = kNegInf, l = 0.0f;
     bool nonfinite = false;
 
-    // The tile's scores in `s`: masks them, if some row does not see all of its keys, and
-    // raises the running maximum, if a score exceeds it by more than kSlack (the wave's sums
-    // here, the outputs when the weights are used).
-    struct Seen {
-        bool visible, there[2];
-    };
-    const auto seen_of = [&](int tl) {
-        Seen v;
-        v.visible = all_visible(key0 + tl * kTileKeys, kTileKeys, t.pos0, t.n, a.window);
-        v.there[0] = page_of(2 * tl) >= 0;
-        v.there[1] = page_of(2 * tl + 1) >= 0;
-        return v;
-    };
+    // whether every row of the tile sees all of tile tl's keys, and which groups have pages
+    const auto all_seen = [&](int tl) { return all_visible(key0 + tl * kTileKeys, kTileKeys, t.pos0, t.n, a.window); };
+    const auto pages_of = [&](int tl) { return (uint32_t)(present >> (2 * tl - window)) & 3u; };
     const auto top_of = [&](const f32x16& s) {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
         return half_max(top) * c;
     };
-    const auto settle = [&](int tl, f32x16& s, float top, const Seen& seen) {
-        if (!seen.visible || !seen.there[0] || !seen.there[1]) {
-            int first = key0 + tl * kTileKeys + 4 * h;
-            asm volatile("" : "+v"(first));
+    // Tile tl's scores in `s`: masks them, if some row does not see all of its keys (or there is
+    // no such tile), and raises the running maximum, if a score exceeds it by more than kSlack
+    // (the wave's sums here, the outputs when the weights are used).
+    const auto settle = [&](int tl, f32x16& s, float top) {
+        if (tl >= count) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = kNegInf;
+            return;
+        }
+        const uint32_t there = pages_of(tl);
+        if (!all_seen(tl) || there != 3u) {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const int pos = sm.pos[32 * wave + (ln & 31)];
+            const int above = a.window > 0 ? pos - a.window : -0x7fffffff;  // keys in (above, pos]
+            const int first = key0 + tl * kTileKeys + 4 * (ln >> 5);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = first + 8 * (i / 4) + i % 4;
-                s[i] = seen.there[i / 8] && key <= pos && key > above ? s[i] : kNegInf;
+                s[i] = (there >> (i / 8) & 1) && key <= pos && key > above ? s[i] : kNegInf;
             }
             top = top_of(s);
         }
@@ -307,155 +331,218 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
             const float alpha = __builtin_amdgcn_exp2f(m - (next == kNegInf ? 0.0f : next));
             m = next;
             l *= alpha;
-            if (h == 0) sm.alpha[tl & 1][tile_row] = alpha;
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            if (ln < 32) sm.alpha[tl & 3][32 * wave + ln] = alpha;
             raised = 1;
         }
-        if (lane == 0) sm.raised[tl & 1][wave] = raised;
+        if (lane == 0) sm.raised[tl & 3][wave] = raised;
     };
 
-    f32x16 s_cur = {};
-    Seen seen = {};
+    VRaw<kVBytes> v[2][4];  // a tile's V: this lane's dims of its keys in each group of 16
+    const auto v_source = [&](int g) { return q4::make_rsrc(v_head + group_offset(g), group_bytes); };
+    const auto fetch_v = [&](__amdgpu_buffer_rsrc_t r, int j) { return load_v<kVBytes>(r, v_lane, (uint32_t)(8 * (j / 2) + 2 * (j % 2)) * row_bytes); };
+
+    // Weight e of a tile's 16 (scores in `s`) is made when weight e - 1 is summed and packed.
+    float before = 0.0f, last = 0.0f;
+    uint32_t pk[4];
+    const auto weight_done = [&](int e, int par, int ln) {
+        if (e < 0) return;
+        l += last;
+        asm volatile("" : "+v"(l));  // here, between the products
+        if (e & 1) pk[e / 2 % 4] = pack_bf16(before, last);
+        if (e % 8 == 7) pbuf[par][wave][e / 8][ln] = u32x4{pk[0], pk[1], pk[2], pk[3]};
+    };
+    const auto weight = [&](int e, const f32x16& s, float base, int par, int ln) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -base));
+        weight_done(e - 1, par, ln);
+        before = last;
+        last = w;
+    };
+
+    f32x16 s2[2] = {};  // scores of an even and an odd tile
     if (count > 0) {
-        dma_k(0);
-        if (count > 1) dma_k(1);
+        const int pages = fetch_pages(0);
+        pages_next = fetch_pages(32);
+        move_window(0, pages);
+        const __amdgpu_buffer_rsrc_t k0 = k_source(0), k1 = k_source(1), k2 = k_source(2);
+#pragma unroll
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k0, 0, j, lane);
+#pragma unroll
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k1, 1, j, lane);
         q4::wait_vm_lds<0>();
         q4::lds_barrier();
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // or all reads move ahead, into registers Q needs
-            s_cur = product(s_cur, unit_of(i), read_k(k_base, unit_of(i)));
-        }
-        seen = seen_of(0);
-        settle(0, s_cur, top_of(s_cur), seen);
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // or all reads move ahead, into registers Q needs
+                s2[b] = product(s2[b], unit_of(i), read_k(k_base(lane), b, unit_of(i)));
+            }
+        settle(0, s2[0], top_of(s2[0]));
+        const float base = m == kNegInf ? 0.0f : m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) weight(e, s2[0], base, 0, lane);
+        weight_done(15, 0, lane);
+        settle(1, s2[1], top_of(s2[1]));
         q4::wait_lds();
         q4::lds_barrier();
-        if (count > 2) dma_k(2);
+#pragma unroll
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k2, 0, j, lane);
+        const __amdgpu_buffer_rsrc_t v0 = v_source(0), v1 = v_source(1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[0][j] = fetch_v(v0, j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[1][j] = fetch_v(v1, j);
     }
 
-    for (int tl = 0; tl < count; ++tl) {
-        if ((tl & 31) == 0 && tl > 0) {
-            if ((tl >> 5) & 1)
-                pages_even = fetch_pages((tl >> 5) + 1);
-            else
-                pages_odd = fetch_pages((tl >> 5) + 1);
-        }
-        const int par = tl & 1;
-        // The next tile's scores; between their products the loads of this tile's V and this
-        // tile's weights (the order is the source's: slices end in scheduling barriers).
-        VWords<kVBytes> v[2][8];
-        const __amdgpu_buffer_rsrc_t vr[2] = {q4::make_rsrc(v_head + group_offset(2 * tl), group_bytes),
-                                              q4::make_rsrc(v_head + group_offset(2 * tl + 1), group_bytes)};
-        f32x16 s_next = {};
-        const float base = m == kNegInf ? 0.0f : m;
-        float last = 0.0f;
-        u32x4 pk = {};
-        uint32_t kb = k_base + (uint32_t)((tl + 1) & 1) * (uint32_t)C::kTileBytes;
-        asm volatile("" : "+v"(kb));
-        constexpr int kAhead = kUnits < 4 ? kUnits : 4;
-        u32x4 kf[kAhead];
+    // Per tile tl: its weights are in LDS and its V is on the way, and the next tile's scores
+    // are in s2.  The products of its V, those of the scores of tile tl + 2, and the weights of
+    // tile tl + 1 take turns, so that neither the matrix cores nor LDS nor the VALU wait for
+    // the others for long.  The order is the source's: slices end in scheduling barriers.
+    constexpr int kSlices = 2 * RG, kPerSlice = kUnits / kSlices;
+    for (int pair = 0; pair < count; pair += 2) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) kf[i] = read_k(kb, unit_of(i));
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-            s_next = product(s_next, unit_of(i), kf[i % kAhead]);
-            if (i + kAhead < kUnits) kf[i % kAhead] = read_k(kb, unit_of(i + kAhead));
-#pragma unroll
-            for (int j = 16 * i / kUnits; j < 16 * (i + 1) / kUnits; ++j)
-                v[j / 8][j % 8] = load_v<kVBytes>(vr[j / 8], v_lane, (uint32_t)(8 * (j % 8 / 4) + j % 4) * row_bytes);
-#pragma unroll
-            for (int e = 16 * i / kUnits; e < 16 * (i + 1) / kUnits; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(s_cur[e], c, -base));
-                l += w;
-                if (e & 1)
-                    pk[e / 2 % 4] = pack_bf16(last, w);
-                last = w;
-                if (e % 8 == 7) pbuf[par][wave][e / 8][lane] = pk;
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int par = 0; par < 2; ++par) {
+            const int tl = pair + par;
+            if (tl >= count) break;
+            // K of tile tl + 2 has landed (its DMAs are older than the 8 loads of V) and the
+            // weights are written
+            q4::wait_vm_lds<8>();
+            q4::lds_barrier();
+            int ln = lane;
+            asm volatile("" : "+v"(ln));  // addresses made from it are made here, not kept
+            const uint32_t kb = k_base(ln);
 
-        // K of tile tl + 2 has landed (its DMAs are older than the 16 loads of V) and the
-        // weights are written
-        q4::wait_vm_lds<16>();
-        q4::lds_barrier();
-
-        if (!seen.visible || !seen.there[0] || !seen.there[1]) {
+            const uint32_t up = sm.raised[tl & 3][ln & (kTileWaves - 1)];
+            const uint32_t there = pages_of(tl);
+            if (!all_seen(tl) || there != 3u) {
+                const bool visible = all_seen(tl);
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                if (seen.visible && seen.there[st]) continue;
-                bool bad = false;
+                for (int st = 0; st < 2; ++st) {
+                    if (visible && (there >> st & 1)) continue;
+                    bool bad = false;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int w = 0; w < VWords<kVBytes>::kCount; ++w) bad |= any_nonfinite<FP8>(v[st][j].w[w]);
-                if (__any(bad)) {
-                    nonfinite = true;
+                        for (int w = 0; w < VRaw<kVBytes>::kCount; ++w) bad |= any_nonfinite<FP8>(v[st][j].w[w]);
+                    if (__any(bad)) {
+                        nonfinite = true;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int w = 0; w < VWords<kVBytes>::kCount; ++w) v[st][j].w[w] = finite_only<FP8>(v[st][j].w[w]);
-                }
-            }
-        }
-
-        const uint32_t up = sm.raised[par][lane & (kTileWaves - 1)];
-        if (__any(up != 0)) {
-#pragma unroll
-            for (int rg = 0; rg < RG; ++rg) {
-                if (__builtin_amdgcn_readlane(up, rg0 + rg) != 0) {
-                    const float f = sm.alpha[par][32 * (rg0 + rg) + n];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        mfma_settled(o[rg][e]);
-                        o[rg][e] *= f;
-                        mfma_settled(o[rg][e]);
-                        __builtin_amdgcn_sched_barrier(0);  // one at a time: they pass through VGPRs
+                            for (int w = 0; w < VRaw<kVBytes>::kCount; ++w) v[st][j].w[w] = finite_only<FP8>(v[st][j].w[w]);
                     }
                 }
             }
-        }
-
-        // this tile's products, the next one's maximum between them
-        const auto transposed = [&](int st, int j, u32x4 (&av)[E]) {
-            av[0][j] = pair_of<FP8, kVBytes, 0>(v[st][2 * j], v[st][2 * j + 1]);
-            av[1][j] = pair_of<FP8, kVBytes, 1>(v[st][2 * j], v[st][2 * j + 1]);
-            if constexpr (E == 4) {
-                av[2][j] = pair_of<FP8, kVBytes, 2>(v[st][2 * j], v[st][2 * j + 1]);
-                av[3][j] = pair_of<FP8, kVBytes, 3>(v[st][2 * j], v[st][2 * j + 1]);
+            if (__any(up != 0)) {
+#pragma unroll
+                for (int rg = 0; rg < RG; ++rg) {
+                    if (__builtin_amdgcn_readlane(up, rg0 + rg) != 0) {
+                        const float f = sm.alpha[tl & 3][32 * (rg0 + rg) + (ln & 31)];
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            mfma_settled(o[rg][e]);
+                            o[rg][e] *= f;
+                            mfma_settled(o[rg][e]);
+                            __builtin_amdgcn_sched_barrier(0);  // one at a time: they pass through VGPRs
+                        }
+                    }
+                }
             }
-        };
-        u32x4 pw[2 * RG];
-        constexpr int kPAhead = 2 * RG < 3 ? 2 * RG : 3;
+
+            // keys 2j and 2j + 1 of a lane's eight in group st, into A's register j
+            const auto transposed = [&](int st, int j, u32x4 (&av)[E]) {
+                VWords<kVBytes> k0, k1;
+                both_keys<kVBytes>(v[st][j], k0, k1);
+                av[0][j] = pair_of<FP8, kVBytes, 0>(k0, k1);
+                av[1][j] = pair_of<FP8, kVBytes, 1>(k0, k1);
+                if constexpr (E == 4) {
+                    av[2][j] = pair_of<FP8, kVBytes, 2>(k0, k1);
+                    av[3][j] = pair_of<FP8, kVBytes, 3>(k0, k1);
+                }
+            };
+            u32x4 kf[kPerSlice], pw[2];
 #pragma unroll
-        for (int i = 0; i < kPAhead; ++i) pw[i] = pbuf[par][rg0 + i % RG][i / RG][lane];
-        u32x4 av0[E], av1[E];
+            for (int i = 0; i < 2; ++i) pw[i] = pbuf[par][rg0 + i % RG][i / RG][ln];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) transposed(0, j, av0);
-        float top = s_next[0];
+            for (int i = 0; i < kPerSlice; ++i) kf[i] = read_k(kb, par, unit_of(i));
+            u32x4 av[E];
 #pragma unroll
-        for (int i = 0; i < 2 * RG; ++i) {
+            for (int j = 0; j < 4; ++j) transposed(0, j, av);
+            __amdgpu_buffer_rsrc_t kr, vr[2];
+            f32x16 s_new = {};
+            const float base = m == kNegInf ? 0.0f : m;
+            constexpr int kTurns = kSlices * E;  // one product of each kind, and a share of the rest
+            const auto score = [&](int i, int turn) {
+                // the unit's product; the next slice's read follows
+#pragma unroll
+                for (int k = kPerSlice * turn / E; k < kPerSlice * (turn + 1) / E; ++k) {
+                    const int u = i * kPerSlice + k;
+                    s_new = product(s_new, unit_of(u), kf[k]);
+                    if (u + kPerSlice < kUnits) kf[k] = read_k(kb, par, unit_of(u + kPerSlice));
+                }
+            };
+            const auto share = [&](int i, int turn) {
+                const int at = i * E + turn;
+#pragma unroll
+                for (int e = 16 * at / kTurns; e < 16 * (at + 1) / kTurns; ++e) weight(e, s2[par ^ 1], base, par ^ 1, ln);
+                // DMAs of K tile tl + 3 into the buffer of the block before, then V's loads into
+                // the registers whose values have been transposed
+                if (at == 0) kr = k_source(tl + 3);
+                if (at == 1) vr[0] = v_source(2 * tl + 2);
+                if (at == 2) vr[1] = v_source(2 * tl + 3);
+                const int half = kTurns / 2, late = at - half;
+                if (late < 0) {
+#pragma unroll
+                    for (int j = kWaveDmas * at / half; j < kWaveDmas * (at + 1) / half; ++j)
+                        dma_k(kr, (uint32_t)(par ^ 1), j, C::kDmaKeys == 1 ? ln : lane);
+                } else {
+#pragma unroll
+                    for (int j = 8 * late / half; j < 8 * (late + 1) / half; ++j) v[j / 4][j % 4] = fetch_v(vr[j / 4], j % 4);
+                }
+            };
+            float top = kNegInf;
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) {
+                // at the change of groups the scores' products cover the transposes, at the end
+                // V's cover the new scores' maximum
+                const bool scores_first = i == RG || i == kSlices - 1;
+                if (scores_first) {
+#pragma unroll
+                    for (int turn = 0; turn < E; ++turn) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        score(i, turn);
+                        if (i == RG)
+#pragma unroll
+                            for (int j = 4 * turn / E; j < 4 * (turn + 1) / E; ++j) transposed(1, j, av);
+                        if (i == kSlices - 1) share(i, turn);
+                    }
+                }
+#pragma unroll
+                for (int turn = 0; turn < E; ++turn) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    mfma_acc(o[i % RG][turn], av[turn], pw[i % 2]);
+                    if (!scores_first) score(i, turn);
+                    if (i < kSlices - 1) share(i, turn);
+                    if (i == kSlices - 1) {
+                        if (turn == 0) weight_done(15, par ^ 1, ln);
+#pragma unroll
+                        for (int j = 16 * turn / E; j < 16 * (turn + 1) / E; ++j) top = fmaxf(top, s_new[j]);
+                    }
+                }
+                if (i + 2 < kSlices) pw[i % 2] = pbuf[par][rg0 + (i + 2) % RG][(i + 2) / RG][ln];
+            }
             __builtin_amdgcn_sched_barrier(0);
-            mfma_acc<E>(o[i % RG], i < RG ? av0 : av1, pw[i]);
-            if (i == (2 * RG + 1) / 2 && tl + 3 < count) dma_k(tl + 3);  // into the buffer read before the barrier
-            if (i + kPAhead < 2 * RG) pw[i + kPAhead] = pbuf[par][rg0 + (i + kPAhead) % RG][(i + kPAhead) / RG][lane];
-            if (i < RG) {
-#pragma unroll
-                for (int j = 4 * i / RG; j < 4 * (i + 1) / RG; ++j) transposed(1, j, av1);
-            } else {
-#pragma unroll
-                for (int j = 16 * (i - RG) / RG; j < 16 * (i - RG + 1) / RG; ++j) top = fmaxf(top, s_next[j]);
+            s2[par] = s_new;
+            settle(tl + 2, s2[par], half_max(top) * c);
+            if ((tl & 15) == 15) {
+                move_window(2 * tl + 2, pages_next);
+                pages_next = fetch_pages(2 * tl + 34);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        top = half_max(top) * c;
-
-        if (tl + 1 < count) {
-            seen = seen_of(tl + 1);
-            settle(tl + 1, s_next, top, seen);
-        }
-        s_cur = s_next;
     }
+    q4::wait_vm<0>();  // no DMA is on its way as the workgroup ends
 
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
@@ -487,35 +574,38 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
         const float total = sm.l[r];
         const int64_t orow = t.row0 + rtok;
         const int ohead = kv_head * group + rig;
-        const int d0 = slice * C::kSliceDims + 4 * h * E;
+        // row 16 x + 8 b + 4 h + i of product e is dim 2 E (8 b + 4 h + i) + E x + e: 8 E in a run
+        const int d0 = slice * C::kSliceDims + 8 * h * E;
         if (t.splits == 1) {
             const float norm = total > 0.0f || total != total ? (FP8 ? a.pages.v_scale : 1.0f) / total : 0.0f;
             uint16_t* op = a.out + orow * a.out_stride + (int64_t)ohead * D + d0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                // rows 8b + 4h + i of the product are dims E (8b + 4h + i) + e: 4 E of them in a run
-                uint32_t w[2 * E];
+            for (int b = 0; b < 2; ++b) {
+                uint32_t w[4 * E];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < E; e += 2)
-                        w[(i * E + e) / 2] = pack_bf16(o[rg][e][4 * b + i] * norm, o[rg][e + 1][4 * b + i] * norm);
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 2 * E; i += 4)
-                    *reinterpret_cast<u32x4*>(op + 8 * b * E + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
+                        for (int e = 0; e < E; e += 2)
+                            w[(2 * E * i + E * x + e) / 2] = pack_bf16(o[rg][e][8 * x + 4 * b + i] * norm, o[rg][e + 1][8 * x + 4 * b + i] * norm);
+#pragma unroll
+                for (int i = 0; i < 4 * E; i += 4)
+                    *reinterpret_cast<u32x4*>(op + 16 * b * E + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
             }
         } else if (sm.m[r] != kNegInf || total != 0.0f) {
             float* op = it.part_o + (slot + r) * D + d0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    const int k0 = 4 * b + i, k1 = 8 + 4 * b + i;
+                    float* at = op + 16 * b * E + 2 * E * i;
                     if constexpr (E == 4) {
-                        *reinterpret_cast<f32x4*>(op + 8 * b * E + i * E) =
-                            f32x4{o[rg][0][4 * b + i], o[rg][1][4 * b + i], o[rg][2][4 * b + i], o[rg][3][4 * b + i]};
-                    } else if ((i & 1) == 0) {
-                        *reinterpret_cast<f32x4*>(op + 8 * b * E + i * E) =
-                            f32x4{o[rg][0][4 * b + i], o[rg][1][4 * b + i], o[rg][0][4 * b + i + 1], o[rg][1][4 * b + i + 1]};
+                        *reinterpret_cast<f32x4*>(at) = f32x4{o[rg][0][k0], o[rg][1][k0], o[rg][2][k0], o[rg][3][k0]};
+                        *reinterpret_cast<f32x4*>(at + 4) = f32x4{o[rg][0][k1], o[rg][1][k1], o[rg][2][k1], o[rg][3][k1]};
+                    } else {
+                        *reinterpret_cast<f32x4*>(at) = f32x4{o[rg][0][k0], o[rg][1][k0], o[rg][0][k1], o[rg][1][k1]};
                     }
                 }
         }

@@ -469,6 +469,12 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, const void* l
                  : "memory");
 }
 
+// The same with the LDS address given as the offset it is (uniform, so no lane is read for it).
+__device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds)
+                 : "memory");
+}
+
 // s_waitcnt with vmcnt(n) only (expcnt / lgkmcnt left free), n < 64
 template <int N>
 __device__ __forceinline__ void wait_vm() {

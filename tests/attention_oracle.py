@@ -84,11 +84,11 @@ def attend(q, k_cache, v_cache, batch, scale, window=0):
             places, pages, slots = (np.array(w, np.int64) for w in zip(*at)) if at else (np.zeros(0, np.int64),) * 3
             held[r] = places, [(k_cache[pages, h, slots], v_cache[pages, h, slots]) for h in range(k_cache.shape[1])]
         places, per_head = held[r]
-        a, e = np.searchsorted(places, [max(0, p - window + 1) if window else 0, p + 1])
-        if a >= e:
+        begin, end = np.searchsorted(places, [max(0, p - window + 1) if window else 0, p + 1])
+        if begin >= end:
             continue
         for h in range(heads):
-            k, v = (x[a:e] for x in per_head[h // group])
+            k, v = (x[begin:end] for x in per_head[h // group])
             s = scale * (k @ q[i, h])
             top = s.max()
             e = np.exp(s - top)
