@@ -53,6 +53,11 @@ struct TileConf {
     static constexpr int kDmaKeys = 1024 / kRowBytes;                 // keys of one DMA
     static constexpr int kDmas = kTileKeys / kDmaKeys;                // DMAs of a tile
     static constexpr int kTileBytes = kTileKeys * kRowBytes;
+    // LDS that holds two tiles of K, and before and after them passes on each wave's rows of Q
+    // and of the outputs (32 rows of a slice, in fp32 if they are partial)
+    static constexpr int kQBytes = 32 * 2 * D, kOutBytes = 32 * 4 * kSliceDims;
+    static constexpr int kWaveBytes = kQBytes > kOutBytes ? kQBytes : kOutBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes > kTileWaves * kWaveBytes ? 2 * kTileBytes : kTileWaves * kWaveBytes;
 };
 
 // K rows lie in LDS as they do in memory, their 16-byte chunks permuted by xor with
@@ -148,6 +153,7 @@ struct TileShared {
     float alpha[4][128];
     uint32_t raised[4][kTileWaves];
     int pos[128];
+    int64_t q_at[128], out_at[128];  // elements from q's and out's start; out -1: no such row
     float m[128], l[128];
     uint32_t found[kTileWaves];
 };
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     using C = TileConf<D, FP8>;
     constexpr int E = C::kE, RG = C::kGroups;
     constexpr int kVBytes = E * C::kElt;
-    __shared__ alignas(1024) uint4 kbuf[2][C::kTileBytes / 16];
+    __shared__ alignas(1024) char stage[C::kStageBytes];
     __shared__ u32x4 pbuf[2][kTileWaves][2][64];
     __shared__ TileShared sm;
 
@@ -182,22 +188,39 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const int row = t.row0 + (live ? tok : 0);
     const int q_head = kv_head * group + (live ? in_group : 0);
     const int pos = live ? t.pos0 + tok : t.pos0;
-    if (h == 0) sm.pos[tile_row] = pos;  // read by the row's own wave only
+    if (h == 0) {  // read by the row's own wave, the last also by those that hold its outputs
+        sm.pos[tile_row] = pos;
+        sm.q_at[tile_row] = (int64_t)row * a.q_stride + (int64_t)q_head * D;
+        sm.out_at[tile_row] = live ? (int64_t)row * a.out_stride + (int64_t)q_head * D : -1;
+    }
 
+    // Q: whole rows by DMA into the wave's part of the stage (a lane's own 16 bytes of 32 rows
+    // would take the vector memory path twice as long), then into registers in B's layout.
     // The scale's sign goes into Q, so that the largest product is the largest score.  A scale
     // of zero makes every score zero (or NaN) in Q already.
     const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * (FP8 ? a.pages.k_scale : 1.0f) * kLog2e;
     u32x4 q[C::kSteps];
     {
-        const uint16_t* qp = a.q + (int64_t)row * a.q_stride + (int64_t)q_head * D;
+        constexpr int kCpr = D / 8, kRows = 64 / kCpr;  // chunks of a row, rows of a DMA
+        typedef const __attribute__((address_space(1))) void* GlobalPtr;
+        typedef __attribute__((address_space(3))) void* LdsPtr;
+        char* const mine = stage + wave * C::kWaveBytes;
+#pragma unroll
+        for (int j = 0; j < 32 / kRows; ++j) {
+            const int r = j * kRows + lane / kCpr, ch = (lane & (kCpr - 1)) ^ swizzle<kCpr>(r);
+            __builtin_amdgcn_global_load_lds((GlobalPtr)(a.q + sm.q_at[32 * wave + r] + 8 * ch), (LdsPtr)(mine + j * 1024), 16, 0, 0);
+        }
+        q4::wait_vm<0>();
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         const uint32_t keep = live && a.scale != 0.0f ? ~0u : 0u;
 #pragma unroll
         for (int s = 0; s < C::kSteps; ++s) {
             // the dims of the K chunk that step s uses in lane half h
-            const int d = FP8 ? 32 * (s / 2) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h;
-            q[s] = (*reinterpret_cast<const u32x4*>(qp + d) ^ flip) & keep;
+            const int ch = FP8 ? 4 * (s / 2) + 2 * h + (s & 1) : 2 * s + h;
+            q[s] = (*reinterpret_cast<const u32x4*>(mine + n * 2 * D + 16 * (ch ^ swizzle<kCpr>(n))) ^ flip) & keep;
         }
+        q4::wait_lds();
+        q4::lds_barrier();  // K takes the stage
     }
 
     const KeyRange keys = visible_keys(t.pos0, t.n, kv_len, a.window);
@@ -243,7 +266,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const auto k_source = [&](int tl) {
         return q4::make_rsrc(k_head + group_offset(2 * tl + first_key / kGroupKeys), tl < count ? group_bytes : 0u);
     };
-    const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)&kbuf[0][0];
+    const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)stage;
     // this lane's row among a DMA's and its chunk there; the DMA's first key adds its own bits
     // (swizzle(key + i) = swizzle(key) ^ swizzle(i) for i < kDmaKeys)
     const auto dma_k = [&](__amdgpu_buffer_rsrc_t r, uint32_t buffer, int j, int ln) {
@@ -435,7 +458,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
                     }
                 }
             }
-            if (__any(up != 0)) {
+            if (tl > 0 && __any(up != 0)) {  // before the first products there is nothing to rescale
 #pragma unroll
                 for (int rg = 0; rg < RG; ++rg) {
                     if (__builtin_amdgcn_readlane(up, rg0 + rg) != 0) {
@@ -566,19 +589,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     if (lane == 0) sm.found[wave] = nonfinite;
     __syncthreads();
 
+    // Outputs pass through the wave's part of the stage, so that stores take whole runs of a
+    // row's slice (16 bytes of 64 rows each took 64 requests an instruction).  Product e's row
+    // 16 x + 8 b + 4 h + i is dim 2 E (8 b + 4 h + i) + E x + e.
+    char* const mine = stage + wave * C::kWaveBytes;
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        const int r = 32 * (rg0 + rg) + n;
-        const int rtok = r / sh.heads, rig = chunk * sh.heads + r - rtok * sh.heads;
-        if (rtok >= t.n || rig >= group) continue;
-        const float total = sm.l[r];
-        const int64_t orow = t.row0 + rtok;
-        const int ohead = kv_head * group + rig;
-        // row 16 x + 8 b + 4 h + i of product e is dim 2 E (8 b + 4 h + i) + E x + e: 8 E in a run
-        const int d0 = slice * C::kSliceDims + 8 * h * E;
+        const int r0 = 32 * (rg0 + rg);
         if (t.splits == 1) {
+            constexpr int kCpr = C::kSliceDims / 8, kRows = 64 / kCpr;
+            const float total = sm.l[r0 + n];
             const float norm = total > 0.0f || total != total ? (FP8 ? a.pages.v_scale : 1.0f) / total : 0.0f;
-            uint16_t* op = a.out + orow * a.out_stride + (int64_t)ohead * D + d0;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 uint32_t w[4 * E];
@@ -590,24 +611,42 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
                         for (int e = 0; e < E; e += 2)
                             w[(2 * E * i + E * x + e) / 2] = pack_bf16(o[rg][e][8 * x + 4 * b + i] * norm, o[rg][e + 1][8 * x + 4 * b + i] * norm);
 #pragma unroll
-                for (int i = 0; i < 4 * E; i += 4)
-                    *reinterpret_cast<u32x4*>(op + 16 * b * E + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
+                for (int i = 0; i < E; ++i) {
+                    const int ch = (2 * b + h) * E + i;
+                    *reinterpret_cast<u32x4*>(mine + n * 2 * C::kSliceDims + 16 * (ch ^ swizzle<kCpr>(n))) =
+                        u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+                }
             }
-        } else if (sm.m[r] != kNegInf || total != 0.0f) {
-            float* op = it.part_o + (slot + r) * D + d0;
+#pragma unroll
+            for (int j = 0; j < 32 / kRows; ++j) {
+                const int r = j * kRows + lane / kCpr, ch = lane & (kCpr - 1);
+                const u32x4 w = *reinterpret_cast<const u32x4*>(mine + r * 2 * C::kSliceDims + 16 * (ch ^ swizzle<kCpr>(r)));
+                const int64_t at = sm.out_at[r0 + r];
+                if (at >= 0) *reinterpret_cast<u32x4*>(a.out + at + slice * C::kSliceDims + 8 * ch) = w;
+            }
+        } else {
+            constexpr int kCpr = C::kSliceDims / 4, kRows = 64 / kCpr;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k0 = 4 * b + i, k1 = 8 + 4 * b + i;
-                    float* at = op + 16 * b * E + 2 * E * i;
-                    if constexpr (E == 4) {
-                        *reinterpret_cast<f32x4*>(at) = f32x4{o[rg][0][k0], o[rg][1][k0], o[rg][2][k0], o[rg][3][k0]};
-                        *reinterpret_cast<f32x4*>(at + 4) = f32x4{o[rg][0][k1], o[rg][1][k1], o[rg][2][k1], o[rg][3][k1]};
-                    } else {
-                        *reinterpret_cast<f32x4*>(at) = f32x4{o[rg][0][k0], o[rg][1][k0], o[rg][0][k1], o[rg][1][k1]};
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < E / 2; ++x) {
+                        const int k0 = 4 * b + i, k1 = 8 + 4 * b + i;
+                        f32x4 w;
+                        if constexpr (E == 4)
+                            w = f32x4{o[rg][0][x ? k1 : k0], o[rg][1][x ? k1 : k0], o[rg][2][x ? k1 : k0], o[rg][3][x ? k1 : k0]};
+                        else
+                            w = f32x4{o[rg][0][k0], o[rg][1][k0], o[rg][0][k1], o[rg][1][k1]};
+                        const int ch = (8 * b + 4 * h + i) * (E / 2) + x;
+                        *reinterpret_cast<f32x4*>(mine + n * 4 * C::kSliceDims + 16 * (ch ^ swizzle<kCpr>(n))) = w;
                     }
-                }
+#pragma unroll
+            for (int j = 0; j < 32 / kRows; ++j) {
+                const int r = j * kRows + lane / kCpr, ch = lane & (kCpr - 1);
+                *reinterpret_cast<f32x4*>(it.part_o + (slot + r0 + r) * D + slice * C::kSliceDims + 4 * ch) =
+                    *reinterpret_cast<const f32x4*>(mine + r * 4 * C::kSliceDims + 16 * (ch ^ swizzle<kCpr>(r)));
+            }
         }
     }
     bool fix = false;
