@@ -338,10 +338,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
 
 // Joins the items of each tile that has several; bound by the latency of its loads for few
 // rows and by their bytes for many.  Sixteen lanes of four dims take a slice of 64 dims of a
-// row.  Up to eight items are summed by one such group; more are dealt to the workgroup's
-// sixteen groups, whose sums meet in LDS.  Either way always in the same order.
+// row.  Where rows fill the card (`many`) or a tile has eight items at most, one such group
+// sums a slice's items; else they are dealt to the workgroup's sixteen groups, whose sums
+// meet in LDS.  Either way always in the same order.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cuts, int rows) {
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cuts, int rows, int many) {
     constexpr int kSets = 16, kSlices = D / 64;
     __shared__ f32x4 sums[kSets][16];
     __shared__ float totals[kSets];
@@ -369,31 +370,36 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Items it, Cuts cu
         if (a.lse != nullptr && d == 0) a.lse[row * a.q_heads + head] = (top + __builtin_amdgcn_logf(total)) * kLn2;
     };
 
-    if (t.splits <= 8) {
+    if (many || t.splits <= 8) {
         for (int w = (int)blockIdx.y * kSets + set; w < work; w += (int)gridDim.y * kSets) {
             const int r = w / kSlices, d = 64 * (w % kSlices) + d4;
             if (r % sh.heads >= heads_here) continue;
             const int64_t first = first_of(r);
-            float2 ml[8];
-            f32x4 v[8];
-            float top = kNegInf;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const int64_t at = first + (s < t.splits ? s : 0) * step;
-                ml[s] = it.part_ml[at];
-                v[s] = *reinterpret_cast<const f32x4*>(it.part_o + at * D + d);
-                top = fmaxf(top, ml[s].x);
-            }
-            const float base = top == kNegInf ? 0.0f : top;
-            float total = 0.0f;
+            float top = kNegInf, total = 0.0f;
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            for (int s0 = 0; s0 < t.splits; s0 += 8) {
+                float2 ml[8];
+                f32x4 v[8];
+                float next = top;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const bool any = s < t.splits && (ml[s].x != kNegInf || ml[s].y != 0.0f);  // else the item left nothing there
-                const float e = __builtin_amdgcn_exp2f(ml[s].x - base);
-                total += any ? ml[s].y * e : 0.0f;
+                for (int s = 0; s < 8; ++s) {
+                    const int64_t at = first + (s0 + s < t.splits ? s0 + s : s0) * step;
+                    ml[s] = it.part_ml[at];
+                    v[s] = *reinterpret_cast<const f32x4*>(it.part_o + at * D + d);
+                    next = fmaxf(next, ml[s].x);
+                }
+                const float base = next == kNegInf ? 0.0f : next, scale = __builtin_amdgcn_exp2f(top - base);
+                total *= scale;
+                o *= scale;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += any ? v[s][i] * e : 0.0f;
+                for (int s = 0; s < 8; ++s) {
+                    const bool any = s0 + s < t.splits && (ml[s].x != kNegInf || ml[s].y != 0.0f);  // else the item left nothing there
+                    const float e = __builtin_amdgcn_exp2f(ml[s].x - base);
+                    total += any ? ml[s].y * e : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] += any ? v[s][i] * e : 0.0f;
+                }
+                top = next;
             }
             store(r, d, o, top, total);
         }
@@ -456,15 +462,19 @@ hipError_t launch_rows16(const AttnArgs& a, const Items& it, hipStream_t stream)
 hipError_t launch_join(const AttnArgs& a, const Items& it, const Cuts& cuts, int rows, hipStream_t stream) {
     if (it.slots == 0) return hipSuccess;
     const int tiles = (it.items - it.slots) * it.parts;
-    const int work = rows * (a.pages.head_dim / 64);
-    int y = ceil_div(1024, tiles);  // enough workgroups to hide the loads' latency
-    y = y > work ? work : y;
+    // slices of 64 dims, of a tile and in all: sixteen a workgroup if they are many
+    const int group = a.q_heads / a.pages.kv_heads, heads = group < rows ? group : rows, slices = a.pages.head_dim / 64;
+    const int64_t live = (int64_t)a.batch.tokens * heads;
+    const int work = (int)(live < rows ? live : rows) * slices;
+    const bool many = (int64_t)a.batch.tokens * a.q_heads * slices >= 2048;
+    const int most = many ? ceil_div(work, 16) : work, fill = ceil_div(1024, tiles);
+    const int y = most < fill ? most : fill;
     const dim3 grid((unsigned)tiles, (unsigned)y);
     switch (a.pages.head_dim) {
-        case 64: join_kernel<64><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
-        case 128: join_kernel<128><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
-        case 256: join_kernel<256><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
-        case 512: join_kernel<512><<<grid, 256, 0, stream>>>(a, it, cuts, rows); break;
+        case 64: join_kernel<64><<<grid, 256, 0, stream>>>(a, it, cuts, rows, many); break;
+        case 128: join_kernel<128><<<grid, 256, 0, stream>>>(a, it, cuts, rows, many); break;
+        case 256: join_kernel<256><<<grid, 256, 0, stream>>>(a, it, cuts, rows, many); break;
+        case 512: join_kernel<512><<<grid, 256, 0, stream>>>(a, it, cuts, rows, many); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -12,26 +12,55 @@
 // launch and its chain of loads for few.  A workgroup takes one row: the row's sines and
 // cosines are computed once, into LDS, for all its heads.  A head is D/8 lanes of 16
 // bytes each; the pair's other half lies s/8 lanes away (or, for adjacent pairs, in the
-// lane itself), so the rotation needs no LDS of its own.
-#include "kv_index.h"
-#include "kv_kernels.h"
-#include "q4_common.h"
+// lane itself), and the head's sum is taken over its lanes, in registers.  Up to five heads'
+// loads per thread go out before anything that waits; fewer than 512 rows give every 256
+// threads of heads a workgroup of their own.
+// One token's 24 heads of 256: 3.5 us (4.2 with the loads after the row's position and with
+// LDS permutes); 32 tokens into a cache of 64-token pages 4.7 (5.3); 2048 tokens of 17 heads
+// of 512, 71 MB: 20 us, 3.5 TB/s, where a large copy moves 4.9.
+#include "kv_device.h"
 
 namespace kv {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 5;  // heads whose loads are on their way at once, per thread
 
+template <int DPP>
+__device__ __forceinline__ float dpp_sum(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), DPP, 0xf, 0xf, true));
+}
+// Sum over a head's lanes, in each of them; all in registers.
 template <int LANES>
 __device__ __forceinline__ float head_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) v += __shfl_xor(v, d);
+    v = dpp_sum<0xB1>(v);                      // lane ^ 1
+    v = dpp_sum<0x4E>(v);                      // lane ^ 2
+    v = dpp_sum<0x141>(v);                     // the other four of eight
+    if (LANES > 8) v = dpp_sum<0x140>(v);      // the other eight of sixteen
+    if (LANES > 16) {
+        const u32x2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(p.x) + __uint_as_float(p.y);
+    }
+    if (LANES > 32) {
+        const u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(p.x) + __uint_as_float(p.y);
+    }
     return v;
 }
 
 __device__ __forceinline__ float clamp_e4m3(float v) {
     // NaN passes, as in a conversion
     return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f);
+}
+
+// of q, k and v's, selected rather than indexed: the arguments stay in scalar registers
+template <class T>
+__device__ __forceinline__ T pick(int which, T q, T k, T v) {
+    return which == 0 ? q : (which == 1 ? k : v);
+}
+template <>
+__device__ __forceinline__ uint4 pick(int which, uint4 q, uint4 k, uint4 v) {
+    return make_uint4(pick(which, q.x, k.x, v.x), pick(which, q.y, k.y, v.y), pick(which, q.z, k.z, v.z), pick(which, q.w, k.w, v.w));
 }
 
 struct Row {
@@ -63,13 +92,41 @@ __device__ __forceinline__ Row find_row(const Batch& b, const Pages& pg, int t, 
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads) void heads_kernel(HeadArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void heads_kernel(HeadArgs a) {
     constexpr int LANES = D / 8;
     constexpr int kUnits = kThreads / LANES;  // heads a workgroup handles at once
     __shared__ float2 turn[D / 2];
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const int row = (int)blockIdx.x;
     const int c = tid & (LANES - 1);
+
+    // A batch of heads at a time: all its loads go out first, the first batch's before anything
+    // that waits (the row's request and page, the angles).
+    const int nq = a.part[0].count, nk = a.part[1].count, nv = a.part[2].count;
+    const int total = nq + nk + nv;
+    const int stride = kUnits * (int)gridDim.y;
+    const int rounds = ceil_div(total, stride);
+    const auto unit_of = [&](int it) { return it * stride + (int)blockIdx.y * kUnits + tid / LANES; };
+    const auto which_of = [&](int u) { return u < nq || u >= total ? 0 : (u < nq + nk ? 1 : 2); };
+    const auto head_of = [&](int u, int which) { return u - (which == 0 ? 0 : (which == 1 ? nq : nq + nk)); };
+    uint4 raw[kBatch];
+    const auto load = [&](int it0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int u = unit_of(it0 + b), which = which_of(u);
+            const uint16_t* x = pick(which, a.part[0].x, a.part[1].x, a.part[2].x);
+            const int64_t x_stride = pick(which, a.part[0].x_stride, a.part[1].x_stride, a.part[2].x_stride);
+            raw[b] = make_uint4(0, 0, 0, 0);
+            if (u < total) raw[b] = *reinterpret_cast<const uint4*>(x + row * x_stride + (int64_t)head_of(u, which) * D + 8 * c);
+        }
+    };
+    load(0);
+    const auto weight_of = [&](const Heads& p) {
+        return p.weight != nullptr ? *reinterpret_cast<const uint4*>(p.weight + 8 * c)
+                                   : make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);  // ones
+    };
+    const uint4 q_weight = weight_of(a.part[0]), k_weight = weight_of(a.part[1]), v_weight = weight_of(a.part[2]);
+
     Row r{0, -1, 0, true};
     if (a.append)
         r = find_row(a.batch, a.pages, row, lane);
@@ -85,35 +142,30 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(HeadArgs a) {
     }
     __syncthreads();
 
-    const int nq = a.part[0].count, nk = a.part[1].count, nv = a.part[2].count;
-    const int total = nq + nk + nv;
-    const int stride = kUnits * (int)gridDim.y;
-    const int rounds = ceil_div(total, stride);
-    for (int it = 0; it < rounds; ++it) {
-        const int u = it * stride + (int)blockIdx.y * kUnits + tid / LANES;
-        const bool live = u < total;
-        const int which = !live ? 0 : (u < nq ? 0 : (u < nq + nk ? 1 : 2));
-        const Heads& p = a.part[which];
-        const int head = u - (which == 0 ? 0 : (which == 1 ? nq : nq + nk));
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live) raw = *reinterpret_cast<const uint4*>(p.x + (int64_t)row * p.x_stride + (int64_t)head * D + 8 * c);
-        const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-        float x[8];
+    for (int it0 = 0; it0 < rounds; it0 += kBatch) {
+        if (it0 > 0) load(it0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = q4::bf16_lo(w4[i]);
-            x[2 * i + 1] = q4::bf16_hi(w4[i]);
-        }
-        float ss = 0.0f;
+        for (int b = 0; b < kBatch; ++b) {
+            if (it0 + b >= rounds) break;
+            const int u = unit_of(it0 + b);
+            const bool live = u < total;
+            const int which = which_of(u), head = head_of(u, which);
+            const uint32_t w4[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+            float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-        ss = head_sum<LANES>(ss);
-        if (p.norm) {
-            const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = q4::bf16_lo(w4[i]);
+                x[2 * i + 1] = q4::bf16_hi(w4[i]);
+            }
+            float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= inv;
-            if (p.weight != nullptr) {
-                const uint4 wr = *reinterpret_cast<const uint4*>(p.weight + 8 * c);
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+            ss = head_sum<LANES>(ss);
+            if (pick(which, a.part[0].norm, a.part[1].norm, a.part[2].norm)) {
+                const float inv = rsqrtf(ss * (1.0f / D) + pick(which, a.part[0].eps, a.part[1].eps, a.part[2].eps));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= inv;
+                const uint4 wr = pick(which, q_weight, k_weight, v_weight);
                 const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -121,62 +173,81 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(HeadArgs a) {
                     x[2 * i + 1] *= q4::bf16_hi(ww[i]);
                 }
             }
-        }
-        if (pairs > 0) {
-            const bool rot = which != 2;
-            if (dist == 1) {
+            if (pairs > 0) {
+                const bool rot = which != 2;
+                if (dist == 1) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int pr = 4 * c + i;
-                    const float2 cs = rot && pr < pairs ? turn[pr] : make_float2(1.0f, 0.0f);
-                    const float u0 = x[2 * i], u1 = x[2 * i + 1];
-                    x[2 * i] = u0 * cs.x - u1 * cs.y;
-                    x[2 * i + 1] = u1 * cs.x + u0 * cs.y;
-                }
-            } else {
-                const int dl = dist / 8;
-                const bool first = 8 * c < pairs, second = 8 * c >= dist && 8 * c < dist + pairs;
-                const int src = lane + (first ? dl : (second ? -dl : 0));
-                const int i0 = first ? 8 * c : 8 * c - dist;
+                    for (int i = 0; i < 4; ++i) {
+                        const int pr = 4 * c + i;
+                        const float2 cs = rot && pr < pairs ? turn[pr] : make_float2(1.0f, 0.0f);
+                        const float u0 = x[2 * i], u1 = x[2 * i + 1];
+                        x[2 * i] = u0 * cs.x - u1 * cs.y;
+                        x[2 * i + 1] = u1 * cs.x + u0 * cs.y;
+                    }
+                } else {
+                    const int dl = dist / 8;
+                    const bool first = 8 * c < pairs, second = 8 * c >= dist && 8 * c < dist + pairs;
+                    const int src = lane + (first ? dl : (second ? -dl : 0));
+                    const int i0 = first ? 8 * c : 8 * c - dist;
+                    // the pair's other half, dl lanes up or down
+                    float other[8];
+                    if (dl == 32) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float other = __shfl(x[i], src);
+                        for (int i = 0; i < 8; ++i) {
+                            const u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+                            other[i] = __uint_as_float(first ? p.y : p.x);
+                        }
+                    } else if (dl == 16) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const u32x2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+                            other[i] = __uint_as_float(first ? p.y : p.x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) other[i] = __shfl(x[i], src);
+                    }
                     if (rot && (first || second)) {
-                        const float2 cs = turn[i0 + i];
-                        x[i] = first ? x[i] * cs.x - other * cs.y : x[i] * cs.x + other * cs.y;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float2 cs = turn[i0 + i];
+                            x[i] = first ? x[i] * cs.x - other[i] * cs.y : x[i] * cs.x + other[i] * cs.y;
+                        }
                     }
                 }
             }
-        }
-        if (!live) continue;
-        if (p.out != nullptr) {
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = r.in_batch ? (uint32_t)q4::f32_to_bf16(x[2 * i]) | ((uint32_t)q4::f32_to_bf16(x[2 * i + 1]) << 16) : 0u;
-            *reinterpret_cast<uint4*>(p.out + (int64_t)row * p.out_stride + (int64_t)head * D + 8 * c) =
-                make_uint4(o[0], o[1], o[2], o[3]);
-        } else if (r.page >= 0) {
-            const Pages& pg = a.pages;
-            const int64_t at = (int64_t)r.page * pg.page_stride + (int64_t)head * pg.head_stride +
-                               (int64_t)r.slot * pg.token_stride + 8 * c;
-            char* base = which == 1 ? pg.k : pg.v;
-            if (pg.fp8) {
-                const float sc = which == 1 ? pg.k_scale : pg.v_scale;
-                float z[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) z[i] = clamp_e4m3(x[i] / sc);
-                int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
-                int hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], hi, true);
-                *reinterpret_cast<uint2*>(base + at) = make_uint2((uint32_t)lo, (uint32_t)hi);
-            } else {
+            if (!live) continue;
+            uint16_t* const out = pick(which, a.part[0].out, a.part[1].out, a.part[2].out);
+            if (out != nullptr) {
+                const int64_t out_stride = pick(which, a.part[0].out_stride, a.part[1].out_stride, a.part[2].out_stride);
                 uint32_t o[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    o[i] = (uint32_t)q4::f32_to_bf16(x[2 * i]) | ((uint32_t)q4::f32_to_bf16(x[2 * i + 1]) << 16);
-                *reinterpret_cast<uint4*>(base + 2 * at) = make_uint4(o[0], o[1], o[2], o[3]);
+                    o[i] = r.in_batch ? pack_bf16(x[2 * i], x[2 * i + 1]) : 0u;
+                *reinterpret_cast<uint4*>(out + row * out_stride + (int64_t)head * D + 8 * c) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+            } else if (r.page >= 0) {
+                const Pages& pg = a.pages;
+                const int64_t at = (int64_t)r.page * pg.page_stride + (int64_t)head * pg.head_stride +
+                                   (int64_t)r.slot * pg.token_stride + 8 * c;
+                char* base = which == 1 ? pg.k : pg.v;
+                if (pg.fp8) {
+                    const float sc = which == 1 ? pg.k_scale : pg.v_scale;
+                    float z[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) z[i] = clamp_e4m3(x[i] / sc);
+                    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+                    lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+                    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
+                    hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], hi, true);
+                    *reinterpret_cast<uint2*>(base + at) = make_uint2((uint32_t)lo, (uint32_t)hi);
+                } else {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+                    *reinterpret_cast<uint4*>(base + 2 * at) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
             }
         }
     }
