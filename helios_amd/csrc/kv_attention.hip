@@ -3,10 +3,10 @@
 //   s_ij = scale q_i . k_j,  out_i = sum_j softmax_j(s_i) v_j,  lse_i = log sum_j exp s_ij
 //
 // over the keys j that row i sees (kv_index.h).  One pass over the keys with the running
-// maximum m and sum l of the softmax, all in fp32; the weights exp(s - m) <= 1 are rounded
-// to bf16 for their product with V (matrix cores), which moves an output by about 2^-9 of
-// its size over the square root of the keys that carry it, less than the output's own
-// rounding to bf16.  l sums the weights before that rounding.  e4m3 keys and values are
+// maximum m and sum l of the softmax, all in fp32; the weights exp(s - m) are rounded to
+// bf16 for their product with V (matrix cores), 2^-8 of each at most: the outputs of 4096
+// random keys are then 1.8e-3 off in the 2-norm (2.2e-3 from the 128-row tiles), 1.7e-3 of it
+// their own rounding.  l sums the weights before that rounding.  e4m3 keys and values are
 // exact in bf16; their scales are applied to s and to the output.
 //
 // rows16_kernel: 16 query rows (tokens x heads sharing a KV head) at a time; each wave of

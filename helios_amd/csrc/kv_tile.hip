@@ -5,7 +5,7 @@
 // rows per key the work is bound by the matrix cores (a key's 2 D bytes of K and V feed
 // 4 x 128 x D operations), so the layout is chosen to keep them fed from one wave per SIMD:
 //
-//   S^T = K Q^T (32x32x16, A = K): wave w holds rows 32w..32w+31 of Q in registers and
+//   S^T = K Q^T (32x32x16, A = K): a wave holds 32 rows of Q in registers and
 //   reads each 32-key tile of K from LDS.  Lane (n = l % 32, h = l / 32) gets s of row n
 //   and keys 8b + 4h + r (b, r < 4), so a row's maximum needs one exchange of two lanes.
 //   O^T += V^T P^T (32x32x16, A = V^T): the waves divide the dims of V, not the rows: the
@@ -24,8 +24,17 @@
 // of them a share of tile i + 1's softmax, of the transposes, of the DMAs of K tile i + 3 and of
 // the loads of V tile i + 1.  (Scores first and V after them, in two blocks: 1095 us at 2048
 // tokens over 16384 keys, 16 heads of 512 over one; in turns of four products 1070; in turns of
-// one 982-1000 us, 1.05 PFLOP/s.)  Loads of V take 16 bytes a lane, two keys at once: the
-// vector memory path moves 64 B a cycle at best, and a wave that waits for it issues no products.
+// one 971, 1.06 PFLOP/s.)  A wave issues an instruction every 6 cycles at best, five beside a
+// product of 32, and a step has some six: that, and the time at its barrier, is what keeps it
+// from the library product's 1.24 PFLOP/s.  Loads of V take 16 bytes a lane, two keys at once:
+// the vector memory path moves 64 B a cycle, and a wave that waits for it issues no products.
+//
+// head_dim 256 has the registers for two waves per SIMD: eight waves, tiles of 64 keys; wave w
+// and w + 4 hold the same rows of Q and score a half of the keys each, exchanging the rows'
+// maxima through LDS; V's dims are in four slices, each for two waves of 64 rows.  2048 tokens
+// of 16 heads over 8, window 1024: 68 us with four waves, 53.4 with eight (644 TFLOP/s; some
+// 19 us of it are a workgroup's start and end, which a longer range pays once).
+//
 // The running maximum of a row is raised only when a score exceeds it by 2^8: weights up to
 // 2^8 lose nothing in bf16 or in the fp32 sums, and the outputs (256 registers at head_dim
 // 512) are seldom rescaled.
@@ -36,28 +45,33 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kTileKeys = 32;
-constexpr int kTileWaves = 4;
 constexpr float kSlack = 8.0f;  // how far a score may exceed the running maximum (log2)
+
+template <int D>
+constexpr int tile_waves = D == 256 ? 8 : 4;
 
 template <int D, bool FP8>
 struct TileConf {
     static constexpr int kElt = FP8 ? 1 : 2;
-    static constexpr int kSlices = D == 512 ? 4 : (D == 64 ? 1 : 2);  // dim slices
-    static constexpr int kGroups = kSlices;                           // 32-row groups of a wave's outputs
+    static constexpr int kWaves = tile_waves<D>;
+    static constexpr int kHalves = kWaves / 4;                        // waves that share 32 rows' scores, by keys
+    static constexpr int kKeys = 32 * kHalves;                        // keys of a tile
+    static constexpr int kSteps16 = kKeys / 16;                       // groups of 16 keys, steps of V's products
+    static constexpr int kSlices = D >= 256 ? 4 : (D == 64 ? 1 : 2);  // dim slices
+    static constexpr int kGroups = 4 * kSlices / kWaves;              // 32-row groups of a wave's outputs
     static constexpr int kSliceDims = D / kSlices;
     static constexpr int kE = kSliceDims / 32;                        // consecutive dims of a lane
     static constexpr int kRowBytes = D * kElt;
     static constexpr int kCpr = kRowBytes / 16;                       // 16-byte chunks of a K row
     static constexpr int kSteps = D / 16;
     static constexpr int kDmaKeys = 1024 / kRowBytes;                 // keys of one DMA
-    static constexpr int kDmas = kTileKeys / kDmaKeys;                // DMAs of a tile
-    static constexpr int kTileBytes = kTileKeys * kRowBytes;
+    static constexpr int kDmas = kKeys / kDmaKeys;                    // DMAs of a tile
+    static constexpr int kTileBytes = kKeys * kRowBytes;
     // LDS that holds two tiles of K, and before and after them passes on each wave's rows of Q
     // and of the outputs (32 rows of a slice, in fp32 if they are partial)
     static constexpr int kQBytes = 32 * 2 * D, kOutBytes = 32 * 4 * kSliceDims;
-    static constexpr int kWaveBytes = kQBytes > kOutBytes ? kQBytes : kOutBytes;
-    static constexpr int kStageBytes = 2 * kTileBytes > kTileWaves * kWaveBytes ? 2 * kTileBytes : kTileWaves * kWaveBytes;
+    static constexpr int kPassBytes = 4 * kQBytes > kWaves * kOutBytes ? 4 * kQBytes : kWaves * kOutBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes > kPassBytes ? 2 * kTileBytes : kPassBytes;
 };
 
 // K rows lie in LDS as they do in memory, their 16-byte chunks permuted by xor with
@@ -73,14 +87,31 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// o += a x p with the accumulators in AGPRs: with the builtin the compiler keeps accumulators
-// either all in VGPRs or, S among them, all in AGPRs, and neither holds 256 of O beside the
-// rest.  It sees no hazards in asm: the wait states cover operands that the VALU has just
-// written, and mfma_settled() goes between these products and the next VALU access to o.
+// o += a x p.  AGPRS: with the accumulators in AGPRs, for head_dim 512: with the builtin the
+// compiler keeps accumulators either all in VGPRs or, S among them, all in AGPRs, and neither
+// holds 256 of O beside the rest.  It sees no hazards in asm.  An operand that the VALU writes
+// needs two wait states before the product (operands_settled() after the transposes; a test
+// reads the compiled code for any other write), and mfma_settled() goes between the products
+// and the next VALU access to o.  (The wait states in each product's own asm cost an issue
+// slot of the five a product has.)
+template <bool AGPRS>
 __device__ __forceinline__ void mfma_acc(f32x16& o, u32x4 a, u32x4 p) {
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+    if constexpr (AGPRS)
+        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+    else
+        o = mfma32(a, p, o);
 }
-__device__ __forceinline__ void mfma_settled(f32x16& o) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o)); }
+template <bool AGPRS>
+__device__ __forceinline__ void operands_settled() {
+    if constexpr (AGPRS) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 1");
+    }
+}
+template <bool AGPRS>
+__device__ __forceinline__ void mfma_settled(f32x16& o) {
+    if constexpr (AGPRS) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o));
+}
 
 __device__ __forceinline__ float half_max(float v) {
     const u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -149,23 +180,26 @@ __device__ __forceinline__ uint32_t pair_of(const VWords<BYTES>& a, const VWords
     }
 }
 
+template <int WAVES>
 struct TileShared {
     float alpha[4][128];
-    uint32_t raised[4][kTileWaves];
+    float top[4][WAVES / 4][128];  // used where two waves share rows
+    uint32_t raised[4][4];         // by 32-row group
     int pos[128];
     int64_t q_at[128], out_at[128];  // elements from q's and out's start; out -1: no such row
-    float m[128], l[128];
-    uint32_t found[kTileWaves];
+    float m[128], l[WAVES / 4][128];
+    uint32_t found[WAVES];
 };
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, Items it) {
+__global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_kernel(AttnArgs a, Items it) {
     using C = TileConf<D, FP8>;
     constexpr int E = C::kE, RG = C::kGroups;
-    constexpr int kVBytes = E * C::kElt;
+    constexpr bool kAgprs = D == 512;
+    constexpr int kVBytes = E * C::kElt, kWaves = C::kWaves, kTileKeys = C::kKeys, kSt = C::kSteps16;
     __shared__ alignas(1024) char stage[C::kStageBytes];
-    __shared__ u32x4 pbuf[2][kTileWaves][2][64];
-    __shared__ TileShared sm;
+    __shared__ u32x4 pbuf[2][4][kSt][64];
+    __shared__ TileShared<kWaves> sm;
 
     const int lane = (int)threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -180,15 +214,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     if (t.n <= 0) return;
     const int kv_len = clampi(t.kv_len, 0, a.batch.width << a.pages.page_shift);
 
-    // this lane's query row
-    const int tile_row = 32 * wave + n;
+    // this lane's query row; where two waves have the same rows, each has its half of a tile's keys
+    const int own = C::kHalves == 1 ? wave : wave & 3, half = C::kHalves == 1 ? 0 : wave >> 2;  // 32-row group, half of the keys
+    const int tile_row = 32 * own + n;
     const int tok = tile_row / sh.heads, hh = tile_row - tok * sh.heads;
     const int in_group = chunk * sh.heads + hh;
     const bool live = tok < t.n && in_group < group;
     const int row = t.row0 + (live ? tok : 0);
     const int q_head = kv_head * group + (live ? in_group : 0);
     const int pos = live ? t.pos0 + tok : t.pos0;
-    if (h == 0) {  // read by the row's own wave, the last also by those that hold its outputs
+    if (h == 0 && half == 0) {
         sm.pos[tile_row] = pos;
         sm.q_at[tile_row] = (int64_t)row * a.q_stride + (int64_t)q_head * D;
         sm.out_at[tile_row] = live ? (int64_t)row * a.out_stride + (int64_t)q_head * D : -1;
@@ -204,13 +239,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
         constexpr int kCpr = D / 8, kRows = 64 / kCpr;  // chunks of a row, rows of a DMA
         typedef const __attribute__((address_space(1))) void* GlobalPtr;
         typedef __attribute__((address_space(3))) void* LdsPtr;
-        char* const mine = stage + wave * C::kWaveBytes;
+        char* const mine = stage + own * C::kQBytes;
+        if (half == 0)
 #pragma unroll
         for (int j = 0; j < 32 / kRows; ++j) {
             const int r = j * kRows + lane / kCpr, ch = (lane & (kCpr - 1)) ^ swizzle<kCpr>(r);
-            __builtin_amdgcn_global_load_lds((GlobalPtr)(a.q + sm.q_at[32 * wave + r] + 8 * ch), (LdsPtr)(mine + j * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((GlobalPtr)(a.q + sm.q_at[32 * own + r] + 8 * ch), (LdsPtr)(mine + j * 1024), 16, 0, 0);
         }
-        q4::wait_vm<0>();
+        q4::wait_vm_lds<0>();
+        if (C::kHalves > 1) q4::lds_barrier();
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         const uint32_t keep = live && a.scale != 0.0f ? ~0u : 0u;
 #pragma unroll
@@ -233,15 +270,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const uint32_t row_bytes = (uint32_t)a.pages.token_stride * C::kElt;
 
     // Where the 16-key groups lie: lane i has group `window` + i's bytes from this head's first
-    // page, and its bit of `present` whether there is a page.  The window moves by 16 tiles; the
-    // pages of the next one are read 16 tiles ahead.
+    // page, and its bit of `present` whether there is a page.  The window moves by 32
+    // groups; the pages of the next one are read that far ahead.
     const uint64_t page_bytes = (uint64_t)a.pages.page_stride * C::kElt;
     const int64_t head_bytes = (int64_t)kv_head * a.pages.head_stride * C::kElt;
     const char* const k_head = a.pages.k + head_bytes;
     const char* const v_head = a.pages.v + head_bytes;
     const auto fetch_pages = [&](int first) {
         const int g = first + lane;
-        return g < 2 * count ? page_at(table, (key0 + g * kGroupKeys) >> a.pages.page_shift, a.batch.width, a.pages.num_pages) : -1;
+        return g < kSt * count ? page_at(table, (key0 + g * kGroupKeys) >> a.pages.page_shift, a.batch.width, a.pages.num_pages) : -1;
     };
     int window = 0, pages_next = 0;
     uint64_t offsets = 0;
@@ -261,10 +298,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     const uint32_t group_bytes = 15u * row_bytes + (uint32_t)C::kRowBytes;
     // K tile `tl` into a buffer: each DMA brings kDmaKeys whole rows, a wave's lie in one group of
     // 16 keys.  Past the last tile the resource is empty (the DMAs bring zeros).
-    constexpr int kWaveDmas = (C::kDmas + kTileWaves - 1) / kTileWaves;
+    constexpr int kWaveDmas = (C::kDmas + kWaves - 1) / kWaves;
     const int first_dma = wave * kWaveDmas % C::kDmas, first_key = first_dma * C::kDmaKeys;
     const auto k_source = [&](int tl) {
-        return q4::make_rsrc(k_head + group_offset(2 * tl + first_key / kGroupKeys), tl < count ? group_bytes : 0u);
+        return q4::make_rsrc(k_head + group_offset(kSt * tl + first_key / kGroupKeys), tl < count ? group_bytes : 0u);
     };
     const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)stage;
     // this lane's row among a DMA's and its chunk there; the DMA's first key adds its own bits
@@ -286,7 +323,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     constexpr int kUnits = C::kCpr / 2, kFar = C::kCpr > 16 ? C::kCpr / 16 : 1, kPer = FP8 ? 2 : 1;
     typedef const __attribute__((address_space(3))) u32x4* LdsPtr;
     const auto k_base = [&](int ln) {
-        return k_lds + (uint32_t)(ln & 31) * C::kRowBytes + 16u * (uint32_t)((ln >> 5) ^ swizzle<C::kCpr>(ln & 31));
+        return k_lds + (uint32_t)(32 * half + (ln & 31)) * C::kRowBytes + 16u * (uint32_t)((ln >> 5) ^ swizzle<C::kCpr>(ln & 31));
     };
     const auto unit_of = [](int i) { return i / kFar + 8 * (i % kFar); };
     const auto read_k = [&](uint32_t base, int buffer, int u) {
@@ -316,38 +353,19 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     float m = kNegInf, l = 0.0f;
     bool nonfinite = false;
 
+    constexpr uint32_t kAllPages = (1u << kSt) - 1u;
     // whether every row of the tile sees all of tile tl's keys, and which groups have pages
     const auto all_seen = [&](int tl) { return all_visible(key0 + tl * kTileKeys, kTileKeys, t.pos0, t.n, a.window); };
-    const auto pages_of = [&](int tl) { return (uint32_t)(present >> (2 * tl - window)) & 3u; };
+    const auto pages_of = [&](int tl) { return (uint32_t)(present >> (kSt * tl - window)) & kAllPages; };
     const auto top_of = [&](const f32x16& s) {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
         return half_max(top) * c;
     };
-    // Tile tl's scores in `s`: masks them, if some row does not see all of its keys (or there is
-    // no such tile), and raises the running maximum, if a score exceeds it by more than kSlack
-    // (the wave's sums here, the outputs when the weights are used).
-    const auto settle = [&](int tl, f32x16& s, float top) {
-        if (tl >= count) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = kNegInf;
-            return;
-        }
-        const uint32_t there = pages_of(tl);
-        if (!all_seen(tl) || there != 3u) {
-            int ln = lane;
-            asm volatile("" : "+v"(ln));
-            const int pos = sm.pos[32 * wave + (ln & 31)];
-            const int above = a.window > 0 ? pos - a.window : -0x7fffffff;  // keys in (above, pos]
-            const int first = key0 + tl * kTileKeys + 4 * (ln >> 5);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = first + 8 * (i / 4) + i % 4;
-                s[i] = (there >> (i / 8) & 1) && key <= pos && key > above ? s[i] : kNegInf;
-            }
-            top = top_of(s);
-        }
+    // Raises the running maximum, if a score of tile tl exceeds it by more than kSlack: the
+    // wave's sums here, the outputs when the weights are used.
+    const auto raise = [&](int tl, float top) {
         uint32_t raised = 0;
         if (__any(top > m + kSlack)) {
             const float next = fmaxf(m, top);
@@ -356,13 +374,52 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
             l *= alpha;
             int ln = lane;
             asm volatile("" : "+v"(ln));
-            if (ln < 32) sm.alpha[tl & 3][32 * wave + ln] = alpha;
+            if (ln < 32 && half == 0) sm.alpha[tl & 3][32 * own + ln] = alpha;
             raised = 1;
         }
-        if (lane == 0) sm.raised[tl & 3][wave] = raised;
+        if (lane == 0 && half == 0) sm.raised[tl & 3][own] = raised;
+    };
+    // Tile tl's scores in `s`: masks them, if some row does not see all of its keys (or there is
+    // no such tile).  Their maximum raises the running one at once where a wave has all of a
+    // row's keys; where two share them it goes to LDS, and both raise (`raise_shared`) after
+    // the next barrier, before the tile's weights.
+    const auto settle = [&](int tl, f32x16& s, float top) {
+        if (tl >= count) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = kNegInf;
+            return;
+        }
+        const uint32_t there = pages_of(tl);
+        if (!all_seen(tl) || there != kAllPages) {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const int pos = sm.pos[32 * own + (ln & 31)];
+            const int above = a.window > 0 ? pos - a.window : -0x7fffffff;  // keys in (above, pos]
+            const int first = key0 + tl * kTileKeys + 32 * half + 4 * (ln >> 5);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = first + 8 * (i / 4) + i % 4;
+                s[i] = (there >> (2 * half + i / 8) & 1) && key <= pos && key > above ? s[i] : kNegInf;
+            }
+            top = top_of(s);
+        }
+        if constexpr (C::kHalves == 1) {
+            raise(tl, top);
+        } else {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            if (ln < 32) sm.top[tl & 3][half][32 * own + ln] = top;
+        }
+    };
+    const auto raise_shared = [&](int tl) {
+        if (C::kHalves == 1 || tl >= count) return;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int r = 32 * own + (ln & 31);
+        raise(tl, fmaxf(sm.top[tl & 3][0][r], sm.top[tl & 3][C::kHalves - 1][r]));
     };
 
-    VRaw<kVBytes> v[2][4];  // a tile's V: this lane's dims of its keys in each group of 16
+    VRaw<kVBytes> v[kSt][4];  // a tile's V: this lane's dims of its keys in each group of 16
     const auto v_source = [&](int g) { return q4::make_rsrc(v_head + group_offset(g), group_bytes); };
     const auto fetch_v = [&](__amdgpu_buffer_rsrc_t r, int j) { return load_v<kVBytes>(r, v_lane, (uint32_t)(8 * (j / 2) + 2 * (j % 2)) * row_bytes); };
 
@@ -374,7 +431,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
         l += last;
         asm volatile("" : "+v"(l));  // here, between the products
         if (e & 1) pk[e / 2 % 4] = pack_bf16(before, last);
-        if (e % 8 == 7) pbuf[par][wave][e / 8][ln] = u32x4{pk[0], pk[1], pk[2], pk[3]};
+        if (e % 8 == 7) pbuf[par][own][2 * half + e / 8][ln] = u32x4{pk[0], pk[1], pk[2], pk[3]};
     };
     const auto weight = [&](int e, const f32x16& s, float base, int par, int ln) {
         const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -base));
@@ -403,46 +460,56 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
                 s2[b] = product(s2[b], unit_of(i), read_k(k_base(lane), b, unit_of(i)));
             }
         settle(0, s2[0], top_of(s2[0]));
+        if constexpr (C::kHalves > 1) {
+            settle(1, s2[1], top_of(s2[1]));
+            q4::wait_lds();
+            q4::lds_barrier();
+            raise_shared(0);
+        }
         const float base = m == kNegInf ? 0.0f : m;
 #pragma unroll
         for (int e = 0; e < 16; ++e) weight(e, s2[0], base, 0, lane);
         weight_done(15, 0, lane);
-        settle(1, s2[1], top_of(s2[1]));
-        q4::wait_lds();
-        q4::lds_barrier();
+        if constexpr (C::kHalves == 1) {
+            settle(1, s2[1], top_of(s2[1]));
+            q4::wait_lds();
+            q4::lds_barrier();
+        }
 #pragma unroll
         for (int j = 0; j < kWaveDmas; ++j) dma_k(k2, 0, j, lane);
-        const __amdgpu_buffer_rsrc_t v0 = v_source(0), v1 = v_source(1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[0][j] = fetch_v(v0, j);
+        for (int st = 0; st < kSt; ++st) {
+            const __amdgpu_buffer_rsrc_t r = v_source(st);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[1][j] = fetch_v(v1, j);
+            for (int j = 0; j < 4; ++j) v[st][j] = fetch_v(r, j);
+        }
     }
 
     // Per tile tl: its weights are in LDS and its V is on the way, and the next tile's scores
     // are in s2.  The products of its V, those of the scores of tile tl + 2, and the weights of
     // tile tl + 1 take turns, so that neither the matrix cores nor LDS nor the VALU wait for
     // the others for long.  The order is the source's: slices end in scheduling barriers.
-    constexpr int kSlices = 2 * RG, kPerSlice = kUnits / kSlices;
+    constexpr int kSlices = kSt * RG, kPerSlice = kUnits / kSlices;
     for (int pair = 0; pair < count; pair += 2) {
 #pragma unroll
         for (int par = 0; par < 2; ++par) {
             const int tl = pair + par;
             if (tl >= count) break;
-            // K of tile tl + 2 has landed (its DMAs are older than the 8 loads of V) and the
+            // K of tile tl + 2 has landed (its DMAs are older than the loads of V) and the
             // weights are written
-            q4::wait_vm_lds<8>();
+            q4::wait_vm_lds<4 * kSt>();
             q4::lds_barrier();
             int ln = lane;
             asm volatile("" : "+v"(ln));  // addresses made from it are made here, not kept
             const uint32_t kb = k_base(ln);
 
-            const uint32_t up = sm.raised[tl & 3][ln & (kTileWaves - 1)];
+            const uint32_t up = sm.raised[tl & 3][ln & 3];
+            raise_shared(tl + 1);
             const uint32_t there = pages_of(tl);
-            if (!all_seen(tl) || there != 3u) {
+            if (!all_seen(tl) || there != kAllPages) {
                 const bool visible = all_seen(tl);
 #pragma unroll
-                for (int st = 0; st < 2; ++st) {
+                for (int st = 0; st < kSt; ++st) {
                     if (visible && (there >> st & 1)) continue;
                     bool bad = false;
 #pragma unroll
@@ -465,9 +532,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
                         const float f = sm.alpha[tl & 3][32 * (rg0 + rg) + (ln & 31)];
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
-                            mfma_settled(o[rg][e]);
+                            mfma_settled<kAgprs>(o[rg][e]);
                             o[rg][e] *= f;
-                            mfma_settled(o[rg][e]);
+                            mfma_settled<kAgprs>(o[rg][e]);
                             __builtin_amdgcn_sched_barrier(0);  // one at a time: they pass through VGPRs
                         }
                     }
@@ -493,7 +560,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
             u32x4 av[E];
 #pragma unroll
             for (int j = 0; j < 4; ++j) transposed(0, j, av);
-            __amdgpu_buffer_rsrc_t kr, vr[2];
+            __amdgpu_buffer_rsrc_t kr, vr[kSt];
             f32x16 s_new = {};
             const float base = m == kNegInf ? 0.0f : m;
             constexpr int kTurns = kSlices * E;  // one product of each kind, and a share of the rest
@@ -513,16 +580,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
                 // DMAs of K tile tl + 3 into the buffer of the block before, then V's loads into
                 // the registers whose values have been transposed
                 if (at == 0) kr = k_source(tl + 3);
-                if (at == 1) vr[0] = v_source(2 * tl + 2);
-                if (at == 2) vr[1] = v_source(2 * tl + 3);
-                const int half = kTurns / 2, late = at - half;
+#pragma unroll
+                for (int st = 0; st < kSt; ++st)
+                    if (at == st + 1) vr[st] = v_source(kSt * (tl + 1) + st);
+                constexpr int kMid = kTurns / 2;
+                const int late = at - kMid;
                 if (late < 0) {
 #pragma unroll
-                    for (int j = kWaveDmas * at / half; j < kWaveDmas * (at + 1) / half; ++j)
+                    for (int j = kWaveDmas * at / kMid; j < kWaveDmas * (at + 1) / kMid; ++j)
                         dma_k(kr, (uint32_t)(par ^ 1), j, C::kDmaKeys == 1 ? ln : lane);
                 } else {
 #pragma unroll
-                    for (int j = 8 * late / half; j < 8 * (late + 1) / half; ++j) v[j / 4][j % 4] = fetch_v(vr[j / 4], j % 4);
+                    for (int j = 4 * kSt * late / kMid; j < 4 * kSt * (late + 1) / kMid; ++j) v[j / 4][j % 4] = fetch_v(vr[j / 4], j % 4);
                 }
             };
             float top = kNegInf;
@@ -530,22 +599,23 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
             for (int i = 0; i < kSlices; ++i) {
                 // at the change of groups the scores' products cover the transposes, at the end
                 // V's cover the new scores' maximum
-                const bool scores_first = i == RG || i == kSlices - 1;
+                const bool next_group = i > 0 && i % RG == 0, scores_first = next_group || i == kSlices - 1;
                 if (scores_first) {
 #pragma unroll
                     for (int turn = 0; turn < E; ++turn) {
                         __builtin_amdgcn_sched_barrier(0);
                         score(i, turn);
-                        if (i == RG)
+                        if (next_group)
 #pragma unroll
-                            for (int j = 4 * turn / E; j < 4 * (turn + 1) / E; ++j) transposed(1, j, av);
+                            for (int j = 4 * turn / E; j < 4 * (turn + 1) / E; ++j) transposed(i / RG, j, av);
                         if (i == kSlices - 1) share(i, turn);
                     }
                 }
+                if (i % RG == 0) operands_settled<kAgprs>();
 #pragma unroll
                 for (int turn = 0; turn < E; ++turn) {
                     __builtin_amdgcn_sched_barrier(0);
-                    mfma_acc(o[i % RG][turn], av[turn], pw[i % 2]);
+                    mfma_acc<kAgprs>(o[i % RG][turn], av[turn], pw[i % 2]);
                     if (!scores_first) score(i, turn);
                     if (i < kSlices - 1) share(i, turn);
                     if (i == kSlices - 1) {
@@ -559,9 +629,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
             __builtin_amdgcn_sched_barrier(0);
             s2[par] = s_new;
             settle(tl + 2, s2[par], half_max(top) * c);
-            if ((tl & 15) == 15) {
-                move_window(2 * tl + 2, pages_next);
-                pages_next = fetch_pages(2 * tl + 34);
+            if (tl % (32 / kSt) == 32 / kSt - 1) {
+                move_window(kSt * (tl + 1), pages_next);
+                pages_next = fetch_pages(kSt * (tl + 1) + 32);
             }
         }
     }
@@ -570,35 +640,36 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-        for (int e = 0; e < E; ++e) mfma_settled(o[rg][e]);
+        for (int e = 0; e < E; ++e) mfma_settled<kAgprs>(o[rg][e]);
 
     const int64_t slot = (int64_t)blockIdx.x * kWideRows;  // rows of this item's partial sums
     // every row's maximum and sum, for the waves that hold its outputs
     l = half_sum(l);
     if (h == 0) {
-        sm.m[tile_row] = m;
-        sm.l[tile_row] = l;
-        if (live) {
-            const int64_t out_row = (int64_t)row * a.q_heads + q_head;
-            if (t.splits > 1)
-                it.part_ml[slot + tile_row] = make_float2(m, l);
-            else if (a.lse != nullptr)
-                a.lse[out_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-        }
+        if (half == 0) sm.m[tile_row] = m;
+        sm.l[half][tile_row] = l;
     }
     if (lane == 0) sm.found[wave] = nonfinite;
     __syncthreads();
+    const auto sum_of = [&](int r) { return C::kHalves == 1 ? sm.l[0][r] : sm.l[0][r] + sm.l[C::kHalves - 1][r]; };
+    if (h == 0 && half == 0 && live) {
+        const float total = sum_of(tile_row);
+        if (t.splits > 1)
+            it.part_ml[slot + tile_row] = make_float2(m, total);
+        else if (a.lse != nullptr)
+            a.lse[(int64_t)row * a.q_heads + q_head] = (m + __builtin_amdgcn_logf(total)) * kLn2;
+    }
 
     // Outputs pass through the wave's part of the stage, so that stores take whole runs of a
     // row's slice (16 bytes of 64 rows each took 64 requests an instruction).  Product e's row
     // 16 x + 8 b + 4 h + i is dim 2 E (8 b + 4 h + i) + E x + e.
-    char* const mine = stage + wave * C::kWaveBytes;
+    char* const mine = stage + wave * C::kOutBytes;
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
         const int r0 = 32 * (rg0 + rg);
         if (t.splits == 1) {
             constexpr int kCpr = C::kSliceDims / 8, kRows = 64 / kCpr;
-            const float total = sm.l[r0 + n];
+            const float total = sum_of(r0 + n);
             const float norm = total > 0.0f || total != total ? (FP8 ? a.pages.v_scale : 1.0f) / total : 0.0f;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -651,12 +722,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
     }
     bool fix = false;
 #pragma unroll
-    for (int w = 0; w < kTileWaves; ++w) fix |= sm.found[w] != 0;
+    for (int w = 0; w < kWaves; ++w) fix |= sm.found[w] != 0;
     if (fix) {
         __syncthreads();  // the outputs are in memory
         const int from = key0;
         const int upto = key0 + count * kTileKeys < keys.hi ? key0 + count * kTileKeys : keys.hi;
-        fix_nonfinite<D, FP8>(a, t, sh, kv_head, from, upto, kTileKeys, 64 * kTileWaves, [&](int i, int hd, int d, float v) {
+        fix_nonfinite<D, FP8>(a, t, sh, kv_head, from, upto, kTileKeys, 64 * kWaves, [&](int i, int hd, int d, float v) {
             const int ig = chunk * sh.heads + hd;
             if (ig >= group) return;
             const int64_t rr = t.row0 + i;
@@ -674,7 +745,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void tile_kernel(AttnArgs a, It
 
 template <int D, bool FP8>
 hipError_t launch(const AttnArgs& a, const Items& it, hipStream_t stream) {
-    tile_kernel<D, FP8><<<(unsigned)it.items * (unsigned)it.parts, 64 * kTileWaves, 0, stream>>>(a, it);
+    tile_kernel<D, FP8><<<(unsigned)it.items * (unsigned)it.parts, 64 * tile_waves<D>, 0, stream>>>(a, it);
     return hipGetLastError();
 }
 

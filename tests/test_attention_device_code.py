@@ -40,6 +40,40 @@ def test_tile_steps_stay_in_registers(tile_asm, d, fp8):
         assert any(" lds" in i for i in ins) or not any("a[" in i for i in ins if i.startswith("v_mfma"))
 
 
+def _vgprs(tok: str):
+    m = re.match(r"v\[(\d+):(\d+)\]$", tok)
+    if m:
+        return set(range(int(m.group(1)), int(m.group(2)) + 1))
+    m = re.match(r"v(\d+)$", tok)
+    return {int(m.group(1))} if m else set()
+
+
+@pytest.mark.parametrize("fp8", [0, 1])
+def test_products_in_asm_wait_for_their_operands(tile_asm, fp8):
+    """The products with accumulators in AGPRs are asm, which the compiler's hazard recognizer
+    cannot see into: no VALU write of an operand within two wait states before one."""
+    (name, lines), = [k for k in _kernels(tile_asm, f"tile_kernelILi512ELb{fp8}E")]
+    products = 0
+    for i, line in enumerate(lines):
+        if not re.match(r"v_mfma_f32_32x32x16_bf16 a\[", line):
+            continue
+        products += 1
+        a, b = (_vgprs(t.strip(",")) for t in line.split()[2:4])
+        assert len(a) == 4 and len(b) == 4, line
+        waits, j = 0, i - 1
+        while j >= 0 and waits < 2:
+            op = lines[j].split()[0]
+            if op == "s_nop":
+                waits += int(lines[j].split()[1]) + 1
+            elif not op.endswith(":"):
+                if op.startswith("v_") and not op.startswith("v_mfma"):
+                    written = set().union(*[_vgprs(t.strip(",")) for t in lines[j].split()[1:3 if "swap" in op else 2]])
+                    assert not written & (a | b), f"{name}: {lines[j]!r} feeds {line!r}"
+                waits += 1
+            j -= 1
+    assert products >= 2 * 32  # an even and an odd tile's
+
+
 def test_attention_register_and_lds_budgets(tile_asm):
     """The 16-row kernel: no scratch, two workgroups of four waves per CU up to head_dim 256
     (256 VGPRs), as the planner counts on; every tile fits the CU's LDS."""
