@@ -65,7 +65,7 @@ Gemma4Status check_pages(const Gemma4KvPages* p, const char* name, kv::Pages* ou
 Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const char* name, kv::Batch* out) {
     if (b == nullptr) return bad(name, "requires a non-null batch");
     if (b->requests == 0 || b->requests > (1u << 20)) return bad(name, "requests must be 1 to 2^20");
-    if (b->tokens > (1u << 24)) return unsupported(name, "tokens exceeds 2^24");
+    if (b->tokens >= (1u << 24)) return unsupported(name, "tokens must be under 2^24");
     if (b->query_starts_dev == nullptr || b->kv_lens_dev == nullptr || b->block_tables_dev == nullptr)
         return bad(name, "requires non-null query_starts, kv_lens and block_tables");
     if (!aligned(b->query_starts_dev, 4) || !aligned(b->kv_lens_dev, 4) || !aligned(b->block_tables_dev, 4))
@@ -137,7 +137,7 @@ Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, con
         if (!head_dim_ok(head_dim)) return unsupported(name, "head_dim must be 64, 128, 256 or 512");
         Gemma4Status st = check_rope(rope, head_dim, name, &a.rope);
         if (st != GEMMA4_OK) return st;
-        if (rows > (1u << 24)) return unsupported(name, "rows exceeds 2^24");
+        if (rows >= (1u << 24)) return unsupported(name, "rows must be under 2^24");
         if (rows == 0) return ok();
         st = check_heads(q, head_dim, true, "q", name, &a.part[0]);
         if (st == GEMMA4_OK && k != nullptr) st = check_heads(k, head_dim, true, "k", name, &a.part[1]);
@@ -216,6 +216,10 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
             return unsupported(name, "tokens * q_heads exceeds 2^31");
         kv::AttnPlan plan = kv::plan_attention(a);
         a.tile_from = plan.tile_from;
+        // a launch's threads are counted in 32 bits, 512 to a workgroup at most
+        for (const kv::Items* it : {&plan.tiles, &plan.rows})
+            if ((uint64_t)it->items * (uint64_t)it->parts >= (1u << 23))
+                return unsupported(name, "tokens * q_heads is too large for one launch");
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
         hipError_t e = hipGetDevice(&sc.device);

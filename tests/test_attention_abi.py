@@ -284,3 +284,19 @@ def test_header_says_what_the_library_has(lib):
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(hbuild.ROOT, "include", "gemma4_qmm.h")).read(), flags=re.S)
     for name in ("gemma4_qk_norm_rope", "gemma4_kv_append", "gemma4_kv_attention"):
         assert re.search(rf"Gemma4Status {name}\(", text) and hasattr(lib, name)
+
+
+@pytest.mark.parametrize("tokens,requests,kv_heads,text", [
+    (1 << 24, 1, 8, "2^24"),                      # tokens
+    ((1 << 24) - 1, 1, 256, "2^31"),              # rows of q
+    (1 << 20, 1 << 20, 16, "one launch"),         # a tile per request and KV head
+])
+def test_launches_too_large_are_refused(lib, tokens, requests, kv_heads, text):
+    b = batch(tokens=tokens, requests=requests)
+    pg = pages(kv_heads=kv_heads, page_stride=kv_heads * 16 * 256)
+    assert attention(lib, pg=pg, b=b, nq=kv_heads, q_stride=kv_heads * 256, out_stride=kv_heads * 256) == NO
+    assert text in qmm.last_error()
+    if tokens >= 1 << 24:
+        assert append(lib, pg=pg, b=b) == NO
+        assert lib.gemma4_qk_norm_rope(ctypes.byref(q_heads()), None, None, None, tokens, 256, None) == NO
+        assert text in qmm.last_error()
