@@ -193,6 +193,15 @@ def _output(out, shape, like, what: str):
     return out, stride
 
 
+def set_attention_kernel(kernel: int) -> int:
+    """Pins the attention kernel for this process: 0 (the default) chooses by the rows of each
+    request and the work of the call, 1 the 128-row tiles for every request with rows enough,
+    2 the 16-row tiles only.  Returns the previous setting."""
+    if int(kernel) not in (0, 1, 2):
+        raise ValueError(f"kernel must be 0, 1 or 2, got {kernel}")
+    return int(qmm.load_library().gemma4_kv_set_attention_kernel(int(kernel)))
+
+
 def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=None, out_k=None, stream=None):
     """Norms (where given) and rotates the heads of q [rows, heads, head_dim] and, unless
     None, of k, in one launch.  ``positions``: int32 [rows].  Returns (q, k) in new

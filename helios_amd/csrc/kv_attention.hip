@@ -488,13 +488,18 @@ int most_tiles(const AttnArgs& a, int tokens, int least, int most) {
     return (int)(by_rows < by_runs ? by_rows : by_runs);
 }
 
+// The most keys a tile of `tokens` can see.
+int64_t most_keys(const AttnArgs& a, int tokens) {
+    const int64_t keys = (int64_t)a.batch.width << a.pages.page_shift;
+    return a.window > 0 && keys > a.window + tokens ? a.window + tokens : keys;
+}
+
 // Items of a kernel's rows: `fill` workgroups fill the card.  No cuts where the tiles alone
 // fill it, or where no tile has keys for two items of `least_keys`.
 Items plan_items(const AttnArgs& a, const Shape& sh, int tiles, int fill, int least_keys) {
     Items it{};
     it.parts = a.pages.kv_heads * sh.chunks;
-    int64_t keys = (int64_t)a.batch.width << a.pages.page_shift;
-    if (a.window > 0 && keys > a.window + sh.tokens) keys = a.window + sh.tokens;
+    const int64_t keys = most_keys(a, sh.tokens);
     const int slots = fill / it.parts;
     it.slots = tiles < slots && keys >= 2 * least_keys ? slots : 0;
     it.items = it.slots + tiles;
@@ -508,12 +513,21 @@ AttnPlan plan_attention(const AttnArgs& a) {
     const int group = a.q_heads / a.pages.kv_heads;
     const int64_t tokens = a.batch.tokens, requests = a.batch.requests;
     const Shape wide = tile_shape(kWideRows, group), thin = tile_shape(kThinRows, group);
-    // A request goes to the 128-row tiles if it fills half of one.
-    const int from = ceil_div(64, wide.heads);
+    // A request goes to the 128-row tiles if it has 64 rows (96 of 64 dims): us of 16-row and of
+    // 128-row tiles, four requests of 32768 keys, 512 dims: 65 / 82 at 32 rows, 101 / 84 at 64;
+    // 256 dims: 222 / 223 and 363 / 227; 128 dims: 86 / 102 at 48, 154 / 101 at 96; 64 dims:
+    // 54 / 71 at 64, 95 / 70 at 128.  In a call of little work (rows x keys x dims under 8e8) the
+    // wide tiles' start costs more than they save: one request of 4096 keys, 512 dims, 256 rows
+    // (5e8) 33 / 39, eight of 128 rows (2e9) 60 / 48; 256 dims, window 1024, one of 128 tokens
+    // (6e8) 26.8 / 27.5; 64 dims, eight of 64 rows (5e8) 22 / 27, of 128 (1.1e9) 32 / 28.
+    const int from = ceil_div(a.pages.head_dim == 64 ? 96 : 64, wide.heads);
+    const double work = (double)tokens * a.q_heads * (double)most_keys(a, wide.tokens) * a.pages.head_dim;
     // One request: its kernel is known.  Several with a row each at least: none reaches
     // `from` rows if the sum stays under this (were some of them empty, the 16-row kernel
     // would still be right).
-    if (requests == 1)
+    if (a.kernel == 2 || (a.kernel == 0 && work < 8e8))
+        p.tile_from = kNoTiles;
+    else if (requests == 1)
         p.tile_from = tokens >= from ? 1 : kNoTiles;
     else
         p.tile_from = tokens >= from + requests - 1 ? from : kNoTiles;

@@ -60,6 +60,7 @@ struct AttnArgs {
     Batch batch;
     int q_heads, window;
     float scale;
+    int kernel;     // gemma4_kv_set_attention_kernel's setting
     int tile_from;  // requests of this many rows or more go to the 128-row tiles, the rest to rows16
 };
 

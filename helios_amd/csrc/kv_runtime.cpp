@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -13,6 +14,8 @@
 namespace {
 
 using namespace rt;
+
+std::atomic<uint32_t> g_attention_kernel{0};
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -128,6 +131,8 @@ Gemma4Status check_heads(const Gemma4Heads* h, uint32_t head_dim, bool has_out, 
 
 extern "C" {
 
+uint32_t gemma4_kv_set_attention_kernel(uint32_t kernel) { return g_attention_kernel.exchange(kernel > 2u ? 0u : kernel); }
+
 Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Rope* rope,
                                  const int32_t* positions_dev, uint32_t rows, uint32_t head_dim, void* stream) {
     try {
@@ -211,6 +216,7 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
         a.q_heads = (int)q_heads;
         a.window = (int)window;
         a.scale = scale;
+        a.kernel = (int)g_attention_kernel.load(std::memory_order_relaxed);
         // a launch's workgroups are counted in 31 bits
         if (((uint64_t)batch->tokens + batch->requests + 1) * q_heads > 0x7FFFFFFFull)
             return unsupported(name, "tokens * q_heads exceeds 2^31");

@@ -123,6 +123,7 @@ def load_library(path: str | None = None):
                                 ctypes.POINTER(vp)],
         "gemma4_qlora_free": [vp],
         "gemma4_qlinear_forward_lora": [vp, vp, vp, vp, ctypes.c_uint32, vp, ctypes.c_int],
+        "gemma4_kv_set_attention_kernel": [ctypes.c_uint32],
         "gemma4_qk_norm_rope": [vp, vp, vp, vp, ctypes.c_uint32, ctypes.c_uint32, vp],
         "gemma4_kv_append": [vp, vp, vp, vp, vp, vp, vp],
         "gemma4_kv_attention": [vp, vp, vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_float, ctypes.c_uint32, vp,
@@ -131,7 +132,7 @@ def load_library(path: str | None = None):
     for name, args in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args
-        fn.restype = ctypes.c_uint32 if name.startswith("gemma4_qmm_set_") else st
+        fn.restype = ctypes.c_uint32 if name.startswith(("gemma4_qmm_set_", "gemma4_kv_set_")) else st
     _lib = lib
     return lib
 

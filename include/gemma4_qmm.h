@@ -424,6 +424,15 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
                                  uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
                                  uint64_t out_stride, float* lse_dev, void* stream);
 
+/* Attention kernels of this process.  No counterpart in the reference; for tests and
+ * benchmarks that pin a kernel.
+ *   0 (the default): by the rows of each request and the work of the call.
+ *   1: 128-row tiles for every request that has rows enough, however small the call.
+ *   2: 16-row tiles only.
+ * Both meet the same accuracy contract and sum in different orders.  Values above 2 are
+ * taken as 0.  Returns the previous setting; takes effect for calls issued after it returns. */
+uint32_t gemma4_kv_set_attention_kernel(uint32_t kernel);
+
 #ifdef __cplusplus
 }
 #endif

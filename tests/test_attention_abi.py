@@ -300,3 +300,11 @@ def test_launches_too_large_are_refused(lib, tokens, requests, kv_heads, text):
         assert append(lib, pg=pg, b=b) == NO
         assert lib.gemma4_qk_norm_rope(ctypes.byref(q_heads()), None, None, None, tokens, 256, None) == NO
         assert text in qmm.last_error()
+
+
+def test_the_attention_kernel_setting(lib):
+    assert A.set_attention_kernel(2) == 0 and lib.gemma4_kv_set_attention_kernel(7) == 2  # 7 is taken as 0
+    assert A.set_attention_kernel(0) == 0
+    for bad in (-1, 3):
+        with pytest.raises(ValueError):
+            A.set_attention_kernel(bad)

@@ -2,6 +2,7 @@
 GPU through the Python API, against the 64-bit implementations and bounds of
 attention_oracle.py."""
 
+import contextlib
 import math
 
 import numpy as np
@@ -27,6 +28,17 @@ def randn(rng, *shape):
 
 def inv_freq(pairs, base=1e4):
     return (base ** (-np.arange(pairs) / pairs)).astype(np.float32)
+
+
+@contextlib.contextmanager
+def kernel(k):
+    from helios_amd import attention as A
+
+    before = A.set_attention_kernel(k)
+    try:
+        yield
+    finally:
+        A.set_attention_kernel(before)
 
 
 # ------------------------------------------------------------------ norm and rotation
@@ -208,6 +220,12 @@ def attend_case(rng, d, hq, hk, q_lens, kv_lens, page, kind="bf16", window=0, pa
     want, bound, wl, lb = O.attend(O.f64(q), k64, v64, b, scale, window)
     O.assert_within(O.f64(out), want, bound, "out")
     O.assert_within(O.f64(lse), wl, lb, "lse")
+    for k in (1, 2):  # each kernel, whatever the call's size
+        with kernel(k):
+            pinned, pinned_lse = cache.attend(q, batch, scale=scale, window=window, return_lse=True)
+            assert torch.equal(cache.attend(q, batch, scale=scale, window=window), pinned), "two runs differ"
+        O.assert_within(O.f64(pinned), want, bound, f"out, kernel {k}")
+        O.assert_within(O.f64(pinned_lse), wl, lb, f"lse, kernel {k}")
     return out, lse, b, cache, batch, q, (k64, v64)
 
 
@@ -309,18 +327,23 @@ def test_infinities_and_nan_in_hidden_places(gpu_lib, d, hq, hk, kind, q_len, kv
         value = odd[n % 3]
         cache.v.view(torch.uint8 if kind == "e4m3" else torch.bfloat16)[page, h, slot, e] = 0x7F if kind == "e4m3" else value
         v64[page, h, slot, e] = value
-    out, lse = cache.attend(q, batch, window=window, return_lse=True)
     want, bound, wl, lb = O.attend(O.f64(q), k64, v64, b, d ** -0.5, window)
-    O.assert_within(O.f64(out), want, bound, "values")
-    O.assert_within(O.f64(lse), wl, lb, "lse")
+    group = hq // hk
+    outs = {}
+    for k in (1, 2):
+        with kernel(k):
+            outs[k], lse = cache.attend(q, batch, window=window, return_lse=True)
+        O.assert_within(O.f64(outs[k]), want, bound, f"values, kernel {k}")
+        O.assert_within(O.f64(lse), wl, lb, f"lse, kernel {k}")
     # a NaN key: rows that see it are NaN, the others as before
     page, slot = O.slot_of(b, 0, kv_len - 1)
     cache.k.view(torch.uint8 if kind == "e4m3" else torch.bfloat16)[page, 0, slot, 0] = 0x7F if kind == "e4m3" else float("nan")
-    got = cache.attend(q, batch, window=window)
-    group = hq // hk
-    assert bool(got[-1, :group].isnan().all())
-    assert torch.equal(got[:-1].nan_to_num(7, 8, 9), out[:-1].nan_to_num(7, 8, 9))
-    assert torch.equal(got[-1, group:].nan_to_num(7, 8, 9), out[-1, group:].nan_to_num(7, 8, 9))
+    for k, out in outs.items():
+        with kernel(k):
+            got = cache.attend(q, batch, window=window)
+        assert bool(got[-1, :group].isnan().all())
+        assert torch.equal(got[:-1].nan_to_num(7, 8, 9), out[:-1].nan_to_num(7, 8, 9))
+        assert torch.equal(got[-1, group:].nan_to_num(7, 8, 9), out[-1, group:].nan_to_num(7, 8, 9))
 
 
 def test_scales_and_extreme_scores(gpu_lib):
