@@ -122,7 +122,8 @@ struct Tile {
 // into runs of `tokens`; their key ranges counted in units of `unit` keys, and cut so that
 // there are about `slots` items (at most slots + the number of tiles; 0: no cuts).
 struct Cuts {
-    int tokens, least, most, unit, slots, min_units, window;
+    int tokens, least, most, unit, slots, window;
+    int min_units, few_units;  // the least units of an item; where all units are fewer than the slots
 };
 
 // Item number `index` of the launch, or (BY_TILE) its tile number `index` as split 0; n = 0
@@ -175,7 +176,8 @@ __device__ __forceinline__ Tile find_item(const Batch& b, int page_shift, const 
         }
         const float cost_alike = (float)parts(items_alike, cuts.slots) * (float)alike;
         per = (float)parts(items_even, cuts.slots) * (float)even < cost_alike ? even : alike;
-        if (per < cuts.min_units) per = cuts.min_units;
+        const int floor = sum <= (float)cuts.slots ? cuts.few_units : cuts.min_units;
+        if (per < floor) per = floor;
     }
     int before = 0, before_items = 0;
     for (int base = 0; base <= b.requests; base += 64) {
@@ -223,14 +225,16 @@ __host__ __device__ inline Shape tile_shape(int rows, int group) {
     return s;
 }
 
-// Units are what a workgroup takes in one step; an item is of 256 keys at least.
+// Units are what a workgroup takes in one step; an item is of 256 keys at least, of 128 where
+// even so half the card is idle (four single tokens over 246 to 3316 keys of 512 dims: 17.8 us
+// in place of 23; one over 32768, where the items are many, 21 either way and its join 8 for 6).
 constexpr int kRowsUnit = 64, kTileUnit = 32;
-constexpr int kRowsLeast = 256, kTileLeast = 256, kTileFill = 256;
+constexpr int kRowsLeast = 256, kRowsFew = 128, kTileLeast = 256, kTileFill = 256;
 __host__ __device__ inline Cuts rows_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {
-    return Cuts{sh.tokens, 1, a.tile_from - 1, kRowsUnit, it.slots, kRowsLeast / kRowsUnit, a.window};
+    return Cuts{sh.tokens, 1, a.tile_from - 1, kRowsUnit, it.slots, a.window, kRowsLeast / kRowsUnit, kRowsFew / kRowsUnit};
 }
 __host__ __device__ inline Cuts tile_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {
-    return Cuts{sh.tokens, a.tile_from, kNoTiles, kTileUnit, it.slots, kTileLeast / kTileUnit, a.window};
+    return Cuts{sh.tokens, a.tile_from, kNoTiles, kTileUnit, it.slots, a.window, kTileLeast / kTileUnit, kTileLeast / kTileUnit};
 }
 
 // Adds the infinities and NaN of groups that some row does not see to the outputs of the
