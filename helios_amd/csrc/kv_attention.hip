@@ -34,6 +34,8 @@ constexpr int kWaves = 4;
 
 // Workgroups of rows16 that run at once: one per CU at head_dim 512 (registers), else two.
 int rows_fill(const AttnArgs& a) { return a.pages.head_dim == 512 ? 256 : 512; }
+// Those of the 128-row tiles: one per CU, two of the smaller heads (registers and LDS).
+int tiles_fill(const AttnArgs& a) { return a.pages.head_dim >= 256 ? 256 : 512; }
 
 template <int D, bool FP8>
 struct Rows16 {
@@ -533,7 +535,7 @@ AttnPlan plan_attention(const AttnArgs& a) {
         p.tile_from = tokens >= from + requests - 1 ? from : kNoTiles;
     p.use_rows = p.tile_from > 1;
     p.use_tiles = p.tile_from != kNoTiles;
-    if (p.use_tiles) p.tiles = plan_items(a, wide, most_tiles(a, wide.tokens, p.tile_from, kNoTiles), kTileFill, kTileLeast);
+    if (p.use_tiles) p.tiles = plan_items(a, wide, most_tiles(a, wide.tokens, p.tile_from, kNoTiles), tiles_fill(a), kTileLeast);
     if (p.use_rows) p.rows = plan_items(a, thin, most_tiles(a, thin.tokens, 1, p.tile_from - 1), rows_fill(a), kRowsLeast);
     return p;
 }

@@ -229,7 +229,7 @@ __host__ __device__ inline Shape tile_shape(int rows, int group) {
 // even so half the card is idle (four single tokens over 246 to 3316 keys of 512 dims: 17.8 us
 // in place of 23; one over 32768, where the items are many, 21 either way and its join 8 for 6).
 constexpr int kRowsUnit = 64, kTileUnit = 32;
-constexpr int kRowsLeast = 256, kRowsFew = 128, kTileLeast = 256, kTileFill = 256;
+constexpr int kRowsLeast = 256, kRowsFew = 128, kTileLeast = 256;
 __host__ __device__ inline Cuts rows_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {
     return Cuts{sh.tokens, 1, a.tile_from - 1, kRowsUnit, it.slots, a.window, kRowsLeast / kRowsUnit, kRowsFew / kRowsUnit};
 }

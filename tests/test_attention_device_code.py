@@ -86,3 +86,18 @@ def test_attention_register_and_lds_budgets(tile_asm):
     assert len(lds) >= len(TILES) and max(lds) <= 160 * 1024
     for name, vgprs, private in _kernel_meta(hbuild.device_asm("kv_heads.hip")):
         assert private == 0 and vgprs <= 80, f"{name}: {vgprs} VGPRs"
+
+
+def test_two_tiles_of_small_heads_share_a_cu(tile_asm):
+    """The planner counts on it: at most 256 VGPRs and half of the LDS up to head_dim 128; one
+    workgroup of two waves per SIMD at 256."""
+    seen = 0
+    for m in re.finditer(r"- \.agpr_count:.*?\.group_segment_fixed_size:\s+(\d+).*?\.name:\s+\S+tile_kernelILi(\d+)E.*?\.vgpr_count:\s+(\d+)",
+                         tile_asm, re.S):
+        lds, d, vgprs = (int(m.group(i)) for i in (1, 2, 3))
+        if d <= 256:
+            assert vgprs <= 256, (d, vgprs)
+        if d <= 128:
+            assert lds <= 80 * 1024, (d, lds)
+        seen += 1
+    assert seen == len(TILES)
