@@ -247,7 +247,10 @@ __device__ void fix_nonfinite(const AttnArgs& a, const Tile& t, const Shape& sh,
     const Pages& pg = a.pages;
     for (int key = lo; key < hi; ++key) {
         const int base = key & ~(granule - 1);
-        if (all_visible(base, granule, t.pos0, t.n, a.window)) continue;
+        if (all_visible(base, granule, t.pos0, t.n, a.window)) {
+            key = base + granule - 1;  // none of the group's
+            continue;
+        }
         const int page = page_at(table, key >> pg.page_shift, a.batch.width, pg.num_pages);
         if (page < 0) continue;
         const int64_t off = (int64_t)page * pg.page_stride + (int64_t)kv_head * pg.head_stride +

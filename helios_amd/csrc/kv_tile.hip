@@ -25,8 +25,8 @@
 // the loads of V tile i + 1.  (Scores first and V after them, in two blocks: 1095 us at 2048
 // tokens over 16384 keys, 16 heads of 512 over one; in turns of four products 1070; in turns of
 // one 971, 1.06 PFLOP/s.)  A wave issues an instruction every 6 cycles at best, five beside a
-// product of 32, and a step has some six: that, and the time at its barrier, is what keeps it
-// from the library product's 1.24 PFLOP/s.  Loads of V take 16 bytes a lane, two keys at once:
+// product of 32, and a step has 316 beside its 64 products: that, and the time at its barrier,
+// is what keeps it from the library product's 1.24 PFLOP/s.  Loads of V take 16 bytes a lane, two keys at once:
 // the vector memory path moves 64 B a cycle, and a wave that waits for it issues no products.
 //
 // head_dim 256 has the registers for two waves per SIMD: eight waves, tiles of 64 keys; wave w
@@ -306,14 +306,20 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
     const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)stage;
     // this lane's row among a DMA's and its chunk there; the DMA's first key adds its own bits
     // (swizzle(key + i) = swizzle(key) ^ swizzle(i) for i < kDmaKeys)
-    const auto dma_k = [&](__amdgpu_buffer_rsrc_t r, uint32_t buffer, int j, int ln) {
+    struct DmaBase {
+        uint32_t to, swz;
+    };
+    const auto dma_base = [&]() {
+        DmaBase d{k_lds + (uint32_t)first_dma * 1024u, 16u * (uint32_t)swizzle<C::kCpr>(first_key)};
+        asm volatile("" : "+s"(d.to), "+s"(d.swz));  // sums with it are cheap to make again and dear to keep
+        return d;
+    };
+    const auto dma_k = [&](__amdgpu_buffer_rsrc_t r, uint32_t buffer, int j, int ln, const DmaBase& d) {
         const uint32_t dma_row = C::kDmaKeys == 1 ? 0u : ((uint32_t)ln / C::kCpr) * row_bytes;
         const uint32_t dma_chunk = 16u * (((uint32_t)ln & (C::kCpr - 1)) ^ (C::kDmaKeys == 1 ? 0u : (uint32_t)swizzle<C::kCpr>(ln / C::kCpr)));
         const int key = first_key + j * C::kDmaKeys;
-        uint32_t to = k_lds + (uint32_t)first_dma * 1024u, swz = 16u * (uint32_t)swizzle<C::kCpr>(first_key);
-        asm volatile("" : "+s"(to), "+s"(swz));  // sums are cheap to make again and dear to keep
-        swz = 16u * (uint32_t)swizzle<C::kCpr>(j * C::kDmaKeys) ^ swz;
-        q4::dma16_at(r, to + buffer * (uint32_t)C::kTileBytes + (uint32_t)j * 1024u, dma_row + (dma_chunk ^ swz),
+        const uint32_t swz = 16u * (uint32_t)swizzle<C::kCpr>(j * C::kDmaKeys) ^ d.swz;
+        q4::dma16_at(r, d.to + buffer * (uint32_t)C::kTileBytes + (uint32_t)j * 1024u, dma_row + (dma_chunk ^ swz),
                      (uint32_t)(key % kGroupKeys) * row_bytes);
     };
 
@@ -447,9 +453,9 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
         move_window(0, pages);
         const __amdgpu_buffer_rsrc_t k0 = k_source(0), k1 = k_source(1), k2 = k_source(2);
 #pragma unroll
-        for (int j = 0; j < kWaveDmas; ++j) dma_k(k0, 0, j, lane);
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k0, 0, j, lane, dma_base());
 #pragma unroll
-        for (int j = 0; j < kWaveDmas; ++j) dma_k(k1, 1, j, lane);
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k1, 1, j, lane, dma_base());
         q4::wait_vm_lds<0>();
         q4::lds_barrier();
 #pragma unroll
@@ -476,7 +482,7 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
             q4::lds_barrier();
         }
 #pragma unroll
-        for (int j = 0; j < kWaveDmas; ++j) dma_k(k2, 0, j, lane);
+        for (int j = 0; j < kWaveDmas; ++j) dma_k(k2, 0, j, lane, dma_base());
 #pragma unroll
         for (int st = 0; st < kSt; ++st) {
             const __amdgpu_buffer_rsrc_t r = v_source(st);
@@ -561,6 +567,8 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
 #pragma unroll
             for (int j = 0; j < 4; ++j) transposed(0, j, av);
             __amdgpu_buffer_rsrc_t kr, vr[kSt];
+            constexpr bool kManyDmas = kWaveDmas >= 8;  // enough to keep their base in registers
+            const DmaBase kd = kManyDmas ? dma_base() : DmaBase{};
             f32x16 s_new = {};
             const float base = m == kNegInf ? 0.0f : m;
             constexpr int kTurns = kSlices * E;  // one product of each kind, and a share of the rest
@@ -588,7 +596,7 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
                 if (late < 0) {
 #pragma unroll
                     for (int j = kWaveDmas * at / kMid; j < kWaveDmas * (at + 1) / kMid; ++j)
-                        dma_k(kr, (uint32_t)(par ^ 1), j, C::kDmaKeys == 1 ? ln : lane);
+                        dma_k(kr, (uint32_t)(par ^ 1), j, kManyDmas ? ln : lane, kManyDmas ? kd : dma_base());
                 } else {
 #pragma unroll
                     for (int j = 4 * kSt * late / kMid; j < 4 * kSt * (late + 1) / kMid; ++j) v[j / 4][j % 4] = fetch_v(vr[j / 4], j % 4);
