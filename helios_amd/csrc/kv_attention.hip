@@ -469,7 +469,7 @@ hipError_t launch_join(const AttnArgs& a, const Items& it, const Cuts& cuts, int
     const int64_t live = (int64_t)a.batch.tokens * heads;
     const int work = (int)(live < rows ? live : rows) * slices;
     const bool many = (int64_t)a.batch.tokens * a.q_heads * slices >= 2048;
-    const int most = many ? ceil_div(work, 16) : work, fill = ceil_div(1024, tiles);
+    const int most = many ? ceil_div(work, 16) : work, fill = ceil_div(2048, tiles);
     const int y = most < fill ? most : fill;
     const dim3 grid((unsigned)tiles, (unsigned)y);
     switch (a.pages.head_dim) {
