@@ -158,7 +158,7 @@ class KVBatch:
         if query_starts.shape[0] != n + 1 or block_tables.shape[0] != n:
             raise _invalid(f"query_starts must have one entry more than kv_lens and block_tables as many rows ({n})")
         width = block_tables.shape[1]
-        stride = block_tables.stride(0) if n > 1 else max(width, block_tables.stride(0))
+        stride = block_tables.stride(0) if n > 1 else width  # a single row's stride says nothing
         if stride < width:
             raise _invalid("block_tables' rows overlap")
         self.requests = n

@@ -75,6 +75,7 @@ Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const c
         return bad(name, "the batch's arrays must be 4-byte aligned");
     if (b->pages_per_request == 0 || b->table_stride < b->pages_per_request)
         return bad(name, "pages_per_request must be > 0 and at most table_stride");
+    if (b->table_stride > 0x7FFFFFFFu) return unsupported(name, "table_stride must be under 2^31");  // an int in the kernels
     if (((uint64_t)b->pages_per_request << pages.page_shift) > ((uint64_t)1 << 30))
         return unsupported(name, "a request's pages exceed 2^30 tokens");
     out->starts = b->query_starts_dev;

@@ -364,7 +364,7 @@ typedef struct Gemma4KvPages {
  *   query_starts_dev  int32 [requests + 1], nondecreasing from 0; rows past the last are
  *                     padding: nothing is stored for them and their outputs are zeros
  *   kv_lens_dev       int32 [requests], the new tokens included
- *   block_tables_dev  int32 [requests, table_stride], pages_per_request entries used.  An
+ *   block_tables_dev  int32 [requests, table_stride < 2^31], pages_per_request entries used.  An
  *                     entry outside [0, num_pages) is an absent page: append stores
  *                     nothing there, attention sees no keys there */
 typedef struct Gemma4KvBatch {
