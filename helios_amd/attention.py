@@ -96,13 +96,17 @@ def _heads_tensor(t, what: str, head_dim: int | None = None):
     return shape, row_stride if rows > 1 else max(row_stride, heads * dim)
 
 
-def _on(index, *tensors):
-    """Every tensor must live on GPU `index`, which must be the current device."""
+def _on(index, tensors, held):
+    """Every tensor, and what the rotations, norms and batches hold, must live on GPU `index`,
+    which must be the current device."""
     import torch
 
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise _invalid("all tensors must be on one device")
+    for h in held:
+        if h is not None and h._device not in (index, None):
+            raise _invalid(f"a {type(h).__name__} is on cuda:{h._device}, the other tensors on cuda:{index}")
     if torch.cuda.current_device() != index:
         raise _invalid(f"the tensors are on cuda:{index}, which is not the current device")
 
@@ -119,6 +123,7 @@ class Rope:
         if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_cuda:
             raise _invalid("inv_freq must be a one-dimensional float32 tensor on the GPU")
         self.inv_freq = inv_freq.contiguous()
+        self._device = inv_freq.get_device()
         pairs = inv_freq.numel()
         self.distance = pairs if distance is None else int(distance)
         if self.distance < 0:
@@ -141,6 +146,7 @@ class HeadNorm:
         self.eps = float(eps)
         self.size = 0 if weight is None else weight.numel()
         self._ptr = 0 if weight is None else weight.data_ptr()
+        self._device = None if weight is None else weight.get_device()  # None: on any
 
 
 class KVBatch:
@@ -163,6 +169,8 @@ class KVBatch:
             raise _invalid("block_tables' rows overlap")
         self.requests = n
         self._device = kv_lens.get_device()
+        if query_starts.get_device() != self._device or block_tables.get_device() != self._device:
+            raise _invalid("query_starts, kv_lens and block_tables must be on one device")
         self._fields = (query_starts.data_ptr(), kv_lens.data_ptr(), block_tables.data_ptr(), n)
         self._table = (width, stride)
         self._packed = (-1, b"")
@@ -227,7 +235,7 @@ def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=Non
         of_k = _heads(k, k_shape, k_stride, k_norm, out_k.data_ptr(), out_stride)
     else:
         out_k = None
-    _on(q.get_device(), k, positions, out_q, out_k)
+    _on(q.get_device(), (k, positions, out_q, out_k), (rope, q_norm, k_norm))
     status = lib.gemma4_qk_norm_rope(of_q, of_k, None if rope is None else rope._ref,
                                      None if positions is None else positions.data_ptr(), rows, head_dim,
                                      qmm._stream_ptr(stream))
@@ -298,7 +306,7 @@ class PagedKVCache:
             of_q = _heads(q, q_shape, q_stride, q_norm, out_q.data_ptr(), out_stride)
         else:
             out_q = None
-        _on(self._device, k, v, q, out_q, batch.kv_lens)
+        _on(self._device, (k, v, q, out_q), (batch, rope, k_norm, v_norm, q_norm))
         status = self._lib.gemma4_kv_append(self._ref, batch._struct(rows), of_q,
                                             _heads(k, shape, k_stride, k_norm, 0, 0), _heads(v, v_shape, v_stride, v_norm, 0, 0),
                                             None if rope is None else rope._ref, qmm._stream_ptr(stream))
@@ -320,7 +328,7 @@ class PagedKVCache:
             raise _invalid("window must be >= 0 (0: none)")
         out, out_stride = _output(out, shape, q, "out")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
-        _on(self._device, q, out, batch.kv_lens)
+        _on(self._device, (q, out), (batch,))
         status = self._lib.gemma4_kv_attention(self._ref, batch._struct(rows), q.data_ptr(), q_stride, heads,
                                                self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
                                                out_stride, None if lse is None else lse.data_ptr(),

@@ -3,10 +3,13 @@ sizes past 32 bits, tensors on several GPUs.  No kernel runs: pointers are check
 followed, and the tensors of the Python checks are fake ones (shapes, strides and devices
 without memory)."""
 
+import warnings
+
 import pytest
 
+from helios_amd import attention as A
 from helios_amd import qmm
-from test_attention_abi import NO, append, attention, batch, lib  # noqa: F401
+from test_attention_abi import BAD, NO, append, attention, batch, lib  # noqa: F401
 
 
 @pytest.mark.parametrize("stride", [1 << 31, (1 << 32) - 4])
@@ -15,3 +18,72 @@ def test_a_table_stride_past_31_bits_is_refused(lib, stride):  # noqa: F811
     for call in (attention, append):
         assert call(lib, b=batch(table_stride=stride)) == NO
         assert "table_stride" in qmm.last_error()
+
+
+# ------------------------------------------------------------------ tensors on several GPUs
+
+class Took(Exception):
+    """The call went through to the library."""
+
+
+class NoLibrary:
+    def __getattr__(self, name):
+        def call(*args):
+            raise Took(name)
+
+        return call
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Fake CUDA tensors on a machine without a GPU; device 0 is current."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(A.qmm, "load_library", NoLibrary)
+    monkeypatch.setattr(A.qmm, "_stream_ptr", lambda stream: 0)
+    with warnings.catch_warnings(), FakeTensorMode():
+        warnings.simplefilter("ignore")  # fake tensors' addresses are 0
+        yield lambda *shape, dtype=torch.bfloat16, gpu=0: torch.empty(shape, dtype=dtype, device=f"cuda:{gpu}")
+
+
+def calls(fake, **gpu):
+    """(name, call) of every entry point, with tensor `name` of each on GPU gpu[name]."""
+    import torch
+
+    at = lambda name: gpu.get(name, 0)  # noqa: E731
+    i32 = lambda name, *shape: fake(*shape, dtype=torch.int32, gpu=at(name))  # noqa: E731
+    rope = A.Rope(fake(64, dtype=torch.float32, gpu=at("inv_freq")))
+    norms = {f"{w}_norm": A.HeadNorm(fake(128, gpu=at(f"{w}_norm"))) for w in "qkv"}
+    q, k, v = (fake(3, n, 128, gpu=at(w)) for n, w in ((4, "q"), (2, "k"), (2, "v")))
+    two = norms["q_norm"], norms["k_norm"]
+    yield "qk_norm_rope", lambda: A.qk_norm_rope(q, k, i32("positions", 3), rope, *two)
+    cache = A.PagedKVCache(*[fake(5, 2, 16, 128, gpu=at("pages")) for _ in "kv"])
+    def batch():
+        return A.KVBatch(i32("query_starts", 3), i32("kv_lens", 2), i32("block_tables", 2, 4))
+    yield "append", lambda: cache.append(k, v, batch(), rope=rope, q=q, **norms)
+    yield "attend", lambda: cache.attend(q, batch())
+
+
+def test_tensors_on_the_current_gpu_are_taken(fake):
+    for name, call in calls(fake):
+        with pytest.raises(Took):
+            call()
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "positions", "inv_freq", "q_norm", "k_norm", "v_norm", "pages", "query_starts",
+                                   "kv_lens", "block_tables"])
+def test_a_tensor_on_another_gpu_is_refused(fake, where):
+    """Whichever it is: its address would be handed to a kernel of the current GPU."""
+    used = {"qk_norm_rope": {"q", "k", "positions", "inv_freq", "q_norm", "k_norm"},
+            "append": {"q", "k", "v", "inv_freq", "q_norm", "k_norm", "v_norm", "pages", "query_starts", "kv_lens", "block_tables"},
+            "attend": {"q", "pages", "query_starts", "kv_lens", "block_tables"}}
+    for name, call in calls(fake, **{where: 1}):
+        if where in used[name]:
+            with pytest.raises(qmm.Gemma4Error) as e:
+                call()
+            assert e.value.status == BAD, name
+        else:
+            with pytest.raises(Took):
+                call()
