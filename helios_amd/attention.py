@@ -21,6 +21,9 @@ One layer of a decoding step, from the fused projection's rows to o's input::
 
 Tensors are bf16 on the GPU (pages may be ``float8_e4m3fn``).  The device arrays of a
 batch are read when the kernels run, so a captured graph follows what is written to them.
+With ``stream`` a call runs there instead of on torch's current stream: its inputs must be
+ready on that stream and stay until it is done with them, and the outputs it makes belong to
+that stream's memory (use them elsewhere after waiting for it).
 Errors surface as :class:`~helios_amd.qmm.Gemma4Error`; there is no fallback.
 """
 
@@ -191,10 +194,21 @@ def _heads(t, shape, stride, norm, out, out_stride):
     return _pack_heads(t.data_ptr(), out, norm._ptr, stride, out_stride, shape[1], 1, norm.eps)
 
 
-def _output(out, shape, like, what: str):
-    """(tensor, row stride) of an output of `shape`."""
+def _new(like, shape, dtype, stream):
+    """A tensor that `stream` writes, from its memory: that of torch's current stream may still
+    be in use there."""
+    import torch
+
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _output(out, shape, like, what: str, stream):
+    """(tensor, row stride) of an output of `shape` that `stream` writes."""
     if out is None:
-        return like.new_empty(shape), shape[1] * shape[2]
+        return _new(like, shape, None, stream), shape[1] * shape[2]
     got, stride = _heads_tensor(out, what)
     if got != shape:
         raise _invalid(f"{what} has the wrong shape")
@@ -227,11 +241,11 @@ def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=Non
             raise _invalid(f"positions must have {rows} entries")
     else:
         positions = None
-    out_q, out_stride = _output(out_q, shape, q, "out_q")
+    out_q, out_stride = _output(out_q, shape, q, "out_q", stream)
     of_q = _heads(q, shape, q_stride, q_norm, out_q.data_ptr(), out_stride)
     of_k = None
     if k is not None:
-        out_k, out_stride = _output(out_k, k_shape, k, "out_k")
+        out_k, out_stride = _output(out_k, k_shape, k, "out_k", stream)
         of_k = _heads(k, k_shape, k_stride, k_norm, out_k.data_ptr(), out_stride)
     else:
         out_k = None
@@ -302,7 +316,7 @@ class PagedKVCache:
             q_shape, q_stride = _heads_tensor(q, "q", self.head_dim)
             if q_shape[0] != rows:
                 raise _invalid("q, k and v must have the same rows")
-            out_q, out_stride = _output(out_q, q_shape, q, "out_q")
+            out_q, out_stride = _output(out_q, q_shape, q, "out_q", stream)
             of_q = _heads(q, q_shape, q_stride, q_norm, out_q.data_ptr(), out_stride)
         else:
             out_q = None
@@ -326,8 +340,8 @@ class PagedKVCache:
         rows, heads, _ = shape
         if window < 0:
             raise _invalid("window must be >= 0 (0: none)")
-        out, out_stride = _output(out, shape, q, "out")
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        out, out_stride = _output(out, shape, q, "out", stream)
+        lse = _new(q, (rows, heads), torch.float32, stream) if return_lse else None
         _on(self._device, (q, out), (batch,))
         status = self._lib.gemma4_kv_attention(self._ref, batch._struct(rows), q.data_ptr(), q_stride, heads,
                                                self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),

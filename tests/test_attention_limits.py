@@ -3,9 +3,11 @@ sizes past 32 bits, tensors on several GPUs.  No kernel runs: pointers are check
 followed, and the tensors of the Python checks are fake ones (shapes, strides and devices
 without memory)."""
 
+import contextlib
 import warnings
 
 import pytest
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from helios_amd import attention as A
 from helios_amd import qmm
@@ -87,3 +89,57 @@ def test_a_tensor_on_another_gpu_is_refused(fake, where):
         else:
             with pytest.raises(Took):
                 call()
+
+
+# ------------------------------------------------------------------ outputs on a named stream
+
+class Made(TorchDispatchMode):
+    """Records, for each tensor operation, the stream that is current."""
+
+    def __init__(self, current):
+        super().__init__()
+        self.current, self.on = current, []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace == "aten":
+            self.on.append((str(func), self.current[-1]))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.fixture
+def made(fake, monkeypatch):
+    """(fake, record(call)): the operations of `call` up to the library's own, with their streams."""
+    import torch
+
+    current = ["current"]
+
+    @contextlib.contextmanager
+    def stream(s):
+        current.append(s)
+        yield
+        current.pop()
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+
+    def record(call):
+        with Made(current) as mode, pytest.raises(Took):
+            call()
+        return mode.on
+
+    return fake, record
+
+
+def test_outputs_belong_to_the_stream_that_writes_them(made):
+    """Memory taken on the current stream may still be in use there when another stream writes it."""
+    import torch
+
+    fake, record = made
+    i32 = lambda *shape: fake(*shape, dtype=torch.int32)  # noqa: E731
+    batch = A.KVBatch(i32(3), i32(2), i32(2, 4))
+    cache = A.PagedKVCache(fake(5, 2, 16, 128), fake(5, 2, 16, 128))
+    q, k = fake(3, 4, 128), fake(3, 2, 128)
+    for call in (lambda s: A.qk_norm_rope(q, k, None, stream=s), lambda s: cache.append(k, k, batch, q=q, stream=s),
+                 lambda s: cache.attend(q, batch, return_lse=True, stream=s)):
+        for s in (None, "side"):
+            on = record(lambda: call(s))
+            assert on and all(where == (s or "current") for _, where in on), on

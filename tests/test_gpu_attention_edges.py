@@ -1,0 +1,45 @@
+"""The paged-cache calls on the GPU at the edges of what they take: outputs on a named stream."""
+
+import numpy as np
+import pytest
+
+import attention_oracle as O
+from test_gpu_attention import attend_case, dev, inv_freq, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def stream_of(t):
+    """The stream whose memory holds t (the allocator's own record; 0: the default stream's)."""
+    import torch
+
+    for s in torch.cuda.memory_snapshot():
+        if s["address"] <= t.data_ptr() < s["address"] + s["total_size"]:
+            return s["stream"]
+    raise AssertionError("not the allocator's memory")
+
+
+def test_outputs_on_a_named_stream(gpu_lib):
+    """An output that a call makes belongs to the stream it is written on, and equals that of
+    the call on the current stream."""
+    import torch
+
+    from helios_amd import attention as A
+
+    rng = np.random.default_rng(61)
+    out, lse, b, cache, batch, q, _ = attend_case(rng, 128, 8, 4, [30, 1], [100, 700], 32)
+    k = randn(rng, b["rows"], 4, 128)
+    pos, rope = dev(np.arange(b["rows"], dtype=np.int32)), A.Rope(dev(inv_freq(64)))
+    turned = A.qk_norm_rope(q, k, pos, rope)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    # attention before the append, which changes the cache
+    got = list(cache.attend(q, batch, return_lse=True, stream=side)) + list(A.qk_norm_rope(q, k, pos, rope, stream=side))
+    appended = cache.append(k, k, batch, q=q, stream=side)
+    side.synchronize()
+    for t in got + [appended]:
+        assert stream_of(t) == side.cuda_stream
+    for t, want in zip(got, (out, lse, *turned)):
+        assert torch.equal(t, want)
+    assert stream_of(out) != side.cuda_stream
+    assert np.array_equal(O.f64(appended), O.f64(q))
