@@ -18,6 +18,10 @@ last-error text, as the reference's Rust wrapper does with ``check()``
 (``crates/gemma4d-ffi/src/lib.rs:1409-1433``).  Torch supplies device memory and
 the current stream only; all arithmetic runs in the HIP kernels.  There is no
 fallback: without the built library every call raises.
+
+With ``stream`` a call runs there instead of on torch's current stream: its inputs must be
+ready on that stream and stay until it is done with them, and the tensors it makes belong to
+that stream's memory (use them elsewhere after waiting for it).
 """
 
 from __future__ import annotations
@@ -233,6 +237,32 @@ def _stream_ptr(stream) -> int:
     return stream.cuda_stream
 
 
+def _made_on(stream):
+    """Where a call that runs on `stream` makes its tensors (outputs, contiguous copies): memory
+    of torch's current stream may still be in use there, and a copy made there would not be
+    waited for."""
+    import torch
+
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _empty(shape, dtype, device, stream):
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with _made_on(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _rows(x, features: int, stream):
+    """x as contiguous [rows, features]."""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
+    with _made_on(stream):
+        return x.reshape(-1, features).contiguous()
+
+
 def _dev_ptr(t) -> int:
     return t.data_ptr()
 
@@ -257,12 +287,13 @@ def _host_triple(weight, scales, biases, n: int, k: int, group_size: int, bits: 
     return w, s, b
 
 
-def _device_triple(weight, scales, biases, n: int, k: int, group_size: int, bits: int):
+def _device_triple(weight, scales, biases, n: int, k: int, group_size: int, bits: int, stream):
     import torch
 
-    w = weight.contiguous()
-    s = scales.contiguous()
-    b = biases.contiguous()
+    with _made_on(stream):
+        w = weight.contiguous()
+        s = scales.contiguous()
+        b = biases.contiguous()
     if w.dtype not in (torch.int32, torch.uint32) or s.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         raise Gemma4Error(Status.INVALID_ARGUMENT, "weight must be int32/uint32 and scales/biases bfloat16")
     wc = k * bits // 32
@@ -289,10 +320,10 @@ def _run_forward(fn, handle, lib, x, in_features: int, out_features: int, out=No
     if x.shape[-1] != in_features:
         raise Gemma4Error(Status.INVALID_ARGUMENT, f"x last dim {x.shape[-1]} != in_features {in_features}")
     lead = x.shape[:-1]
-    x2 = x if x.dim() == 2 and x.is_contiguous() else x.reshape(-1, in_features).contiguous()
+    x2 = _rows(x, in_features, stream)
     rows = x2.shape[0]
     if out is None:
-        out = torch.empty((*lead, out_features), dtype=out_dtype, device=x.device)
+        out = _empty((*lead, out_features), out_dtype, x.device, stream)
     elif out.dtype != out_dtype or tuple(out.shape) != (*lead, out_features) or not out.is_contiguous():
         raise Gemma4Error(Status.INVALID_ARGUMENT, "out has the wrong dtype, shape or layout")
     status = fn(handle, _stream_ptr(stream), x2.data_ptr(), rows, out.data_ptr(),
@@ -359,7 +390,7 @@ class QuantizedLinear(_Handle):
         else:
             import torch
 
-            t = _device_triple(weight, scales, biases, n, k, group_size, bits)
+            t = _device_triple(weight, scales, biases, n, k, group_size, bits, stream)
             with torch.cuda.device(t[0].device):
                 status = self._lib.gemma4_qlinear_create_device(ctypes.byref(desc), *map(_dev_ptr, t),
                                                                 _stream_ptr(stream), ctypes.byref(self._handle))
@@ -403,11 +434,11 @@ class QuantizedLinear(_Handle):
             raise Gemma4Error(Status.INVALID_ARGUMENT, "out_dtype must be bfloat16 or float32")
         if x.dtype != torch.bfloat16 or x.shape[-1] != self.in_features:
             raise Gemma4Error(Status.INVALID_ARGUMENT, f"x must be bfloat16 [..., {self.in_features}]")
-        x2 = x.reshape(-1, self.in_features).contiguous()
+        x2 = _rows(x, self.in_features, stream)
         rows = x2.shape[0]
-        token = torch.empty((rows,), dtype=torch.int32, device=x.device)
-        value = torch.empty((rows,), dtype=torch.float32, device=x.device)
-        logits = torch.empty((rows, self.out_features), dtype=out_dtype, device=x.device) if return_logits else None
+        token = _empty((rows,), torch.int32, x.device, stream)
+        value = _empty((rows,), torch.float32, x.device, stream)
+        logits = _empty((rows, self.out_features), out_dtype, x.device, stream) if return_logits else None
         code = DTYPE_F32 if out_dtype == torch.float32 else DTYPE_BF16
         check(self._lib.gemma4_qlinear_forward_greedy(
             self._handle, _stream_ptr(stream), _dev_ptr(x2), rows, float(softcap),
@@ -431,8 +462,9 @@ class QuantizedLinear(_Handle):
         out_dtype = out_dtype or torch.bfloat16
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise Gemma4Error(Status.INVALID_ARGUMENT, "out_dtype must be bfloat16 or float32")
-        ids = ids.to(torch.int32).contiguous()
-        out = torch.empty((ids.numel(), self.in_features), dtype=out_dtype, device=ids.device)
+        with _made_on(stream):
+            ids = ids.to(torch.int32).contiguous()
+        out = _empty((ids.numel(), self.in_features), out_dtype, ids.device, stream)
         check(self._lib.gemma4_qlinear_embed(self._handle, _stream_ptr(stream), _dev_ptr(ids), ids.numel(),
                                              _dev_ptr(out), DTYPE_F32 if out_dtype == torch.float32 else DTYPE_BF16),
               self._lib)
@@ -441,7 +473,7 @@ class QuantizedLinear(_Handle):
     def dequantize(self, stream=None):
         import torch
 
-        out = torch.empty((self.out_features, self.in_features), dtype=torch.float32, device=self.device)
+        out = _empty((self.out_features, self.in_features), torch.float32, self.device, stream)
         check(self._lib.gemma4_qlinear_dequantize(self._handle, _stream_ptr(stream), _dev_ptr(out)), self._lib)
         return out
 
@@ -469,8 +501,8 @@ class QuantizedGeGLU(_Handle):
         else:
             import torch
 
-            tg = _device_triple(*gate, n, k, group_size, bits)
-            tu = _device_triple(*up, n, k, group_size, bits)
+            tg = _device_triple(*gate, n, k, group_size, bits, stream)
+            tu = _device_triple(*up, n, k, group_size, bits, stream)
             with torch.cuda.device(tg[0].device):
                 status = self._lib.gemma4_qgeglu_create_device(ctypes.byref(desc), *map(_dev_ptr, tg),
                                                                *map(_dev_ptr, tu), _stream_ptr(stream),
@@ -498,12 +530,12 @@ class QuantizedGeGLU(_Handle):
         if x.dtype != torch.bfloat16 or x.shape[-1] != self.in_features:
             raise Gemma4Error(Status.INVALID_ARGUMENT, f"x must be bfloat16 [..., {self.in_features}]")
         lead = tuple(x.shape[:-1])
-        x2 = x.reshape(-1, self.in_features).contiguous()
+        x2 = _rows(x, self.in_features, stream)
         rows = x2.shape[0]
         if h is None:
-            h = torch.empty(lead + (self.out_features,), dtype=torch.bfloat16, device=x.device)
+            h = _empty(lead + (self.out_features,), torch.bfloat16, x.device, stream)
         if out is None:
-            out = torch.empty(lead + (down.out_features,), dtype=torch.bfloat16, device=x.device)
+            out = _empty(lead + (down.out_features,), torch.bfloat16, x.device, stream)
         for t, n, what in ((h, self.out_features, "h"), (out, down.out_features, "out")):
             if t.dtype != torch.bfloat16 or tuple(t.shape) != lead + (n,) or not t.is_contiguous():
                 raise Gemma4Error(Status.INVALID_ARGUMENT, f"{what} has the wrong dtype, shape or layout")
@@ -521,7 +553,7 @@ class QuantizedGeGLU(_Handle):
         """fp32 [2, F, K]: the gate rows, then the up rows (bit-exact)."""
         import torch
 
-        out = torch.empty((2, self.out_features, self.in_features), dtype=torch.float32, device=self.device)
+        out = _empty((2, self.out_features, self.in_features), torch.float32, self.device, stream)
         check(self._lib.gemma4_qlinear_dequantize(self._handle, _stream_ptr(stream), _dev_ptr(out)), self._lib)
         return out
 
