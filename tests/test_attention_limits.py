@@ -143,3 +143,20 @@ def test_outputs_belong_to_the_stream_that_writes_them(made):
         for s in (None, "side"):
             on = record(lambda: call(s))
             assert on and all(where == (s or "current") for _, where in on), on
+
+
+# ------------------------------------------------------------------ numbers past 32 bits in Python
+
+@pytest.mark.parametrize("window", [(1 << 30) + 1, 1 << 32, (1 << 32) + 5, 1 << 70])
+def test_a_window_past_the_librarys_limit_is_refused(fake, window):
+    """Cut to 32 bits, 2^32 would mean no window and 2^32 + 5 one of 5."""
+    import torch
+
+    i32 = lambda *shape: fake(*shape, dtype=torch.int32)  # noqa: E731
+    cache = A.PagedKVCache(fake(5, 2, 16, 128), fake(5, 2, 16, 128))
+    batch = A.KVBatch(i32(3), i32(2), i32(2, 4))
+    with pytest.raises(qmm.Gemma4Error) as e:
+        cache.attend(fake(3, 4, 128), batch, window=window)
+    assert "window" in str(e.value)
+    with pytest.raises(Took):
+        cache.attend(fake(3, 4, 128), batch, window=1 << 30)
