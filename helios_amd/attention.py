@@ -129,8 +129,8 @@ class Rope:
         self._device = inv_freq.get_device()
         pairs = inv_freq.numel()
         self.distance = pairs if distance is None else int(distance)
-        if self.distance < 0:
-            raise _invalid("distance must be positive")
+        if not 0 <= self.distance < 1 << 32:  # the rest is checked with the head_dim
+            raise _invalid("distance must be positive and fit 32 bits")
         self._c = _Rope(self.inv_freq.data_ptr(), pairs, self.distance)
         self._ref = ctypes.byref(self._c)
 

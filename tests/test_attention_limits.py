@@ -160,3 +160,14 @@ def test_a_window_past_the_librarys_limit_is_refused(fake, window):
     assert "window" in str(e.value)
     with pytest.raises(Took):
         cache.attend(fake(3, 4, 128), batch, window=1 << 30)
+
+
+@pytest.mark.parametrize("distance", [1 << 32, (1 << 32) + 1, (1 << 32) + 64, 1 << 70, -1])
+def test_a_distance_past_32_bits_is_refused(fake, distance):
+    """Cut to 32 bits, 2^32 + 1 would mean adjacent pairs."""
+    import torch
+
+    with pytest.raises(qmm.Gemma4Error) as e:
+        A.Rope(fake(64, dtype=torch.float32), distance)
+    assert "distance" in str(e.value)
+    A.Rope(fake(64, dtype=torch.float32), 256)
