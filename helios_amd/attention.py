@@ -338,8 +338,10 @@ class PagedKVCache:
 
         shape, q_stride = _heads_tensor(q, "q", self.head_dim)
         rows, heads, _ = shape
-        if not 0 <= window <= 1 << 30:  # here: a larger one does not reach the library whole
-            raise _invalid("window must be 0 (none) to 2^30")
+        if window < 0:
+            raise _invalid("window must be >= 0 (0: none)")
+        if window > 1 << 30:  # the library's limit, checked here: a larger one does not reach it whole
+            raise Gemma4Error(Status.UNSUPPORTED_CONFIG, "window exceeds 2^30 (0: none)")
         out, out_stride = _output(out, shape, q, "out", stream)
         lse = _new(q, (rows, heads), torch.float32, stream) if return_lse else None
         _on(self._device, (q, out), (batch,))
