@@ -96,7 +96,7 @@ def _heads_tensor(t, what: str, head_dim: int | None = None):
     if one != 1 or (heads > 1 and head_stride != dim):
         raise _invalid(f"{what} must have its heads contiguous within a row")
     # a single row's stride says nothing
-    return shape, row_stride if rows > 1 else max(row_stride, heads * dim)
+    return shape, row_stride if rows > 1 else heads * dim
 
 
 def _on(index, tensors, held):

@@ -171,3 +171,13 @@ def test_a_distance_past_32_bits_is_refused(fake, distance):
         A.Rope(fake(64, dtype=torch.float32), distance)
     assert "distance" in str(e.value)
     A.Rope(fake(64, dtype=torch.float32), 256)
+
+
+# ------------------------------------------------------------------ strides that say nothing
+
+@pytest.mark.parametrize("width", [4 * 128 + 4, 4 * 128 + 1, (1 << 33) + 8])
+def test_a_single_rows_stride_says_nothing(fake, width):
+    """One token's heads may be cut from a row of any width."""
+    one = fake(1, 4, 128).as_strided((1, 4, 128), (width, 128, 1))
+    assert A._heads_tensor(one, "q")[1] == 4 * 128
+    assert A._heads_tensor(fake(2, 5, 128)[:, :4], "q")[1] == 5 * 128
