@@ -1,4 +1,5 @@
-"""The paged-cache calls on the GPU at the edges of what they take: outputs on a named stream."""
+"""The paged-cache calls on the GPU at the edges of what they take: outputs on a named stream,
+infinities and NaN beside rotated pairs."""
 
 import numpy as np
 import pytest
@@ -43,3 +44,34 @@ def test_outputs_on_a_named_stream(gpu_lib):
         assert torch.equal(t, want)
     assert stream_of(out) != side.cuda_stream
     assert np.array_equal(O.f64(appended), O.f64(q))
+
+
+@pytest.mark.parametrize("distance", [1, 8, 32])
+def test_infinities_and_nan_beside_the_rotated_pairs(gpu_lib, distance):
+    """An element outside the rotated pairs passes as it is, whatever lies next to it, and so do
+    all of the values."""
+    import torch
+
+    from helios_amd import attention as A
+
+    rng = np.random.default_rng(71)
+    d, pairs, rows = 128, 8, 3
+    rope = A.Rope(dev(inv_freq(pairs)), distance)
+    pos = dev(np.array([5, 1000, 77], np.int32))
+    x = randn(rng, rows, 4, d)
+    plain, _ = A.qk_norm_rope(x, None, pos, rope)
+    odd = [float("inf"), float("-inf"), float("nan")]
+    y, want = x.clone(), plain.clone()
+    for row in range(rows):
+        for e in (50, 71, 127):  # neither these nor their neighbours are rotated
+            y[row, 1, e] = want[row, 1, e] = odd[row]
+    got, _ = A.qk_norm_rope(y, None, pos, rope)
+    same = lambda a, b: torch.equal(a.nan_to_num(7, 8, 9), b.nan_to_num(7, 8, 9)) and torch.equal(a.isnan(), b.isnan())  # noqa: E731
+    assert same(got, want)
+    # values are not rotated at all: neither their first pair nor the others
+    v = y.clone()
+    v[:, 0, 0], v[:, 2, 3], v[:, 3, distance] = odd[0], odd[1], odd[2]
+    b = O.make_batch(rng, [rows], [rows], 16)
+    cache = A.PagedKVCache.allocate(b["num_pages"], 16, 4, d)
+    cache.append(x, v, O.device_batch(b), rope=rope)
+    assert same(cache.v[int(b["tables"][0, 0]), :, :rows].transpose(0, 1), v)
