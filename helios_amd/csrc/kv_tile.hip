@@ -232,8 +232,11 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
     // Q: whole rows by DMA into the wave's part of the stage (a lane's own 16 bytes of 32 rows
     // would take the vector memory path twice as long), then into registers in B's layout.
     // The scale's sign goes into Q, so that the largest product is the largest score.  A scale
-    // of zero makes every score zero (or NaN) in Q already.
-    const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * (FP8 ? a.pages.k_scale : 1.0f) * kLog2e;
+    // of zero (or one that vanishes with the keys') makes every score zero (or NaN) in Q already:
+    // as a factor it would make NaN of the hidden keys' -inf.
+    const float factor = fabsf(a.scale) * (FP8 ? a.pages.k_scale : 1.0f) * kLog2e;
+    const bool no_scale = factor == 0.0f;
+    const float c = no_scale ? 1.0f : factor;
     u32x4 q[C::kSteps];
     {
         constexpr int kCpr = D / 8, kRows = 64 / kCpr;  // chunks of a row, rows of a DMA
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
         q4::wait_vm_lds<0>();
         if (C::kHalves > 1) q4::lds_barrier();
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        const uint32_t keep = live && a.scale != 0.0f ? ~0u : 0u;
+        const uint32_t keep = live && !no_scale ? ~0u : 0u;
 #pragma unroll
         for (int s = 0; s < C::kSteps; ++s) {
             // the dims of the K chunk that step s uses in lane half h

@@ -1,11 +1,11 @@
 """The paged-cache calls on the GPU at the edges of what they take: outputs on a named stream,
-infinities and NaN beside rotated pairs."""
+infinities and NaN beside rotated pairs, scales that leave fp32's range."""
 
 import numpy as np
 import pytest
 
 import attention_oracle as O
-from test_gpu_attention import attend_case, dev, inv_freq, randn
+from test_gpu_attention import attend_case, dev, inv_freq, kernel, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,24 @@ def test_infinities_and_nan_beside_the_rotated_pairs(gpu_lib, distance):
     cache = A.PagedKVCache.allocate(b["num_pages"], 16, 4, d)
     cache.append(x, v, O.device_batch(b), rope=rope)
     assert same(cache.v[int(b["tables"][0, 0]), :, :rows].transpose(0, 1), v)
+
+
+@pytest.mark.parametrize("d,hq,hk", [(64, 8, 2), (128, 4, 2), (256, 4, 2), (512, 16, 1)])
+@pytest.mark.parametrize("scale,k_scale,kind", [(1e-20, 1e-30, "e4m3"), (-1e-20, 1e-30, "e4m3"), (1.5e-45, 1.0, "bf16"), (1e-38, 1.0, "bf16")])
+def test_scales_below_fp32s_range(gpu_lib, d, hq, hk, scale, k_scale, kind):
+    """A scale that vanishes (with that of the keys) leaves every visible key the same weight,
+    and the hidden ones none."""
+    import torch
+
+    from helios_amd import attention as A
+
+    rng = np.random.default_rng(d)
+    *_, b, cache, batch, q, (k64, v64) = attend_case(rng, d, hq, hk, [40, 1, 3], [90, 33, 2], 16, kind, window=37)
+    small = A.PagedKVCache(cache.k, cache.v, k_scale, cache.v_scale)
+    k64 = O.f64(cache.k) * k_scale
+    want, bound, wl, lb = O.attend(O.f64(q), k64, v64, b, scale, 37)
+    for kernel_ in (1, 2):
+        with kernel(kernel_):
+            out, lse = small.attend(q, batch, scale=scale, window=37, return_lse=True)
+        O.assert_within(O.f64(out), want, bound, f"out, kernel {kernel_}")
+        O.assert_within(O.f64(lse), wl, lb, f"lse, kernel {kernel_}")
