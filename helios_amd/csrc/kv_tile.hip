@@ -113,6 +113,11 @@ __device__ __forceinline__ void mfma_settled(f32x16& o) {
     if constexpr (AGPRS) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o));
 }
 
+// The two bf16 of a word times zero.
+__device__ __forceinline__ uint32_t nonfinite_as_nan(uint32_t w) {
+    return ((w & 0x7F80u) == 0x7F80u ? 0x7FC0u : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 0x7FC00000u : 0u);
+}
+
 __device__ __forceinline__ float half_max(float v) {
     const u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
     // Q: whole rows by DMA into the wave's part of the stage (a lane's own 16 bytes of 32 rows
     // would take the vector memory path twice as long), then into registers in B's layout.
     // The scale's sign goes into Q, so that the largest product is the largest score.  A scale
-    // of zero (or one that vanishes with the keys') makes every score zero (or NaN) in Q already:
+    // of zero (or one that vanishes with the keys') makes every score zero or NaN in Q already:
     // as a factor it would make NaN of the hidden keys' -inf.
     const float factor = fabsf(a.scale) * (FP8 ? a.pages.k_scale : 1.0f) * kLog2e;
     const bool no_scale = factor == 0.0f;
@@ -252,12 +257,18 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
         q4::wait_vm_lds<0>();
         if (C::kHalves > 1) q4::lds_barrier();
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        const uint32_t keep = live && !no_scale ? ~0u : 0u;
+        const uint32_t keep = live ? ~0u : 0u;
 #pragma unroll
         for (int s = 0; s < C::kSteps; ++s) {
             // the dims of the K chunk that step s uses in lane half h
             const int ch = FP8 ? 4 * (s / 2) + 2 * h + (s & 1) : 2 * s + h;
             q[s] = (*reinterpret_cast<const u32x4*>(mine + n * 2 * D + 16 * (ch ^ swizzle<kCpr>(n))) ^ flip) & keep;
+        }
+        if (no_scale) {  // zeros, and NaN for what is infinite or NaN
+#pragma unroll
+            for (int s = 0; s < C::kSteps; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[s][i] = nonfinite_as_nan(q[s][i]);
         }
         q4::wait_lds();
         q4::lds_barrier();  // K takes the stage

@@ -96,3 +96,24 @@ def test_scales_below_fp32s_range(gpu_lib, d, hq, hk, scale, k_scale, kind):
             out, lse = small.attend(q, batch, scale=scale, window=37, return_lse=True)
         O.assert_within(O.f64(out), want, bound, f"out, kernel {kernel_}")
         O.assert_within(O.f64(lse), wl, lb, f"lse, kernel {kernel_}")
+
+
+@pytest.mark.parametrize("d,hq,hk,kind", [(64, 8, 2, "bf16"), (128, 4, 2, "e4m3"), (256, 4, 2, "bf16"), (512, 16, 1, "bf16")])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf"), float("-inf")])
+def test_queries_that_are_not_finite_at_scale_zero(gpu_lib, d, hq, hk, kind, odd):
+    """Zero times an infinite or NaN score is NaN: such a query's head is NaN in its row, and
+    nothing else changes."""
+    import torch
+
+    rng = np.random.default_rng(d + 1)
+    out, lse, b, cache, batch, q, _ = attend_case(rng, d, hq, hk, [40, 1], [60, 33], 16, kind, scale=0.0)
+    for k in (1, 2):
+        with kernel(k):
+            before, before_lse = cache.attend(q, batch, scale=0.0, return_lse=True)
+            q2 = q.clone()
+            q2[7, 1, 5] = q2[40, 0, d - 1] = odd
+            got, got_lse = cache.attend(q2, batch, scale=0.0, return_lse=True)
+        for row, head in ((7, 1), (40, 0)):
+            assert bool(got[row, head].isnan().all()) and bool(got_lse[row, head].isnan()), (k, row)
+            got[row, head], got_lse[row, head] = before[row, head], before_lse[row, head]
+        assert torch.equal(got, before) and torch.equal(got_lse, before_lse), k
