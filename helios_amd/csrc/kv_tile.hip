@@ -113,8 +113,8 @@ __device__ __forceinline__ void mfma_settled(f32x16& o) {
     if constexpr (AGPRS) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o));
 }
 
-// The two bf16 of a word times zero.
-__device__ __forceinline__ uint32_t nonfinite_as_nan(uint32_t w) {
+// The two bf16 of a word times zero: zeros, and NaN for what is infinite or NaN.
+__device__ __forceinline__ uint32_t times_zero(uint32_t w) {
     return ((w & 0x7F80u) == 0x7F80u ? 0x7FC0u : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 0x7FC00000u : 0u);
 }
 
@@ -255,6 +255,16 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
             __builtin_amdgcn_global_load_lds((GlobalPtr)(a.q + sm.q_at[32 * own + r] + 8 * ch), (LdsPtr)(mine + j * 1024), 16, 0, 0);
         }
         q4::wait_vm_lds<0>();
+        if (no_scale && half == 0) {
+            // in LDS: beside Q's registers it cost every call (a mixed batch of 12 requests 186 -> 189 us)
+#pragma nounroll
+            for (int i = lane; i < C::kQBytes / 16; i += 64) {
+                u32x4* const at = reinterpret_cast<u32x4*>(mine) + i;
+                const u32x4 w = *at;
+                *at = u32x4{times_zero(w.x), times_zero(w.y), times_zero(w.z), times_zero(w.w)};
+            }
+            q4::wait_lds();
+        }
         if (C::kHalves > 1) q4::lds_barrier();
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         const uint32_t keep = live ? ~0u : 0u;
@@ -263,12 +273,6 @@ __global__ __launch_bounds__(64 * tile_waves<D>, tile_waves<D> / 4) void tile_ke
             // the dims of the K chunk that step s uses in lane half h
             const int ch = FP8 ? 4 * (s / 2) + 2 * h + (s & 1) : 2 * s + h;
             q[s] = (*reinterpret_cast<const u32x4*>(mine + n * 2 * D + 16 * (ch ^ swizzle<kCpr>(n))) ^ flip) & keep;
-        }
-        if (no_scale) {  // zeros, and NaN for what is infinite or NaN
-#pragma unroll
-            for (int s = 0; s < C::kSteps; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[s][i] = nonfinite_as_nan(q[s][i]);
         }
         q4::wait_lds();
         q4::lds_barrier();  // K takes the stage
