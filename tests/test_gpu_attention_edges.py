@@ -1,5 +1,6 @@
 """The paged-cache calls on the GPU at the edges of what they take: outputs on a named stream,
-infinities and NaN beside rotated pairs, scales that leave fp32's range."""
+infinities and NaN beside rotated pairs, scales that leave fp32's range,
+more query heads to a KV head than a tile has rows."""
 
 import numpy as np
 import pytest
@@ -117,3 +118,13 @@ def test_queries_that_are_not_finite_at_scale_zero(gpu_lib, d, hq, hk, kind, odd
             assert bool(got[row, head].isnan().all()) and bool(got_lse[row, head].isnan()), (k, row)
             got[row, head], got_lse[row, head] = before[row, head], before_lse[row, head]
         assert torch.equal(got, before) and torch.equal(got_lse, before_lse), k
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("d,hq,hk", [(64, 130, 1), (64, 300, 1), (128, 260, 2), (512, 130, 1)])
+def test_more_heads_to_a_key_than_a_tile_has_rows(gpu_lib, d, hq, hk, kind):
+    """A KV head's query heads in several runs of 128 (and of 16), the last one partly filled:
+    uncut, and with items to join."""
+    attend_case(np.random.default_rng(hq), d, hq, hk, [5, 1, 0, 2], [40, 33, 7, 2], 16, kind, window=20, padding=1)
+    attend_case(np.random.default_rng(hq), d, hq, hk, [2, 1], [1500, 700], 32, kind)
+    attend_case(np.random.default_rng(hq), d, hq, hk, [1], [2100], 64, kind, window=1800)
