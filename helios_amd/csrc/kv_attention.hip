@@ -482,12 +482,9 @@ hipError_t launch_join(const AttnArgs& a, const Items& it, const Cuts& cuts, int
     return hipGetLastError();
 }
 
-// The most tiles of `tokens` rows that runs of least..most rows can make (the padding is a run too).
+// The most tiles that runs of least..most rows can make (the padding is a run too).
 int most_tiles(const AttnArgs& a, int tokens, int least, int most) {
-    const int64_t runs = (int64_t)a.batch.requests + 1, fit = a.batch.tokens / least;
-    const int64_t by_rows = a.batch.tokens / tokens + (fit < runs ? fit : runs);
-    const int64_t by_runs = runs * ((most < a.batch.tokens ? most : a.batch.tokens) / tokens + 1);
-    return (int)(by_rows < by_runs ? by_rows : by_runs);
+    return kv::most_tiles(a.batch.tokens, (int64_t)a.batch.requests + 1, tokens, least, most);
 }
 
 // The most keys a tile of `tokens` can see.

@@ -144,20 +144,15 @@ __device__ __forceinline__ Tile find_item(const Batch& b, int page_shift, const 
             run.len = r < b.requests ? b.kv_lens[r] : 0;
             run.rows = end - run.start >= cuts.least && end - run.start <= cuts.most ? end - run.start : 0;
         }
-        run.tiles = (int)((uint32_t)(run.rows + cuts.tokens - 1) / (uint32_t)cuts.tokens);
-        int keys = clampi(run.len, 0, b.width << page_shift);
-        const int reach = cuts.window + (run.rows < cuts.tokens ? run.rows : cuts.tokens);
-        if (cuts.window > 0 && keys > reach) keys = reach;
-        run.units = run.rows > 0 ? (int)((uint32_t)(keys + cuts.unit - 1) / (uint32_t)cuts.unit) : 0;
-        if (run.units < 1) run.units = 1;
+        run.tiles = tiles_of(run.rows, cuts.tokens);
+        run.units = units_of(run.rows, run.len, b.width << page_shift, cuts.tokens, cuts.unit, cuts.window);
         return run;
     };
-    const auto parts = [](int units, int per) { return (int)((uint32_t)(units + per - 1) / (uint32_t)per); };
     const Run head = load(0);
     int per = 0x7fffffff >> 1;  // units of an item
     if (cuts.slots > 0) {
         float sum = 0.0f;
-        int tiles = 0, most = 0;
+        int tiles = 0, most = 1;  // where the launch has no tile, too
         for (int base = 0; base <= b.requests; base += 64) {
             const Run r = base == 0 ? head : load(base);
             sum += wave_total((float)r.tiles * (float)r.units);
@@ -165,24 +160,19 @@ __device__ __forceinline__ Tile find_item(const Batch& b, int page_shift, const 
             const int u = wave_max(r.tiles > 0 ? r.units : 0);
             most = most > u ? most : u;
         }
-        // all requests alike: as many parts of each as there are slots for; else an even share
-        const int alike = parts(most, tiles > 0 && tiles < cuts.slots ? cuts.slots / tiles : 1);
-        const int even = (int)fminf(sum * 1.0001f / (float)cuts.slots, 1.0e9f) + 1;
+        const int alike = alike_units(most, tiles, cuts.slots), even = even_units(sum, cuts.slots);
         int items_alike = 0, items_even = 0;
         for (int base = 0; base <= b.requests; base += 64) {
             const Run r = base == 0 ? head : load(base);
-            items_alike += wave_total(r.tiles * parts(r.units, alike));
-            items_even += wave_total(r.tiles * parts(r.units, even));
+            items_alike += wave_total(r.tiles * parts_of(r.units, alike));
+            items_even += wave_total(r.tiles * parts_of(r.units, even));
         }
-        const float cost_alike = (float)parts(items_alike, cuts.slots) * (float)alike;
-        per = (float)parts(items_even, cuts.slots) * (float)even < cost_alike ? even : alike;
-        const int floor = sum <= (float)cuts.slots ? cuts.few_units : cuts.min_units;
-        if (per < floor) per = floor;
+        per = item_units(alike, items_alike, even, items_even, cuts.slots, sum <= (float)cuts.slots ? cuts.few_units : cuts.min_units);
     }
     int before = 0, before_items = 0;
     for (int base = 0; base <= b.requests; base += 64) {
         const Run r = base == 0 ? head : load(base);
-        const int splits = parts(r.units, per);
+        const int splits = parts_of(r.units, per);
         const int sum = wave_scan(BY_TILE ? r.tiles : r.tiles * splits);
         const unsigned long long past = __ballot(before + sum > index);
         const int items = BY_TILE ? wave_scan(r.tiles * splits) : sum;

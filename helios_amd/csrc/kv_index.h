@@ -10,6 +10,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace kv {
@@ -45,6 +46,41 @@ __host__ __device__ inline TileRange split_tiles(int tiles, int s, int splits, i
     r.first = s * per < tiles ? s * per : tiles;
     r.last = r.first + per < tiles ? r.first + per : tiles;
     return r;
+}
+
+// How a launch's tiles are cut into items (find_item in kv_device.h): tiles of a run of `rows`
+// rows, `tokens` to a tile; the units of `unit` keys that one of them sees at most (1 for a
+// tile without keys: it is an item too); the items of a tile of so many units, `per` to an item.
+__host__ __device__ inline int tiles_of(int rows, int tokens) { return (int)((uint32_t)(rows + tokens - 1) / (uint32_t)tokens); }
+__host__ __device__ inline int units_of(int rows, int len, int table_keys, int tokens, int unit, int window) {
+    int keys = clampi(len, 0, table_keys);
+    const int reach = window + (rows < tokens ? rows : tokens);
+    if (window > 0 && keys > reach) keys = reach;
+    const int units = rows > 0 ? (int)((uint32_t)(keys + unit - 1) / (uint32_t)unit) : 0;
+    return units < 1 ? 1 : units;
+}
+__host__ __device__ inline int parts_of(int units, int per) { return (int)((uint32_t)(units + per - 1) / (uint32_t)per); }
+
+// Units of an item, two ways.  All requests alike: as many parts of each tile as there are slots
+// for (at most `slots` items, or one to a tile); `most` is 1 at least.  Else an even share of all units, `sum` over
+// the tiles (rounded up past the sum's error: at most `slots` items and one more to a tile).
+__host__ __device__ inline int alike_units(int most, int tiles, int slots) {
+    return parts_of(most, tiles > 0 && tiles < slots ? slots / tiles : 1);
+}
+__host__ __device__ inline int even_units(float sum, int slots) { return (int)fminf(sum * 1.0001f / (float)slots, 1.0e9f) + 1; }
+// The one whose items, `slots` at a time, end sooner; but `least` at least.
+__host__ __device__ inline int item_units(int alike, int items_alike, int even, int items_even, int slots, int least) {
+    const float cost_alike = (float)parts_of(items_alike, slots) * (float)alike;
+    const int per = (float)parts_of(items_even, slots) * (float)even < cost_alike ? even : alike;
+    return per < least ? least : per;
+}
+
+// The most tiles of `tokens` rows that `runs` runs of least..most rows, `rows` in all, can make.
+__host__ __device__ inline int most_tiles(int64_t rows, int64_t runs, int tokens, int least, int most) {
+    const int64_t fit = rows / least;
+    const int64_t by_rows = rows / tokens + (fit < runs ? fit : runs);
+    const int64_t by_runs = runs * ((most < rows ? most : rows) / tokens + 1);
+    return (int)(by_rows < by_runs ? by_rows : by_runs);
 }
 
 // Whether all 16 keys from `key` on are seen by every one of `n` rows from `pos0` on.
