@@ -6,7 +6,9 @@
 // maximum m and sum l of the softmax, all in fp32; the weights exp(s - m) are rounded to
 // bf16 for their product with V (matrix cores), 2^-8 of each at most: the outputs of 4096
 // random keys are then 1.8e-3 off in the 2-norm (2.2e-3 from the 128-row tiles), 1.7e-3 of it
-// their own rounding.  l sums the weights before that rounding.  e4m3 keys and values are
+// their own rounding.  A row's largest weight is exactly 1 here, so that a row that one key
+// dominates loses little; in the 128-row tiles it need not be (kv_tile.hip).  l sums the
+// weights before that rounding.  e4m3 keys and values are
 // exact in bf16; their scales are applied to s and to the output.
 //
 // rows16_kernel: 16 query rows (tokens x heads sharing a KV head) at a time; each wave of
@@ -32,7 +34,9 @@ namespace {
 
 constexpr int kWaves = 4;
 
-// Workgroups of rows16 that run at once: one per CU at head_dim 512 (registers), else two.
+// Workgroups of rows16 that cuts are made for: one per CU at head_dim 512, where the registers
+// hold one wave per SIMD, else two.  (At 64 and 128 dims the registers would hold three or more;
+// what more and shorter items do there has not been measured.)
 int rows_fill(const AttnArgs& a) { return a.pages.head_dim == 512 ? 256 : 512; }
 // Those of the 128-row tiles: one per CU, two of the smaller heads (registers and LDS).
 int tiles_fill(const AttnArgs& a) { return a.pages.head_dim >= 256 ? 256 : 512; }

@@ -216,8 +216,11 @@ __host__ __device__ inline Shape tile_shape(int rows, int group) {
 }
 
 // Units are what a workgroup takes in one step; an item is of 256 keys at least, of 128 where
-// even so half the card is idle (four single tokens over 246 to 3316 keys of 512 dims: 17.8 us
-// in place of 23; one over 32768, where the items are many, 21 either way and its join 8 for 6).
+// the call's units of 64 are no more than the slots, so that items of 128 fill half of them at
+// most (four single tokens over 246 to 3316 keys of 512 dims: 17.8 us in place of 23; one over
+// 32768, where the items are many, 21 either way and its join 8 for 6).  One unit past that
+// border halves the items: of requests with 8 tokens over 1032 keys and 8 KV heads three (51
+// units, 64 slots) make 216 workgroups, four (68) make 160.
 constexpr int kRowsUnit = 64, kTileUnit = 32;
 constexpr int kRowsLeast = 256, kRowsFew = 128, kTileLeast = 256;
 __host__ __device__ inline Cuts rows_cuts(const AttnArgs& a, const Items& it, const Shape& sh) {

@@ -1,5 +1,5 @@
-// Launch interface of the paged-cache kernels (kv_heads.hip, kv_attention.hip); arguments
-// are checked by kv_runtime.cpp.
+// Launch interface of the paged-cache kernels (kv_heads.hip, kv_attention.hip, kv_tile.hip);
+// arguments are checked by kv_runtime.cpp.
 #pragma once
 
 #include <hip/hip_runtime.h>

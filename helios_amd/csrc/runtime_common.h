@@ -1,4 +1,4 @@
-// What the C ABI's entry points share (qmm_runtime.cpp, attn_runtime.cpp): the last
+// What the C ABI's entry points share (qmm_runtime.cpp, kv_runtime.cpp): the last
 // error, the scratch memory kept per (device, stream) and the device guard.
 //
 // Conventions of the reference runtime (native/gemma4_mlx/src/runtime.cc): status
@@ -112,11 +112,12 @@ inline StreamWorkspace* stream_workspace(int device, hipStream_t stream) {
 }
 
 // Device memory one call borrows for its kernels' scratch (the GEMM's group sums and
-// split-K partials, the greedy head's keys, LoRA's x.A^T): consecutive 256-byte-aligned
-// pieces of the stream's workspace, or, for the allocation-free entry point, of
-// `scratch`.  A call captured into a graph whose stream workspace is too small takes
-// stream-ordered allocations from the private pool instead, released on the same
-// stream after the launches (allocation nodes of the graph).
+// split-K partials, the greedy head's keys, LoRA's x.A^T, attention's partial sums):
+// consecutive 256-byte-aligned pieces of the stream's workspace, or, for the
+// allocation-free entry point, of `scratch`.  A call captured into a graph whose stream
+// workspace is too small takes stream-ordered allocations from the private pool
+// instead, released on the same stream after the launches (allocation nodes of the
+// graph).
 struct Scratch {
     hipStream_t stream = nullptr;
     int device = 0;
@@ -160,7 +161,7 @@ struct Scratch {
         if (!capturing) {
             // grow: a new buffer for this and later calls.  Pieces this call took from
             // the old one stay valid (it is released only after this call's launches,
-            // see `finish`), as does every graph that used it.  (The pool for the
+            // see `release`), as does every graph that used it.  (The pool for the
             // fallback below is made here too, outside any capture.)
             hipMemPool_t pool = nullptr;
             (void)scratch_pool(device, &pool);

@@ -41,14 +41,14 @@
  * device work is asynchronous on that stream.  A handle is immutable after
  * create, so forward/dequantize may run concurrently on several streams and
  * threads; create and free must not overlap use.  Scratch (split-K partial sums,
- * the 256-row GEMM tile's group sums, the greedy head's keys, LoRA's x.A^T) comes
- * from device memory the library keeps per (device, stream) and reuses call after
- * call in stream order.  A HIP graph that captured a call uses its capture stream's
- * memory, so replays of graphs captured on one stream must not overlap one another
- * or calls on that stream (replay them on one stream, or serialize).  When a call
- * needs more, the stream's memory grows; the outgrown buffer is freed unless a
- * capture used it.  The memory is held until gemma4_qmm_release_scratch or the end
- * of the process.
+ * the 256-row GEMM tile's group sums, the greedy head's keys, LoRA's x.A^T, the
+ * partial sums of attention whose key ranges are cut) comes from device memory the
+ * library keeps per (device, stream) and reuses call after call in stream order.  A
+ * HIP graph that captured a call uses its capture stream's memory, so replays of
+ * graphs captured on one stream must not overlap one another or calls on that stream
+ * (replay them on one stream, or serialize).  When a call needs more, the stream's
+ * memory grows; the outgrown buffer is freed unless a capture used it.  The memory is
+ * held until gemma4_qmm_release_scratch or the end of the process.
  */
 #ifndef GEMMA4_QMM_H
 #define GEMMA4_QMM_H
@@ -418,8 +418,10 @@ Gemma4Status gemma4_kv_append(const Gemma4KvPages* pages, const Gemma4KvBatch* b
  *   q_dev [tokens, q_heads, head_dim] with q_stride between rows, 16-byte aligned
  *   out_dev the same shape with out_stride
  *   lse_dev float [tokens, q_heads], log of the softmax's sum; NULL to skip
- * Pages that no row's window reaches are not read.  Long key ranges of small batches are
- * split over the card and joined by a second launch, in the stream's scratch memory. */
+ * Pages that no row's window reaches never count, and their table entries may be absent (a
+ * tile of up to 64 keys at the window's edge may load what a present entry there names).
+ * Long key ranges of small batches are split over the card and joined by further launches,
+ * in the stream's scratch memory. */
 Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch* batch, const uint16_t* q_dev,
                                  uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
                                  uint64_t out_stride, float* lse_dev, void* stream);
