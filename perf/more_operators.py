@@ -345,9 +345,10 @@ def _plain_pages(state):
     starts = torch.cat([torch.zeros_like(new[:1]), new.cumsum(0)])
     kv = old + new
     first, end = (old + page - 1) // page, (kv + page - 1) // page
-    need = end - first
+    fits = end <= width
+    need = (end - first) * fits
     upto = need.cumsum(0)
-    granted = (need == 0) | ((upto <= free_count) & (end <= width))
+    granted = fits & ((need == 0) | (upto <= free_count))
     j = torch.arange(width, device="cuda")[None, :]
     fresh = granted[:, None] & (j >= first[:, None]) & (j < end[:, None])
     nth = (upto - need)[:, None] + j - first[:, None]
