@@ -29,7 +29,7 @@ import torch
 own = False
 
 EPS = 1e-6
-LOW, HIGH = -100, 118  # exponents of a block's scale
+LOW, HIGH = -100, 80  # exponents of a block's scale
 # name -> query heads, KV heads, head_dim, window, rope base, rotated pairs, pair distance
 LAYERS = {
     "sliding": (16, 8, 256, 1024, 1.0e4, 128, 128),
