@@ -7,11 +7,14 @@ projection of Gemma 4 12B, native/gemma4_mlx/src/native_model.cc:349-362 and
 epilogue (native_model.cc:934-949, :378-386).  ``helios_amd.qmm`` is the Python
 binding of that ABI.  ``helios_amd.attention`` binds what lies between a layer's q|k|v
 and o projections: head norms with rotation, the paged key/value cache and the attention
-over it.
+over it; ``helios_amd.paging`` gives out that cache's pages on the GPU, and
+``helios_amd.sampling`` draws tokens from logits and checks drafted ones.
 """
 
 from .attention import HeadNorm, KVBatch, PagedKVCache, Rope, qk_norm_rope  # noqa: F401
+from .paging import PagePool  # noqa: F401
 from .quantize import quantize  # noqa: F401
+from .sampling import sample, verify_drafts  # noqa: F401
 from .qmm import (  # noqa: F401
     Gemma4Error,
     QuantizedGeGLU,

@@ -47,6 +47,10 @@ class _Pages(ctypes.Structure):
                 ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
 
 
+class _Scales(ctypes.Structure):
+    _fields_ = [("k_dev", _vp), ("v_dev", _vp), ("page_stride", _u64), ("head_stride", _u64), ("block", _u32)]
+
+
 class _Batch(ctypes.Structure):
     _fields_ = [("query_starts_dev", _vp), ("kv_lens_dev", _vp), ("block_tables_dev", _vp), ("requests", _u32),
                 ("tokens", _u32), ("pages_per_request", _u32), ("table_stride", _u32)]
@@ -258,13 +262,38 @@ def qk_norm_rope(q, k, positions, rope=None, q_norm=None, k_norm=None, out_q=Non
     return out_q, out_k
 
 
+def _block_scales(k_scale, v_scale, k, h: int, s: int):
+    """The blocks' scales of pages k, whose dims h and s are the heads and the slots."""
+    import torch
+
+    kinds = (torch.uint8, torch.float8_e8m0fnu)
+    for t in (k_scale, v_scale):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3 or not t.is_cuda or t.dtype not in kinds:
+            raise _invalid("block scales must be two float8_e8m0fnu (or uint8) tensors [pages, kv_heads, blocks] on the GPU")
+    if k.dtype != torch.float8_e4m3fn:
+        raise _invalid("block scales belong to float8_e4m3fn pages")
+    if k_scale.shape != v_scale.shape or k_scale.stride() != v_scale.stride() or k_scale.device != k.device or v_scale.device != k.device:
+        raise _invalid("the block scales must have the same shape and strides, and the pages' device")
+    pages, heads, per = k_scale.shape
+    if pages != k.shape[0] or heads != k.shape[h] or per == 0 or k.shape[s] % per:
+        raise _invalid(f"block scales must be [{k.shape[0]}, {k.shape[h]}, a divisor of {k.shape[s]}]")
+    if per > 1 and k_scale.stride(2) != 1:
+        raise _invalid("a page's block scales must lie side by side")
+    # the stride of an axis of one says nothing
+    strides = [k_scale.stride(i) if k_scale.shape[i] > 1 else per for i in (0, 1)]
+    return _Scales(k_scale.data_ptr(), v_scale.data_ptr(), *strides, k.shape[s] // per)
+
+
 class PagedKVCache:
     """Keys and values of many requests in pages: two tensors [pages, kv_heads, page_size,
     head_dim] (``layout`` "phsd") or [pages, page_size, kv_heads, head_dim] ("pshd"), bf16
-    or float8_e4m3fn, of equal strides.  e4m3 pages hold value / scale.  The tensors are the
-    caller's; ``PagedKVCache.allocate`` makes them."""
+    or float8_e4m3fn, of equal strides.  e4m3 pages hold value / scale: one scale for all, or,
+    with float8_e8m0fnu (or uint8) tensors [pages, kv_heads, page_size // block] of equal
+    strides, a power of two for each ``block`` consecutive tokens (16 to 256) of a page and
+    KV head, which ``append`` sets from the values it stores.  The tensors are the caller's;
+    ``PagedKVCache.allocate`` makes them."""
 
-    def __init__(self, k, v, k_scale: float = 1.0, v_scale: float = 1.0, layout: str = "phsd"):
+    def __init__(self, k, v, k_scale=1.0, v_scale=1.0, layout: str = "phsd"):
         import torch
 
         kinds = {torch.bfloat16: KV_BF16, torch.float8_e4m3fn: KV_E4M3}
@@ -278,8 +307,14 @@ class PagedKVCache:
         if k.numel() == 0 or k.stride(3) != 1:
             raise _invalid("k and v must not be empty and must have head_dim contiguous")
         self.k, self.v = k, v
-        self.k_scale, self.v_scale = float(k_scale), float(v_scale)
         h, s = (1, 2) if layout == "phsd" else (2, 1)
+        self._scales = None
+        if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor):
+            self._scales = _block_scales(k_scale, v_scale, k, h, s)
+            self._scales_ref = ctypes.byref(self._scales)
+            self.k_scale, self.v_scale = k_scale, v_scale
+        else:
+            self.k_scale, self.v_scale = float(k_scale), float(v_scale)
         self.kv_heads, self.page_size, self.head_dim = k.shape[h], k.shape[s], k.shape[3]
         self.num_pages = k.shape[0]
         self.device = k.device
@@ -288,17 +323,25 @@ class PagedKVCache:
         # the stride of an axis of one says nothing
         strides = [k.stride(i) if k.shape[i] > 1 else self.head_dim for i in (0, s, h)]
         self._c = _Pages(k.data_ptr(), v.data_ptr(), *strides, self.num_pages, self.page_size, self.kv_heads,
-                         self.head_dim, kinds[k.dtype], self.k_scale, self.v_scale)
+                         self.head_dim, kinds[k.dtype], *((1.0, 1.0) if self._scales else (self.k_scale, self.v_scale)))
         self._ref = ctypes.byref(self._c)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, k_scale: float = 1.0,
-                 v_scale: float = 1.0, device="cuda"):
-        """A cache of new, uninitialised pages (unused slots are never read into a result)."""
+                 v_scale: float = 1.0, device="cuda", scale_block: int = 0):
+        """A cache of new, uninitialised pages (unused slots are never read into a result).  With
+        ``scale_block`` (float8_e4m3fn pages) each block of so many tokens has a scale."""
         import torch
 
         shape = (num_pages, kv_heads, page_size, head_dim)
         k, v = (torch.empty(shape, dtype=dtype or torch.bfloat16, device=device) for _ in range(2))
+        if scale_block:
+            if scale_block < 0 or page_size % scale_block:
+                raise _invalid("scale_block must divide page_size")
+            if k_scale != 1.0 or v_scale != 1.0:
+                raise _invalid("k_scale and v_scale belong to caches without scale_block")
+            k_scale, v_scale = (torch.empty((num_pages, kv_heads, page_size // scale_block), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                                for _ in range(2))
         return cls(k, v, k_scale, v_scale)
 
     def append(self, k, v, batch: KVBatch, rope=None, k_norm=None, v_norm=None, q=None, q_norm=None, out_q=None,
@@ -321,9 +364,12 @@ class PagedKVCache:
         else:
             out_q = None
         _on(self._device, (k, v, q, out_q), (batch, rope, k_norm, v_norm, q_norm))
-        status = self._lib.gemma4_kv_append(self._ref, batch._struct(rows), of_q,
-                                            _heads(k, shape, k_stride, k_norm, 0, 0), _heads(v, v_shape, v_stride, v_norm, 0, 0),
-                                            None if rope is None else rope._ref, qmm._stream_ptr(stream))
+        args = (batch._struct(rows), of_q, _heads(k, shape, k_stride, k_norm, 0, 0), _heads(v, v_shape, v_stride, v_norm, 0, 0),
+                None if rope is None else rope._ref, qmm._stream_ptr(stream))
+        if self._scales is None:
+            status = self._lib.gemma4_kv_append(self._ref, *args)
+        else:
+            status = self._lib.gemma4_kv_append_scaled(self._ref, self._scales_ref, *args)
         if status != 0:
             qmm.check(status, self._lib)
         return out_q
@@ -345,10 +391,12 @@ class PagedKVCache:
         out, out_stride = _output(out, shape, q, "out", stream)
         lse = _new(q, (rows, heads), torch.float32, stream) if return_lse else None
         _on(self._device, (q, out), (batch,))
-        status = self._lib.gemma4_kv_attention(self._ref, batch._struct(rows), q.data_ptr(), q_stride, heads,
-                                               self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                               out_stride, None if lse is None else lse.data_ptr(),
-                                               qmm._stream_ptr(stream))
+        args = (batch._struct(rows), q.data_ptr(), q_stride, heads, self.head_dim ** -0.5 if scale is None else scale, window,
+                out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(), qmm._stream_ptr(stream))
+        if self._scales is None:
+            status = self._lib.gemma4_kv_attention(self._ref, *args)
+        else:
+            status = self._lib.gemma4_kv_attention_scaled(self._ref, self._scales_ref, *args)
         if status != 0:
             qmm.check(status, self._lib)
         return (out, lse) if return_lse else out

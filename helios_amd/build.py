@@ -23,7 +23,7 @@ LIB_NAME = "libgemma4_qmm.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 
 SOURCES = ["qmm_runtime.cpp", "q4_layout.hip", "q4_decode.hip", "q4_limbs.hip", "q4_gemm.hip", "q4_gemm_kpair.hip", "q4_lora.hip",
-           "kv_runtime.cpp", "kv_heads.hip", "kv_attention.hip", "kv_tile.hip"]
+           "kv_runtime.cpp", "kv_heads.hip", "kv_scaled_append.hip", "kv_attention.hip", "kv_tile.hip", "kv_scaled.hip", "kv_pool.hip", "verify_runtime.cpp", "verify.hip"]
 ARCH = "gfx950"
 # measurement aid for the benchmark (a read-only HBM streaming kernel), its own library
 PROBE_SOURCES = ["hbm_probe.hip"]
@@ -48,7 +48,7 @@ DEVICE_FLAGS = [
 # group, which cannot read AGPRs
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 # the 128-row attention tile's step is one straight run of code: its loops must all unroll
-UNROLL_SOURCES = ("kv_tile.hip",)
+UNROLL_SOURCES = ("kv_tile.hip", "kv_scaled.hip")
 
 
 def device_flags(source: str) -> list:

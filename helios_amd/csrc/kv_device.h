@@ -40,10 +40,26 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));  // one conversion of two
 }
 
-// Two e4m3 of a word as two bf16 (exact).
+// Two e4m3 of a word as two bf16, times a power of two (exact).
 template <bool HI>
-__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t w, float scale = 1.0f) {
+    return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+
+__device__ __forceinline__ float scale_value(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+__device__ __forceinline__ int least_scale(float top) { return least_scale_of(__float_as_uint(top)); }
+
+// Where pages' values have scales of their own, if they do: a kernel's further arguments.
+struct NoScales {};
+__device__ __forceinline__ NoScales scales_of() { return NoScales{}; }
+__device__ __forceinline__ const BlockScales& scales_of(const BlockScales& s) { return s; }
+
+// The bytes of K's and V's scales (V's above K's) at slot `slot` of a page and head; those of 1
+// where there is no page.
+__device__ __forceinline__ uint32_t scale_bytes(const BlockScales& s, int page, int head, uint32_t slot) {
+    const int64_t at = (int64_t)page * s.page_stride + (int64_t)head * s.head_stride + (slot >> s.block_shift);
+    if (page < 0) return kScaleBias | kScaleBias << 8;
+    return (uint32_t)clamp_scale(s.k[at]) | (uint32_t)clamp_scale(s.v[at]) << 8;
 }
 
 // Zeros the bf16 (or e4m3) values of a word that are infinite or NaN.

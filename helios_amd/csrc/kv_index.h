@@ -88,6 +88,17 @@ __host__ __device__ inline bool all_visible(int key, int keys, int pos0, int n, 
     return key + keys - 1 <= pos0 && (window <= 0 || key > pos0 + n - 1 - window);
 }
 
+// Scales of blocks of e4m3: 2^(byte - 127), the bytes held to 2^-100..2^80: a code of 2^-9 times
+// the least is normal, and 2^30 values of 448 times the largest, weighted by up to 2^8 (the
+// 128-row tiles' slack), sum to less than 2^128.
+constexpr int kScaleBias = 127, kScaleLow = -100, kScaleHigh = 80;
+__host__ __device__ inline int clamp_scale(int byte) { return clampi(byte, kScaleBias + kScaleLow, kScaleBias + kScaleHigh); }
+// The least scale's byte with top <= 448 * 2^(byte - 127), of the bits of a finite top >= 0.
+__host__ __device__ inline int least_scale_of(uint32_t bits) {
+    // top = m 2^(e - 127) with 1 <= m < 2; 448 = 1.75 * 2^8
+    return clamp_scale((int)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+}
+
 // Entry `at` of a request's table: its page, or -1 if there is none (past the table, or not
 // a page of the cache).
 __host__ __device__ inline int page_at(const int* table, int at, int width, int num_pages) {

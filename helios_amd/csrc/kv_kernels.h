@@ -1,4 +1,5 @@
-// Launch interface of the paged-cache kernels (kv_heads.hip, kv_attention.hip, kv_tile.hip);
+// Launch interface of the paged-cache kernels (kv_heads.hip, kv_scaled_append.hip, kv_attention.hip,
+// kv_tile.hip, kv_scaled.hip);
 // arguments are checked by kv_runtime.cpp.
 #pragma once
 
@@ -6,6 +7,28 @@
 #include <stdint.h>
 
 namespace kv {
+
+// The pages of a cache that are free (the first free_count of free_pages, the last one next), the
+// requests' tokens and their tables.
+struct Pool {
+    int* free_pages;
+    int* free_count;
+    int* lens;
+    int* tables;
+    int64_t stride;
+    int num_pages, page_shift, requests, width;
+};
+struct Reserve {
+    const int* new_tokens;
+    int* starts;
+    int* kv_lens;
+    int* granted;      // may be null, as the next two
+    int* positions;
+    int64_t* slots;
+};
+hipError_t launch_reserve(const Pool& p, const Reserve& a, int rows, hipStream_t stream);  // kv_pool.hip
+size_t release_scratch(const Pool& p);  // bytes of launch_release's counts; 0: null
+hipError_t launch_release(const Pool& p, const int* lens, int window, int* counts, hipStream_t stream);
 
 // Strides in elements.
 struct Pages {
@@ -15,6 +38,15 @@ struct Pages {
     int num_pages, page_shift, kv_heads, head_dim;
     int fp8;  // pages hold e4m3, else bf16
     float k_scale, v_scale;
+};
+
+// A scale for each block of 2^block_shift tokens of a page and KV head, 2^(byte - 127): those of
+// page p and head h at p * page_stride + h * head_stride, a page's blocks side by side.
+struct BlockScales {
+    uint8_t* k;
+    uint8_t* v;
+    int64_t page_stride, head_stride;
+    int block_shift;
 };
 
 struct Batch {
@@ -50,6 +82,10 @@ struct HeadArgs {
 };
 
 hipError_t launch_heads(const HeadArgs& a, hipStream_t stream);
+// Workgroups of a launch, which counts its threads (256 to a workgroup) in 32 bits.
+constexpr uint32_t kMostGroups = (1u << 24) - 1;
+int64_t scaled_append_groups(const HeadArgs& a, const BlockScales& sc);
+hipError_t launch_scaled_append(const HeadArgs& a, const BlockScales& sc, hipStream_t stream);  // kv_scaled_append.hip
 
 struct AttnArgs {
     const uint16_t* q;
@@ -91,6 +127,9 @@ struct AttnPlan {
 constexpr int kThinRows = 16, kWideRows = 128;
 AttnPlan plan_attention(const AttnArgs& a);
 hipError_t launch_tiles(const AttnArgs& a, const Items& it, hipStream_t stream);  // kv_tile.hip
-hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream);
+hipError_t launch_scaled_tiles(const AttnArgs& a, const Items& it, const BlockScales& sc, hipStream_t stream);  // kv_scaled.hip
+hipError_t launch_scaled_rows16(const AttnArgs& a, const Items& it, const BlockScales& sc, hipStream_t stream);
+// scales: null, or those of e4m3 pages
+hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, const BlockScales* scales, hipStream_t stream);
 
 }  // namespace kv

@@ -65,6 +65,25 @@ Gemma4Status check_pages(const Gemma4KvPages* p, const char* name, kv::Pages* ou
     return GEMMA4_OK;
 }
 
+// Block scales: pages as those of e4m3 whose own scales are 1.
+Gemma4Status check_scaled(const Gemma4KvPages* p, const Gemma4KvScales* sc, const char* name, kv::Pages* pages, kv::BlockScales* out) {
+    if (p == nullptr) return bad(name, "requires non-null pages");
+    if (sc == nullptr || sc->k_dev == nullptr || sc->v_dev == nullptr) return bad(name, "requires non-null k and v scales");
+    if (p->dtype != GEMMA4_KV_E4M3) return bad(name, "block scales belong to E4M3 pages");
+    Gemma4KvPages own = *p;
+    own.k_scale = own.v_scale = 1.0f;
+    const Gemma4Status st = check_pages(&own, name, pages);
+    if (st != GEMMA4_OK) return st;
+    if (sc->block < 16 || sc->block > 256 || (sc->block & (sc->block - 1)) != 0 || sc->block > p->page_size)
+        return unsupported(name, "a scale's block must be a power of two from 16 to 256, at most page_size");
+    const uint64_t per = p->page_size / sc->block, most = (uint64_t)1 << 40;
+    if (sc->page_stride > most || sc->head_stride > most) return unsupported(name, "a scale stride exceeds 2^40 bytes");
+    if ((p->kv_heads > 1 && sc->head_stride < per) || (p->num_pages > 1 && sc->page_stride < per))
+        return bad(name, "a scale stride is shorter than a page's blocks");
+    *out = kv::BlockScales{sc->k_dev, sc->v_dev, (int64_t)sc->page_stride, (int64_t)sc->head_stride, __builtin_ctz(sc->block)};
+    return GEMMA4_OK;
+}
+
 Gemma4Status check_batch(const Gemma4KvBatch* b, const kv::Pages& pages, const char* name, kv::Batch* out) {
     if (b == nullptr) return bad(name, "requires a non-null batch");
     if (b->requests == 0 || b->requests > (1u << 20)) return bad(name, "requests must be 1 to 2^20");
@@ -128,6 +147,114 @@ Gemma4Status check_heads(const Gemma4Heads* h, uint32_t head_dim, bool has_out, 
     return GEMMA4_OK;
 }
 
+Gemma4Status check_pool(const Gemma4KvPool* p, const char* name, kv::Pool* out) {
+    if (p == nullptr) return bad(name, "requires a non-null pool");
+    if (p->free_pages_dev == nullptr || p->free_count_dev == nullptr || p->lens_dev == nullptr || p->block_tables_dev == nullptr)
+        return bad(name, "requires non-null free_pages, free_count, lens and block_tables");
+    if (!aligned(p->free_pages_dev, 4) || !aligned(p->free_count_dev, 4) || !aligned(p->lens_dev, 4) || !aligned(p->block_tables_dev, 4))
+        return bad(name, "the pool's arrays must be 4-byte aligned");
+    if (p->page_size < 16 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)) != 0)
+        return unsupported(name, "page_size must be a power of two from 16 to 65536");
+    if (p->num_pages == 0 || p->num_pages > (1u << 30)) return bad(name, "num_pages must be 1 to 2^30");
+    if (p->requests == 0 || p->requests > (1u << 20)) return bad(name, "requests must be 1 to 2^20");
+    if (p->pages_per_request == 0 || p->table_stride < p->pages_per_request)
+        return bad(name, "pages_per_request must be > 0 and at most table_stride");
+    if (p->table_stride > 0x7FFFFFFFu) return unsupported(name, "table_stride must be under 2^31");
+    if ((uint64_t)p->pages_per_request * p->page_size > ((uint64_t)1 << 30))
+        return unsupported(name, "a request's pages exceed 2^30 tokens");
+    *out = kv::Pool{p->free_pages_dev, p->free_count_dev, p->lens_dev, p->block_tables_dev, (int64_t)p->table_stride, (int)p->num_pages,
+                    __builtin_ctz(p->page_size), (int)p->requests, (int)p->pages_per_request};
+    return GEMMA4_OK;
+}
+
+// scales: null, or those of the pages' blocks
+Gemma4Status append(const char* name, const Gemma4KvPages* pages, const Gemma4KvScales* scales, bool scaled, const Gemma4KvBatch* batch,
+                    const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream) {
+    kv::HeadArgs a{};
+    kv::BlockScales sc{};
+    Gemma4Status st = scaled ? check_scaled(pages, scales, name, &a.pages, &sc) : check_pages(pages, name, &a.pages);
+    if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
+    if (st == GEMMA4_OK) st = check_rope(rope, pages->head_dim, name, &a.rope);
+    if (st != GEMMA4_OK) return st;
+    if (k == nullptr || v == nullptr) return bad(name, "requires non-null k and v");
+    if (k->count != pages->kv_heads || v->count != pages->kv_heads)
+        return bad(name, "k and v must have the cache's kv_heads");
+    if (batch->tokens == 0) return ok();
+    if (q != nullptr) st = check_heads(q, pages->head_dim, true, "q", name, &a.part[0]);
+    if (st == GEMMA4_OK) st = check_heads(k, pages->head_dim, false, "k", name, &a.part[1]);
+    if (st == GEMMA4_OK) st = check_heads(v, pages->head_dim, false, "v", name, &a.part[2]);
+    if (st != GEMMA4_OK) return st;
+    a.rows = (int)batch->tokens;
+    a.head_dim = (int)pages->head_dim;
+    a.append = 1;
+    if (scaled && kv::scaled_append_groups(a, sc) > (int64_t)kv::kMostGroups)
+        return unsupported(name, "tokens * heads is too large for one launch");
+    const hipError_t e = scaled ? kv::launch_scaled_append(a, sc, static_cast<hipStream_t>(stream))
+                                : kv::launch_heads(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail((std::string(name) + ": launch").c_str(), e);
+    return ok();
+}
+
+Gemma4Status attend(const char* name, const Gemma4KvPages* pages, const Gemma4KvScales* scales, bool scaled, const Gemma4KvBatch* batch,
+                    const uint16_t* q_dev, uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
+                    uint64_t out_stride, float* lse_dev, void* stream) {
+    kv::AttnArgs a{};
+    kv::BlockScales sc{};
+    Gemma4Status st = scaled ? check_scaled(pages, scales, name, &a.pages, &sc) : check_pages(pages, name, &a.pages);
+    if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
+    if (st != GEMMA4_OK) return st;
+    if (q_heads == 0 || q_heads > 65536 || q_heads % pages->kv_heads != 0)
+        return bad(name, "q_heads must be a multiple of kv_heads (and at most 65536)");
+    if (!std::isfinite(scale)) return bad(name, "scale must be finite");
+    if (window > (1u << 30)) return unsupported(name, "window exceeds 2^30 (0: none)");
+    if (batch->tokens == 0) return ok();
+    if (q_dev == nullptr || out_dev == nullptr) return bad(name, "requires non-null q and out");
+    if (!aligned(q_dev, 16) || !aligned(out_dev, 16) || q_stride % 8 != 0 || out_stride % 8 != 0 || !aligned(lse_dev, 4))
+        return bad(name, "q, out and their strides must be multiples of 16 bytes, lse of 4");
+    const uint64_t least = (uint64_t)q_heads * pages->head_dim, most = (uint64_t)1 << 32;
+    if (q_stride < least || out_stride < least || q_stride > most || out_stride > most)
+        return bad(name, "q_stride and out_stride must hold q_heads * head_dim elements (and at most 2^32)");
+    a.q = q_dev;
+    a.out = out_dev;
+    a.lse = lse_dev;
+    a.q_stride = (int64_t)q_stride;
+    a.out_stride = (int64_t)out_stride;
+    a.q_heads = (int)q_heads;
+    a.window = (int)window;
+    a.scale = scale;
+    a.kernel = (int)g_attention_kernel.load(std::memory_order_relaxed);
+    // a launch's workgroups are counted in 31 bits
+    if (((uint64_t)batch->tokens + batch->requests + 1) * q_heads > 0x7FFFFFFFull)
+        return unsupported(name, "tokens * q_heads exceeds 2^31");
+    kv::AttnPlan plan = kv::plan_attention(a);
+    a.tile_from = plan.tile_from;
+    // a launch's threads are counted in 32 bits, 512 to a workgroup at most
+    for (const kv::Items* it : {&plan.tiles, &plan.rows})
+        if ((uint64_t)it->items * (uint64_t)it->parts >= (1u << 23))
+            return unsupported(name, "tokens * q_heads is too large for one launch");
+    Scratch scratch;
+    scratch.stream = static_cast<hipStream_t>(stream);
+    hipError_t e = hipGetDevice(&scratch.device);
+    if (e != hipSuccess) return hip_fail((std::string(name) + ": hipGetDevice").c_str(), e);
+    const int d = a.pages.head_dim;
+    const size_t wide_o = plan.o_bytes(plan.tiles, kv::kWideRows, d), wide_ml = plan.ml_bytes(plan.tiles, kv::kWideRows);
+    const size_t thin_o = plan.o_bytes(plan.rows, kv::kThinRows, d), thin_ml = plan.ml_bytes(plan.rows, kv::kThinRows);
+    void* ws = nullptr;
+    e = scratch.take(wide_o + wide_ml + thin_o + thin_ml, &ws);
+    if (e != hipSuccess)
+        return fail(GEMMA4_ERR_MEMORY_GUARD, std::string(name) + ": workspace allocation failed: " + hipGetErrorString(e));
+    char* at = static_cast<char*>(ws);
+    plan.tiles.part_o = reinterpret_cast<float*>(at);
+    plan.tiles.part_ml = reinterpret_cast<float2*>(at + wide_o);
+    plan.rows.part_o = reinterpret_cast<float*>(at + wide_o + wide_ml);
+    plan.rows.part_ml = reinterpret_cast<float2*>(at + wide_o + wide_ml + thin_o);
+    e = kv::launch_attention(a, plan, scaled ? &sc : nullptr, scratch.stream);
+    const hipError_t er = scratch.release();
+    if (e != hipSuccess) return hip_fail((std::string(name) + ": launch").c_str(), e);
+    if (er != hipSuccess) return hip_fail((std::string(name) + ": workspace release").c_str(), er);
+    return ok();
+}
+
 }  // namespace
 
 extern "C" {
@@ -164,28 +291,19 @@ Gemma4Status gemma4_qk_norm_rope(const Gemma4Heads* q, const Gemma4Heads* k, con
 Gemma4Status gemma4_kv_append(const Gemma4KvPages* pages, const Gemma4KvBatch* batch, const Gemma4Heads* q,
                               const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream) {
     try {
-        const char* const name = "gemma4_kv_append";
-        kv::HeadArgs a{};
-        Gemma4Status st = check_pages(pages, name, &a.pages);
-        if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
-        if (st == GEMMA4_OK) st = check_rope(rope, pages->head_dim, name, &a.rope);
-        if (st != GEMMA4_OK) return st;
-        if (k == nullptr || v == nullptr) return bad(name, "requires non-null k and v");
-        if (k->count != pages->kv_heads || v->count != pages->kv_heads)
-            return bad(name, "k and v must have the cache's kv_heads");
-        if (batch->tokens == 0) return ok();
-        if (q != nullptr) st = check_heads(q, pages->head_dim, true, "q", name, &a.part[0]);
-        if (st == GEMMA4_OK) st = check_heads(k, pages->head_dim, false, "k", name, &a.part[1]);
-        if (st == GEMMA4_OK) st = check_heads(v, pages->head_dim, false, "v", name, &a.part[2]);
-        if (st != GEMMA4_OK) return st;
-        a.rows = (int)batch->tokens;
-        a.head_dim = (int)pages->head_dim;
-        a.append = 1;
-        const hipError_t e = kv::launch_heads(a, static_cast<hipStream_t>(stream));
-        if (e != hipSuccess) return hip_fail("gemma4_kv_append: launch", e);
-        return ok();
+        return append("gemma4_kv_append", pages, nullptr, false, batch, q, k, v, rope, stream);
     } catch (...) {
         return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_append: unexpected native exception");
+    }
+}
+
+Gemma4Status gemma4_kv_append_scaled(const Gemma4KvPages* pages, const Gemma4KvScales* scales, const Gemma4KvBatch* batch,
+                                     const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope,
+                                     void* stream) {
+    try {
+        return append("gemma4_kv_append_scaled", pages, scales, true, batch, q, k, v, rope, stream);
+    } catch (...) {
+        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_append_scaled: unexpected native exception");
     }
 }
 
@@ -193,63 +311,70 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
                                  uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
                                  uint64_t out_stride, float* lse_dev, void* stream) {
     try {
-        const char* const name = "gemma4_kv_attention";
-        kv::AttnArgs a{};
-        Gemma4Status st = check_pages(pages, name, &a.pages);
-        if (st == GEMMA4_OK) st = check_batch(batch, a.pages, name, &a.batch);
+        return attend("gemma4_kv_attention", pages, nullptr, false, batch, q_dev, q_stride, q_heads, scale, window, out_dev, out_stride,
+                      lse_dev, stream);
+    } catch (...) {
+        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_attention: unexpected native exception");
+    }
+}
+
+Gemma4Status gemma4_kv_attention_scaled(const Gemma4KvPages* pages, const Gemma4KvScales* scales, const Gemma4KvBatch* batch,
+                                        const uint16_t* q_dev, uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window,
+                                        uint16_t* out_dev, uint64_t out_stride, float* lse_dev, void* stream) {
+    try {
+        return attend("gemma4_kv_attention_scaled", pages, scales, true, batch, q_dev, q_stride, q_heads, scale, window, out_dev,
+                      out_stride, lse_dev, stream);
+    } catch (...) {
+        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_attention_scaled: unexpected native exception");
+    }
+}
+
+Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_tokens_dev, int32_t* query_starts_dev, int32_t* kv_lens_dev,
+                               int32_t* granted_dev, uint32_t rows, int32_t* positions_dev, int64_t* slots_dev, void* stream) {
+    try {
+        const char* const name = "gemma4_kv_reserve";
+        kv::Pool p{};
+        const Gemma4Status st = check_pool(pool, name, &p);
         if (st != GEMMA4_OK) return st;
-        if (q_heads == 0 || q_heads > 65536 || q_heads % pages->kv_heads != 0)
-            return bad(name, "q_heads must be a multiple of kv_heads (and at most 65536)");
-        if (!std::isfinite(scale)) return bad(name, "scale must be finite");
+        if (new_tokens_dev == nullptr || query_starts_dev == nullptr || kv_lens_dev == nullptr)
+            return bad(name, "requires non-null new_tokens, query_starts and kv_lens");
+        if (kv_lens_dev == pool->lens_dev) return bad(name, "kv_lens must not be the pool's lens");
+        if (!aligned(new_tokens_dev, 4) || !aligned(query_starts_dev, 4) || !aligned(kv_lens_dev, 4) || !aligned(granted_dev, 4) ||
+            !aligned(positions_dev, 4) || !aligned(slots_dev, 8))
+            return bad(name, "arrays must be aligned to their type");
+        if (rows >= (1u << 24)) return unsupported(name, "rows must be under 2^24");
+        const kv::Reserve a{new_tokens_dev, query_starts_dev, kv_lens_dev, granted_dev, positions_dev, slots_dev};
+        const hipError_t e = kv::launch_reserve(p, a, (int)rows, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return hip_fail("gemma4_kv_reserve: launch", e);
+        return ok();
+    } catch (...) {
+        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_reserve: unexpected native exception");
+    }
+}
+
+Gemma4Status gemma4_kv_release(const Gemma4KvPool* pool, const int32_t* lens_dev, uint32_t window, void* stream) {
+    try {
+        const char* const name = "gemma4_kv_release";
+        kv::Pool p{};
+        const Gemma4Status st = check_pool(pool, name, &p);
+        if (st != GEMMA4_OK) return st;
+        if (lens_dev == nullptr || !aligned(lens_dev, 4)) return bad(name, "requires non-null lens, 4-byte aligned");
         if (window > (1u << 30)) return unsupported(name, "window exceeds 2^30 (0: none)");
-        if (batch->tokens == 0) return ok();
-        if (q_dev == nullptr || out_dev == nullptr) return bad(name, "requires non-null q and out");
-        if (!aligned(q_dev, 16) || !aligned(out_dev, 16) || q_stride % 8 != 0 || out_stride % 8 != 0 || !aligned(lse_dev, 4))
-            return bad(name, "q, out and their strides must be multiples of 16 bytes, lse of 4");
-        const uint64_t least = (uint64_t)q_heads * pages->head_dim, most = (uint64_t)1 << 32;
-        if (q_stride < least || out_stride < least || q_stride > most || out_stride > most)
-            return bad(name, "q_stride and out_stride must hold q_heads * head_dim elements (and at most 2^32)");
-        a.q = q_dev;
-        a.out = out_dev;
-        a.lse = lse_dev;
-        a.q_stride = (int64_t)q_stride;
-        a.out_stride = (int64_t)out_stride;
-        a.q_heads = (int)q_heads;
-        a.window = (int)window;
-        a.scale = scale;
-        a.kernel = (int)g_attention_kernel.load(std::memory_order_relaxed);
-        // a launch's workgroups are counted in 31 bits
-        if (((uint64_t)batch->tokens + batch->requests + 1) * q_heads > 0x7FFFFFFFull)
-            return unsupported(name, "tokens * q_heads exceeds 2^31");
-        kv::AttnPlan plan = kv::plan_attention(a);
-        a.tile_from = plan.tile_from;
-        // a launch's threads are counted in 32 bits, 512 to a workgroup at most
-        for (const kv::Items* it : {&plan.tiles, &plan.rows})
-            if ((uint64_t)it->items * (uint64_t)it->parts >= (1u << 23))
-                return unsupported(name, "tokens * q_heads is too large for one launch");
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
         hipError_t e = hipGetDevice(&sc.device);
-        if (e != hipSuccess) return hip_fail("gemma4_kv_attention: hipGetDevice", e);
-        const int d = a.pages.head_dim;
-        const size_t wide_o = plan.o_bytes(plan.tiles, kv::kWideRows, d), wide_ml = plan.ml_bytes(plan.tiles, kv::kWideRows);
-        const size_t thin_o = plan.o_bytes(plan.rows, kv::kThinRows, d), thin_ml = plan.ml_bytes(plan.rows, kv::kThinRows);
-        void* ws = nullptr;
-        e = sc.take(wide_o + wide_ml + thin_o + thin_ml, &ws);
+        if (e != hipSuccess) return hip_fail("gemma4_kv_release: hipGetDevice", e);
+        void* counts = nullptr;
+        e = sc.take(kv::release_scratch(p), &counts);
         if (e != hipSuccess)
             return fail(GEMMA4_ERR_MEMORY_GUARD, std::string(name) + ": workspace allocation failed: " + hipGetErrorString(e));
-        char* at = static_cast<char*>(ws);
-        plan.tiles.part_o = reinterpret_cast<float*>(at);
-        plan.tiles.part_ml = reinterpret_cast<float2*>(at + wide_o);
-        plan.rows.part_o = reinterpret_cast<float*>(at + wide_o + wide_ml);
-        plan.rows.part_ml = reinterpret_cast<float2*>(at + wide_o + wide_ml + thin_o);
-        e = kv::launch_attention(a, plan, sc.stream);
+        e = kv::launch_release(p, lens_dev, (int)window, static_cast<int*>(counts), sc.stream);
         const hipError_t er = sc.release();
-        if (e != hipSuccess) return hip_fail("gemma4_kv_attention: launch", e);
-        if (er != hipSuccess) return hip_fail("gemma4_kv_attention: workspace release", er);
+        if (e != hipSuccess) return hip_fail("gemma4_kv_release: launch", e);
+        if (er != hipSuccess) return hip_fail("gemma4_kv_release: workspace release", er);
         return ok();
     } catch (...) {
-        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_attention: unexpected native exception");
+        return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_release: unexpected native exception");
     }
 }
 

@@ -132,6 +132,13 @@ def load_library(path: str | None = None):
         "gemma4_kv_append": [vp, vp, vp, vp, vp, vp, vp],
         "gemma4_kv_attention": [vp, vp, vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_float, ctypes.c_uint32, vp,
                                 ctypes.c_uint64, vp, vp],
+        "gemma4_kv_append_scaled": [vp, vp, vp, vp, vp, vp, vp, vp],
+        "gemma4_kv_attention_scaled": [vp, vp, vp, vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_float, ctypes.c_uint32, vp,
+                                       ctypes.c_uint64, vp, vp],
+        "gemma4_kv_reserve": [vp, vp, vp, vp, vp, ctypes.c_uint32, vp, vp, vp],
+        "gemma4_kv_release": [vp, vp, ctypes.c_uint32, vp],
+        "gemma4_sample": [vp, ctypes.c_uint32, ctypes.c_uint32, vp, ctypes.c_float, vp, vp, vp],
+        "gemma4_verify_drafts": [vp, vp, vp, vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, vp, ctypes.c_float, vp, vp, vp, vp],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

@@ -426,6 +426,122 @@ Gemma4Status gemma4_kv_attention(const Gemma4KvPages* pages, const Gemma4KvBatch
                                  uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window, uint16_t* out_dev,
                                  uint64_t out_stride, float* lse_dev, void* stream);
 
+/* ---- Pages of e4m3 with a scale for each block of tokens ----
+ * The two calls above on E4M3 pages whose values are code * 2^(byte - 127), a byte for each
+ * `block` consecutive tokens of a page and KV head, for K and for V (the pages' own k_scale and
+ * v_scale are ignored).  No scale has to be known beforehand: the append sets a block's byte
+ * from the values it stores. No counterpart in the reference.
+ *   k_dev, v_dev  uint8: page p and head h's bytes at p * page_stride + h * head_stride, one for
+ *                 each block of the page, side by side.  Bytes are taken as at least 27 and at
+ *                 most 207 (2^-100 to 2^80)
+ *   block         a power of two from 16 to 256, at most page_size */
+typedef struct Gemma4KvScales {
+    uint8_t* k_dev;
+    uint8_t* v_dev;
+    uint64_t page_stride, head_stride; /* bytes */
+    uint32_t block;
+} Gemma4KvScales;
+
+/* gemma4_kv_append.  For the batch's new tokens of a block, of one KV head, the byte becomes the
+ * least whose scale times 448 holds the largest finite value among them (0 to 2^-100 take 27);
+ * where the block holds tokens before them (its first slot is not among the new ones) it never
+ * falls, and where it rises the codes held are brought to the new scale and rounded again.
+ * Infinities are stored as +-448 times the scale, NaN as NaN.  Slots after the new tokens are
+ * left as they are.  A block must be stored to for one request only in a call. */
+Gemma4Status gemma4_kv_append_scaled(const Gemma4KvPages* pages, const Gemma4KvScales* scales, const Gemma4KvBatch* batch,
+                                     const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope,
+                                     void* stream);
+
+/* gemma4_kv_attention over such pages. */
+Gemma4Status gemma4_kv_attention_scaled(const Gemma4KvPages* pages, const Gemma4KvScales* scales, const Gemma4KvBatch* batch,
+                                        const uint16_t* q_dev, uint64_t q_stride, uint32_t q_heads, float scale, uint32_t window,
+                                        uint16_t* out_dev, uint64_t out_stride, float* lse_dev, void* stream);
+
+/* ---- Pages given out and taken back on the GPU ----
+ * What a scheduler does to a batch's tables between two steps, from lengths on the device, so
+ * that a captured step needs no host: pages for new tokens (gemma4_kv_reserve), which also
+ * makes the arrays of the step's Gemma4KvBatch, and pages no longer needed back to the free
+ * ones (gemma4_kv_release).  No counterpart in the reference (MLX grows an array per request).
+ *   free_pages_dev   int32 [num_pages]: the first free_count of them are the free pages, the last
+ *                    of those given out next
+ *   free_count_dev   int32 [1]
+ *   lens_dev         int32 [requests]: tokens that each request holds (0: an empty slot)
+ *   block_tables_dev int32 [requests, table_stride], pages_per_request entries used; entries
+ *                    outside [0, num_pages) are absent.  A page is in one table, or free
+ * The calls on a pool must follow each other (one stream, or waits). */
+typedef struct Gemma4KvPool {
+    int32_t* free_pages_dev;
+    int32_t* free_count_dev;
+    int32_t* lens_dev;
+    int32_t* block_tables_dev;
+    uint32_t num_pages, page_size, requests, pages_per_request, table_stride;
+} Gemma4KvPool;
+
+/* Pages for new_tokens[r] tokens (negative: none) after the lens[r] that request r holds: absent
+ * entries up to that of its last new token are filled, in the order of requests and entries,
+ * from the end of the free pages.  A request gets all of its pages or none: none where the sum
+ * of what it and those before it need exceeds the free pages, or its table is too short.
+ *   query_starts_dev int32 [requests + 1], kv_lens_dev int32 [requests]: those of the batch
+ *                    (exclusive sums of the new tokens; lens + new_tokens, also where pages were
+ *                    not granted: the tokens then have absent pages, and nothing is stored for them
+ *                    beyond the request's last page).  kv_lens_dev is not the pool's lens_dev
+ *   granted_dev      int32 [requests], 1 or 0; NULL to skip
+ *   positions_dev    int32 [rows], slots_dev int64 [rows]; each NULL to skip: position of each of
+ *                    the batch's rows in its request, and page * page_size + slot (-1 where there
+ *                    is no page); rows past the last start get 0 and -1
+ * lens are not changed: gemma4_kv_release sets them once it is known what is kept. */
+Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_tokens_dev, int32_t* query_starts_dev, int32_t* kv_lens_dev,
+                               int32_t* granted_dev, uint32_t rows, int32_t* positions_dev, int64_t* slots_dev, void* stream);
+
+/* Keeps lens[r] tokens of request r (0: the request is done) and gives back the pages behind
+ * them and, with window > 0, those before what the next token sees (positions under
+ * lens - window + 1).  Freed pages go to the end of the free ones, the last freed first, so
+ * that a release of what was just reserved leaves them as they were.  lens_dev may be the
+ * pool's own.  Tables of more than 16384 entries in all take scratch of 4 bytes a request. */
+Gemma4Status gemma4_kv_release(const Gemma4KvPool* pool, const int32_t* lens_dev, uint32_t window, void* stream);
+
+/* ---- Sampling, and drafted tokens ----
+ * Rows of logits [rows, vocab], row r at x_dev + r * stride elements, BF16 or F32, aligned to their
+ * type.  softcap > 0: cap * tanh(x / cap) in their place (native_model.cc:1794, unrounded).
+ * Logits of -inf and NaN have no probability, whatever the softcap. */
+typedef struct Gemma4Logits {
+    const void* x_dev;
+    uint64_t stride;
+    uint32_t dtype; /* Gemma4QmmDtype */
+    float softcap;
+} Gemma4Logits;
+
+/* A token from each row's p = softmax(logits / temperature): the first i with
+ * p_0 + .. + p_i > uniforms[row]; the first largest logit where the temperature is 0.
+ *   uniforms_dev     float [rows] in [0, 1)
+ *   temperatures_dev float [rows] (0 or less: greedy), or NULL: `temperature` for all
+ *   out_tokens_dev   int32 [rows]; -1 where no logit has a probability
+ * Weights and sums are fp64.  Scratch: 16 bytes a row and chunk of 2048 to 8192 logits. */
+Gemma4Status gemma4_sample(const Gemma4Logits* logits, uint32_t rows, uint32_t vocab, const float* uniforms_dev, float temperature,
+                           const float* temperatures_dev, int32_t* out_tokens_dev, void* stream);
+
+/* Drafted tokens against the target's probabilities.  Request r's rows are query_starts[r] ..
+ * query_starts[r + 1] - 1: the first was fed its last known token, the others its drafts, so row
+ * i's logits answer for the token of row i + 1.  Draft tokens[i + 1] stands while
+ *     uniforms[i][0] * q(token) < p(token),
+ * p and q the softmax of row i's logits and draft logits over the request's temperature (q = 1
+ * where draft_logits is NULL: drafts that were not drawn at random).  At the first that falls a
+ * token is drawn from max(p - q, 0) by uniforms[i][1]; where all stand, from the last row's p.
+ * Temperature 0: p and q are 1 at the first largest logit.
+ *   tokens_dev       int32 [rows], those fed; one outside [0, vocab) never stands
+ *   query_starts_dev int32 [requests + 1], nondecreasing from 0; rows past the last are padding
+ *   uniforms_dev     float [rows, 2] in [0, 1)
+ *   temperatures_dev float [requests], or NULL
+ *   out_tokens_dev   int32 [rows]: the accepted drafts from the request's first row on, then the
+ *                    drawn token, then -1 (padding -1)
+ *   accepted_dev     int32 [requests]: accepted drafts; accepted + 1 tokens are new (none where a
+ *                    request has no rows)
+ * draft_logits has the rows of logits; its last row of each request is not read for a result. */
+Gemma4Status gemma4_verify_drafts(const Gemma4Logits* logits, const Gemma4Logits* draft_logits, const int32_t* tokens_dev,
+                                  const int32_t* query_starts_dev, uint32_t requests, uint32_t rows, uint32_t vocab,
+                                  const float* uniforms_dev, float temperature, const float* temperatures_dev, int32_t* out_tokens_dev,
+                                  int32_t* accepted_dev, void* stream);
+
 /* Attention kernels of this process.  No counterpart in the reference; for tests and
  * benchmarks that pin a kernel.
  *   0 (the default): by the rows of each request and the work of the call.
