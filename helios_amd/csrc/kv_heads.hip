@@ -79,7 +79,11 @@ __global__ __launch_bounds__(kThreads, 6) void heads_kernel(HeadArgs a) {
 
     const int pairs = a.rope.pairs, dist = a.rope.distance;
     for (int i = tid; i < pairs; i += kThreads) {
-        turn[i] = turn_by(r.pos, a.rope.inv_freq[i]);
+        const double turns = (double)r.pos * (double)a.rope.inv_freq[i] * 0.15915494309189533577;
+        const float f = (float)(turns - rint(turns));
+        float s, cs;
+        sincospif(2.0f * f, &s, &cs);
+        turn[i] = make_float2(cs, s);
     }
     __syncthreads();
 
@@ -93,14 +97,73 @@ __global__ __launch_bounds__(kThreads, 6) void heads_kernel(HeadArgs a) {
             const int which = which_of(u), head = head_of(u, which);
             const uint32_t w4[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
             float x[8];
-            unpack_head(w4, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = q4::bf16_lo(w4[i]);
+                x[2 * i + 1] = q4::bf16_hi(w4[i]);
+            }
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
             ss = head_sum<LANES>(ss);
-            if (pick(which, a.part[0].norm, a.part[1].norm, a.part[2].norm))
-                norm_head<D>(x, ss, pick(which, a.part[0].eps, a.part[1].eps, a.part[2].eps), pick(which, q_weight, k_weight, v_weight));
-            if (pairs > 0) turn_head(x, turn, pairs, dist, which != 2, c, lane);
+            if (pick(which, a.part[0].norm, a.part[1].norm, a.part[2].norm)) {
+                const float inv = rsqrtf(ss * (1.0f / D) + pick(which, a.part[0].eps, a.part[1].eps, a.part[2].eps));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= inv;
+                const uint4 wr = pick(which, q_weight, k_weight, v_weight);
+                const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[2 * i] *= q4::bf16_lo(ww[i]);
+                    x[2 * i + 1] *= q4::bf16_hi(ww[i]);
+                }
+            }
+            if (pairs > 0) {
+                const bool rot = which != 2;
+                if (dist == 1) {
+                    // a lane's four pairs turn or pass together (pairs is a multiple of 8); those that pass
+                    // are selected, as a turn by zero would spread an infinity to its neighbour (as a
+                    // branch it cost the other distances: 2048 tokens of 17 heads of 512 20.4 -> 20.9 us)
+                    const bool turns = rot && 4 * c < pairs;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 cs = turns ? turn[4 * c + i] : make_float2(1.0f, 0.0f);
+                        const float u0 = x[2 * i], u1 = x[2 * i + 1];
+                        x[2 * i] = turns ? u0 * cs.x - u1 * cs.y : u0;
+                        x[2 * i + 1] = turns ? u1 * cs.x + u0 * cs.y : u1;
+                    }
+                } else {
+                    const int dl = dist / 8;
+                    const bool first = 8 * c < pairs, second = 8 * c >= dist && 8 * c < dist + pairs;
+                    const int src = lane + (first ? dl : (second ? -dl : 0));
+                    const int i0 = first ? 8 * c : 8 * c - dist;
+                    // the pair's other half, dl lanes up or down
+                    float other[8];
+                    if (dl == 32) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+                            other[i] = __uint_as_float(first ? p.y : p.x);
+                        }
+                    } else if (dl == 16) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const u32x2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+                            other[i] = __uint_as_float(first ? p.y : p.x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) other[i] = __shfl(x[i], src);
+                    }
+                    if (rot && (first || second)) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float2 cs = turn[i0 + i];
+                            x[i] = first ? x[i] * cs.x - other[i] * cs.y : x[i] * cs.x + other[i] * cs.y;
+                        }
+                    }
+                }
+            }
             if (!live) continue;
             uint16_t* const out = pick(which, a.part[0].out, a.part[1].out, a.part[2].out);
             if (out != nullptr) {

@@ -1,5 +1,7 @@
 // Device pieces of the head norms, the rotation and the appends (kv_heads.hip, kv_scaled_append.hip):
-// a head of D elements lies in D/8 neighbouring lanes, eight to a lane.
+// a head of D elements lies in D/8 neighbouring lanes, eight to a lane.  heads_kernel has the norm and
+// the turn written out: by these functions its code is ordered otherwise, and 2048 tokens of 17 heads
+// of 512 took 22.4 us in place of 21.7.
 #pragma once
 
 #include "kv_device.h"

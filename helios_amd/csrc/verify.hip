@@ -10,24 +10,21 @@
 // Sums and weights are fp64: a token is a place in a sum of some 2^18 terms, and an fp32 sum
 // (2^-24 of it off) would miss by one wherever the terms are smaller than that.
 //
-// Bound by reading the logits once.  A row is cut into chunks, a workgroup each, that stay in
-// registers between the search for the chunk's maximum and the sum of weights relative to it
-// (stats_kernel).  Each request's own workgroups then join its rows' chunks, find the first draft
-// that falls and sum max(p - q, 0) over their chunk of that one row (rest_kernel); a workgroup
-// per request finds the chunk and the place in it (pick_kernel).  Orders are fixed: no atomics.
+// Bound by reading the logits once, and nearly as much by their exponentials (some 14 fp64
+// operations each, which run at fp32's rate).  A row is cut into parts of 2048 (or 512) places; a wave holds
+// a part in registers between the search for its maximum and the sum of its weights relative to
+// that (stats_kernel).  Each request's own workgroups then join its rows' sums, find the first
+// draft that falls and sum max(p - q, 0) over parts of that one row (rest_kernel); a workgroup per
+// request finds the part and the place in it (pick_kernel).  Orders are fixed: no atomics.
 #include "q4_common.h"
+#include "verify_index.h"
 #include "verify_kernels.h"
 
 namespace verify {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kSweep = 8 * kThreads;  // places that a workgroup reads at once
-
-__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// A chunk's largest logit (as it is), the first place that has it, and the sum of its weights
-// relative to it.
+// The sum of a part's weights relative to `top`, the largest logit (as it is) of the part's
+// chunk; for greedy requests the first place that has it.
 struct alignas(16) Part {
     double sum;
     float top;
@@ -44,70 +41,177 @@ struct alignas(16) Spot {
 };
 
 struct Work {
-    Part* parts;   // [target rows, then drafter's rows][chunks]
-    double* rest;  // [requests][chunks], of requests whose spot is of kind 2
+    Part* parts;   // [target rows, then drafter's rows][parts]
+    double* rest;  // [requests][parts], of requests whose spot is of kind 2
     Spot* spots;   // [requests]
 };
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+constexpr float kInf = __builtin_huge_valf();
 
-__device__ __forceinline__ float value_of(const Logits& l, int64_t at) {
-    return l.f32 ? static_cast<const float*>(l.x)[at] : __uint_as_float((uint32_t) static_cast<const uint16_t*>(l.x)[at] << 16);
+// 2^(j / 256), by the series of the exponential; j / 256 is taken off the exponent and mantissa
+// field again, so that adding n 2^-8 to that field, n % 256 = j, gives the bits of 2^(n / 256).
+constexpr int kSteps = 256;
+typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+struct Exp2Table {
+    uint64_t v[kSteps];
+};
+constexpr Exp2Table make_exp2() {
+    Exp2Table t{};
+    for (int j = 0; j < kSteps; ++j) {
+        const double x = 0.69314718055994530942 * j / kSteps;
+        double sum = 0.0;
+        for (int k = 24; k > 0; --k) sum = (sum + 1.0) * x / k;
+        t.v[j] = __builtin_bit_cast(uint64_t, 1.0 + sum) - ((uint64_t)j << 44);
+    }
+    return t;
+}
+__device__ const Exp2Table kExp2 = make_exp2();
+
+template <int THREADS>
+__device__ __forceinline__ void take_exp2(U2* table) {
+    if (THREADS == kSteps || (int)threadIdx.x < kSteps) table[threadIdx.x] = __builtin_bit_cast(U2, kExp2.v[threadIdx.x]);
 }
 
-__device__ __forceinline__ double capped(float x, double cap) {
-    return cap > 0.0 ? cap * tanh((double)x / cap) : (double)x;
+// e^z for kLeast <= z <= 0, 2e-13 of it off at most; any bits for other z.  z = (n + r) ln2 / 256 with
+// |r| <= 1/2: the series to the third power of at most ln2 / 512 (the next term is 1.4e-13), and a
+// factor 2^(n / 256) from the table.  The constants sit in registers from the kernel's start.
+constexpr double kLeast = -700.0;
+struct Exp {
+    const U2* table;
+    double per_step, step, sixth, magic;
+    __device__ __forceinline__ explicit Exp(const U2* t)
+        : table(t), per_step(kSteps / 0.69314718055994530942), step(-0.69314718055994530942 / kSteps), sixth(1.0 / 6),
+          magic(6755399441055744.0) {  // 1.5 * 2^52: the low bits of a sum with it are the nearest integer
+        asm volatile("" : "+s"(per_step), "+s"(step), "+s"(sixth));
+        asm volatile("" : "+v"(magic));
+    }
+    __device__ __forceinline__ double operator()(double z) const {
+        const double t = __builtin_fma(z, per_step, magic);
+        const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+        const double r = __builtin_fma(t - magic, step, z);
+        U2 two = table[n & (kSteps - 1)];
+        two.y += n << 12;
+        const double f = __builtin_bit_cast(double, two);
+        const double q = __builtin_fma(__builtin_fma(r, sixth, 0.5), r, 1.0);
+        return __builtin_fma(f * r, q, f);
+    }
+};
+
+// A distribution over a row's places: z = cap tanh(x / cap) / T, relative to that of `top`.
+struct Scale {
+    double inv_heat, top_z;     // 1 / T, z of the top
+    double cap_heat, inv_cap2;  // cap / T and 2 / cap (0: no cap)
+    float top;
+};
+
+// tanh(x / cap) by e^(-2 |x / cap|): the quotient's Newton steps start from the hardware's estimate.
+__device__ __forceinline__ double tanh_of(double x, double inv_cap2, const Exp& exp) {
+    const double z = -__builtin_fabs(x) * inv_cap2;
+    const double e = z >= kLeast ? exp(z) : 0.0, d = 1.0 + e;
+    double y = __builtin_amdgcn_rcp(d);
+    y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+    y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+    return __builtin_copysign((1.0 - e) * y, x);
+}
+// CAP: the target's or the drafter's logits are capped.
+template <bool CAP>
+__device__ __forceinline__ double heated(float x, const Scale& s, const Exp& exp) {
+    return CAP && s.inv_cap2 > 0.0 ? s.cap_heat * tanh_of(x, s.inv_cap2, exp) : (double)x * s.inv_heat;
+}
+template <bool CAP>
+__device__ __forceinline__ Scale scale_of(float top, double cap, double inv_heat, const Exp& exp) {
+    Scale s{inv_heat, 0.0, cap * inv_heat, CAP && cap > 0.0 ? 2.0 / cap : 0.0, top};
+    s.top_z = heated<CAP>(top, s, exp);
+    return s;
+}
+// e^(z(x) - z(top)); 0 for -inf, NaN and less than e^-700.
+template <bool CAP>
+__device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp) {
+    const double z = CAP ? heated<CAP>(x, s, exp) - s.top_z : __builtin_fma((double)x, s.inv_heat, -s.top_z);
+    const double e = z >= kLeast ? exp(z) : 0.0;
+    if (CAP && s.inv_cap2 > 0.0) return x > -kInf ? e : 0.0;
+    return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
+}
+// The same as a term of a sum, where e^-700 is nothing; the top finite, or capped and not -inf.
+template <bool CAP>
+__device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) {
+    if (CAP && s.inv_cap2 > 0.0) return weight<CAP>(x, s, exp);
+    double z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
+    asm("v_max_f64 %0, %1, %2" : "=v"(z) : "v"(z), "s"(kLeast));  // NaN too; the compiler's form takes two
+    return exp(z);
 }
 
-// e^(z(x) - z(top)); 0 for -inf and NaN.
-__device__ __forceinline__ double weight(float x, float top, double z_top, double cap, double inv_heat) {
-    if (x == top) return x == -__builtin_huge_valf() ? 0.0 : 1.0;
-    if (!(x > -__builtin_huge_valf())) return 0.0;
-    return exp((capped(x, cap) - z_top) * inv_heat);
-}
-
-// Eight values from place i0 on; -inf from `end` on.
+// Eight logits from place i0 on, as they are; -inf from `end` on.
 template <bool F32>
-__device__ __forceinline__ void load8(const Logits& l, int64_t row, int i0, int end, float (&x)[8]) {
+__device__ __forceinline__ void load8(const Logits& l, int64_t row, int i0, int end, uint32_t (&w)[F32 ? 8 : 4]) {
+    typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2)));  // rows may start anywhere
+    const int64_t at = row * l.stride + i0;
+    if (i0 + 8 <= end) {
+        const U4* const from = reinterpret_cast<const U4*>(static_cast<const char*>(l.x) + at * (F32 ? 4 : 2));
+#pragma unroll
+        for (int j = 0; j < (F32 ? 2 : 1); ++j) {
+            const U4 v = from[j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * j + i] = v[i];
+        }
+        return;
+    }
     if constexpr (F32) {
-        const float* at = static_cast<const float*>(l.x) + row * l.stride + i0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i0 + i < end ? at[i] : -__builtin_huge_valf();
+        for (int i = 0; i < 8; ++i) w[i] = i0 + i < end ? static_cast<const uint32_t*>(l.x)[at + i] : 0xFF800000u;
     } else {
-        const uint16_t* at = static_cast<const uint16_t*>(l.x) + row * l.stride + i0;
+        const auto one = [&](int i) { return i0 + i < end ? (uint32_t) static_cast<const uint16_t*>(l.x)[at + i] : 0xFF80u; };
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i0 + i < end ? __uint_as_float((uint32_t)at[i] << 16) : -__builtin_huge_valf();
+        for (int i = 0; i < 4; ++i) w[i] = one(2 * i) | one(2 * i + 1) << 16;
     }
 }
+template <bool F32>
+__device__ __forceinline__ float load1(const Logits& l, int64_t row, int at) {
+    const int64_t i = row * l.stride + at;
+    return F32 ? static_cast<const float*>(l.x)[i] : __uint_as_float((uint32_t) static_cast<const uint16_t*>(l.x)[i] << 16);
+}
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+template <int DPP, int ROWS>
+__device__ __forceinline__ double dpp_of(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, DPP, ROWS, 0xf, ROWS == 0xf);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), DPP, ROWS, 0xf, ROWS == 0xf);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Inclusive sums over the lanes (row shifts of 1, 2, 4, 8, then the rows' last lanes to the rows after
+// them), and the sum of all.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += dpp_of<0x111, 0xf>(v);
+    v += dpp_of<0x112, 0xf>(v);
+    v += dpp_of<0x114, 0xf>(v);
+    v += dpp_of<0x118, 0xf>(v);
+    v += dpp_of<0x142, 0xa>(v);
+    v += dpp_of<0x143, 0xc>(v);
     return v;
 }
-// The larger logit, the earlier place of equals.
-__device__ __forceinline__ void better(float& top, int& at, float other, int other_at) {
-    const bool take = other > top || (other == top && other_at < at);
-    top = take ? other : top;
-    at = take ? other_at : at;
+__device__ __forceinline__ double wave_sum(double v) { return lane_of(wave_scan(v), 63); }
+template <int DPP, int ROWS>
+__device__ __forceinline__ float dpp_top(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), DPP, ROWS, 0xf, false)));
 }
-__device__ __forceinline__ void wave_best(float& top, int& at) {
+__device__ __forceinline__ float wave_top(float v) {
+    v = dpp_top<0x118, 0xf>(dpp_top<0x114, 0xf>(dpp_top<0x112, 0xf>(dpp_top<0x111, 0xf>(v))));
+    v = dpp_top<0x143, 0xc>(dpp_top<0x142, 0xa>(v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ int wave_least(int v) {
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) {
-        const float t = __shfl_xor(top, d);
-        const int i = __shfl_xor(at, d);
-        better(top, at, t, i);
+        const int o = __shfl_xor(v, d);
+        v = o < v ? o : v;
     }
-}
-__device__ __forceinline__ double group_sum(double v, double* sums) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double all = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) all += sums[w];
-    return all;
+    return v;
 }
 
 // The request of a row; `requests` for none.  Every lane of the wave takes part.
@@ -128,56 +232,75 @@ __device__ __forceinline__ int start_of(const Args& a, int r) { return a.starts 
 // 0 where the request is greedy
 __device__ __forceinline__ double inv_heat_of(const Args& a, int r) {
     const float t = a.heats != nullptr ? a.heats[r] : a.heat;
-    return t > 0.0f ? 1.0 / (double)t : 0.0;
+    return t > 0.0f ? 1.0 / (double)fminf(t, 1e30f) : 0.0;  // past that all finite logits are equal
 }
 
-template <bool F32, int SWEEPS>
-__global__ __launch_bounds__(kThreads) void stats_kernel(Args a, Work w, Chunks c) {
-    __shared__ double sums[kWaves];
-    __shared__ float tops[kWaves];
-    __shared__ int ats[kWaves];
-    const int tid = (int)threadIdx.x;
-    const int index = (int)blockIdx.x / c.count, chunk = (int)blockIdx.x - index * c.count;
-    const bool of_draft = index >= a.rows;
-    const int row = of_draft ? index - a.rows : index;
+constexpr int kNowhere = 0x7fffffff;
+
+// A part's logits as a wave holds them: lane l has places 512 j + 8 l + i (j < S, i < 8).
+template <bool F32, int S>
+struct Held {
+    uint32_t w[S][F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const Logits& l, int64_t row, int begin, int vocab) {
+        const int lane = (int)threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < S; ++j) load8<F32>(l, row, begin + 512 * j + 8 * lane, vocab, w[j]);
+    }
+    __device__ __forceinline__ float at(int j, int i) const {
+        if (F32) return __uint_as_float(w[j][i]);
+        return __uint_as_float((i & 1) ? w[j][i / 2] & 0xFFFF0000u : w[j][i / 2] << 16);
+    }
+};
+
+template <bool F32, bool CAP, int S>
+__global__ __launch_bounds__(kStatsThreads, CAP ? 4 : 8) void stats_kernel(Args a, Work w, Plan plan) {
+    __shared__ U2 table[kSteps];
+    const int lane = (int)threadIdx.x & 63;
+    const Place place = place_of(plan, __builtin_amdgcn_readfirstlane((int)blockIdx.x * (kStatsThreads / 64) + ((int)threadIdx.x >> 6)));
+    const bool of_draft = place.row >= a.rows;  // the plan has those rows only where there is a drafter
+    const int row = of_draft ? place.row - a.rows : place.row;
     const Logits& l = of_draft ? a.draft : a.target;
-    const int begin = chunk * c.size, end = begin + c.size < a.vocab ? begin + c.size : a.vocab;
-    float x[SWEEPS][8];
-#pragma unroll
-    for (int s = 0; s < SWEEPS; ++s) load8<F32>(l, row, begin + s * kSweep + 8 * tid, end, x[s]);
-    const int r = request_of(a, row);
-    if (r >= a.requests) return;  // padding
-    float top = -__builtin_huge_valf();
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int s = 0; s < SWEEPS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (x[s][i] > top) {
-                top = x[s][i];
-                at = begin + s * kSweep + 8 * tid + i;
-            }
-    wave_best(top, at);
-    if ((tid & 63) == 0) {
-        tops[tid >> 6] = top;
-        ats[tid >> 6] = at;
-    }
+    const int begin = place.part * plan.size();
+    Held<F32, S> x;
+    if (place.part >= 0) x.load(l, row, begin, a.vocab);
+    take_exp2<kStatsThreads>(table);
+    const Exp exp(table);
     __syncthreads();
-    top = tops[0];
-    at = ats[0];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) better(top, at, tops[i], ats[i]);
+    if (place.part < 0) return;
+    const int r = request_of(a, row);
+    if (r >= a.requests) return;                                // padding
+    if (of_draft && row + 1 >= start_of(a, r + 1)) return;      // no draft was drawn from it
     const double inv_heat = inv_heat_of(a, r);
+    float top = -kInf;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, x.at(j, i));  // NaN has no say
+    top = wave_top(top);
     double sum = 0.0;
+    int at = kNowhere;
     if (inv_heat > 0.0) {
-        const double cap = l.cap, z_top = capped(top, cap);
+        const Scale scale = scale_of<CAP>(top, l.cap, inv_heat, exp);
+        if (top > -kInf && (top < kInf || (CAP && scale.inv_cap2 > 0.0))) {
 #pragma unroll
-        for (int s = 0; s < SWEEPS; ++s)
+            for (int j = 0; j < S; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += weight(x[s][i], top, z_top, cap, inv_heat);
-        sum = group_sum(sum, sums);
+                for (int i = 0; i < 8; ++i) sum += term<CAP>(x.at(j, i), scale, exp);
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += x.at(j, i) == kInf;  // infinities share all there is; -inf has none
+        }
+        sum = wave_sum(sum);
+    } else if (top > -kInf) {
+#pragma unroll
+        for (int j = S - 1; j >= 0; --j)
+#pragma unroll
+            for (int i = 7; i >= 0; --i) at = x.at(j, i) == top ? begin + 512 * j + 8 * lane + i : at;
+        at = wave_least(at);
     }
-    if (tid == 0) w.parts[(int64_t)index * c.count + chunk] = Part{sum, top, at};
+    if (lane == 0) w.parts[(int64_t)place.row * plan.parts + place.part] = Part{sum, top, at};
 }
 
 struct Total {
@@ -185,301 +308,425 @@ struct Total {
     float top;
     int at;
 };
-// A row's chunks joined, by the lanes of a wave.
-__device__ __forceinline__ Total join(const Part* parts, int count, double cap, double inv_heat) {
+// A row's parts joined, by the lanes of a wave.
+template <bool CAP, int HELD>
+__device__ __forceinline__ Total join(const Part* parts, int count, double cap, double inv_heat, const Exp& exp) {
     const int lane = (int)threadIdx.x & 63;
-    Total t{0.0, -__builtin_huge_valf(), 0x7fffffff};
-    for (int i = lane; i < count; i += 64) better(t.top, t.at, parts[i].top, parts[i].at);
-    wave_best(t.top, t.at);
+    Total t{0.0, -kInf, kNowhere};
+    const Part none{0.0, -kInf, kNowhere};
+    // the first of a lane's parts stay in registers
+    constexpr int kHeld = HELD;
+    Part held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = lane + 64 * i < count ? parts[lane + 64 * i] : none;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) t.top = fmaxf(t.top, held[i].top);
+    for (int i = lane + 64 * kHeld; i < count; i += 64) t.top = fmaxf(t.top, parts[i].top);
+    t.top = wave_top(t.top);
     if (inv_heat > 0.0) {
-        const double z_top = capped(t.top, cap);
-        for (int i = lane; i < count; i += 64) t.sum += parts[i].sum * weight(parts[i].top, t.top, z_top, cap, inv_heat);
+        const Scale scale = scale_of<CAP>(t.top, cap, inv_heat, exp);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) t.sum += held[i].sum * weight<CAP>(held[i].top, scale, exp);
+        for (int i = lane + 64 * kHeld; i < count; i += 64) t.sum += parts[i].sum * weight<CAP>(parts[i].top, scale, exp);
         t.sum = wave_sum(t.sum);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (held[i].top == t.top) t.at = held[i].at < t.at ? held[i].at : t.at;
+        for (int i = lane + 64 * kHeld; i < count; i += 64)
+            if (parts[i].top == t.top) t.at = parts[i].at < t.at ? parts[i].at : t.at;
+        t.at = wave_least(t.at);
     }
     return t;
 }
 
-// The probability of place `at`, as of its row's total.
-__device__ __forceinline__ double chance(const Logits& l, int64_t row, int at, int vocab, const Total& t, double inv_heat) {
+// The weight of place `at` of a row of that total; greedy: 1 at its first largest logit.
+template <bool F32, bool CAP>
+__device__ __forceinline__ double weight_at(const Logits& l, int64_t row, int at, int vocab, const Total& t, double inv_heat, const Exp& exp) {
     if (at < 0 || at >= vocab) return 0.0;
     if (!(inv_heat > 0.0)) return at == t.at ? 1.0 : 0.0;
-    const double w = weight(value_of(l, row * l.stride + at), t.top, capped(t.top, l.cap), l.cap, inv_heat);
-    return t.sum > 0.0 ? w / t.sum : 0.0;
+    return weight<CAP>(load1<F32>(l, row, at), scale_of<CAP>(t.top, l.cap, inv_heat, exp), exp);
 }
 
-// The weight of place `at` of a request's row to sample from.
-__device__ __forceinline__ double rest_weight(const Args& a, const Spot& s, int at, float x, float y, double p_z, double q_z, double inv_heat) {
-    double v = weight(x, s.p_top, p_z, a.target.cap, inv_heat) * s.p_scale;
-    if (s.kind == 2) {
-        if (a.draft.x != nullptr) {
-            v -= weight(y, s.q_top, q_z, a.draft.cap, inv_heat) * s.q_scale;
-            v = v > 0.0 ? v : 0.0;
-        } else if (at == s.token) {
-            v = 0.0;
-        }
+// The weights of a request's row to sample from.
+template <bool CAP>
+struct Rest {
+    Scale p, q;
+    double p_scale, q_scale;
+    int token;
+    bool minus_q;
+    __device__ __forceinline__ Rest(const Args& a, const Spot& s, double inv_heat, const Exp& exp)
+        : p(scale_of<CAP>(s.p_top, a.target.cap, inv_heat, exp)), p_scale(s.p_scale), q_scale(s.q_scale), token(s.token),
+          minus_q(s.kind == 2 && a.draft.x != nullptr) {
+        q = minus_q ? scale_of<CAP>(s.q_top, a.draft.cap, inv_heat, exp) : p;
+        plain = (s.p_top < kInf || p.inv_cap2 > 0.0) && (!minus_q || (fabsf(s.q_top) < kInf || (s.q_top > 0.0f && q.inv_cap2 > 0.0)));
     }
-    return v;
+    // what of() gives, as a term of a sum; not where the top is infinite (`plain` says so)
+    bool plain;
+    __device__ __forceinline__ double term_of(int at, float x, float y, const Exp& exp) const {
+        const double v = term<CAP>(x, p, exp) * p_scale;
+        if (minus_q) return __builtin_fmax(v - term<CAP>(y, q, exp) * q_scale, 0.0);
+        return at == token ? 0.0 : v;
+    }
+    // place `at`, whose logit is x and the drafter's y
+    __device__ __forceinline__ double of(int at, float x, float y, const Exp& exp) const {
+        double v = weight<CAP>(x, p, exp) * p_scale;
+        if (minus_q) v = __builtin_fmax(v - weight<CAP>(y, q, exp) * q_scale, 0.0);
+        return at == token ? 0.0 : v;
+    }
+};
+
+// A row's total as what to sample from it.
+__device__ __forceinline__ Spot spot_of(const Total& p, int row, double inv_heat, int kind) {
+    Spot s{};
+    s.row = row;
+    s.kind = inv_heat > 0.0 && p.sum > 0.0 ? kind : 0;
+    s.p_top = p.top;
+    s.p_scale = p.sum > 0.0 ? 1.0 / p.sum : 0.0;
+    s.token = -1;
+    return s;
 }
 
-template <bool F32>
-__global__ __launch_bounds__(kThreads) void rest_kernel(Args a, Work w, Chunks c) {
-    __shared__ double sums[kWaves];
-    __shared__ int firsts[kWaves];
+// Greedy, or nothing has a weight: the first largest logit, or none.
+__device__ __forceinline__ int greedy_token(const Total& p, double inv_heat) { return !(inv_heat > 0.0) && p.at != kNowhere ? p.at : -1; }
+
+// `groups` workgroups to a request; each finds its first draft that falls, and its waves take
+// the parts of that row.
+template <bool F32, bool CAP, int S>
+__global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, int groups) {
+    constexpr int kWaves = kWide / 64, kHeld = S == 1 ? 8 : 2;  // a row of 262144
+    __shared__ U2 table[kSteps];
+    __shared__ Total totals[2][kWaves];  // of the rows in hand, and of the drafter's
+    __shared__ int falls[kWaves];
     __shared__ Spot spot;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r = (int)blockIdx.x / c.count, chunk = (int)blockIdx.x - r * c.count;
-    const int start = start_of(a, r);
-    const int n = a.starts == nullptr ? 1 : start_of(a, r + 1) - start;
+    const int r = (int)blockIdx.x / groups, chunk = (int)blockIdx.x - r * groups;
+    take_exp2<kWide>(table);
+    const Exp exp(table);
+    const int start = start_of(a, r), n = start_of(a, r + 1) - start;
     if (chunk == 0) {
         // rows of no request
-        if (a.starts != nullptr && r == a.requests - 1)
-            for (int i = clampi(a.starts[a.requests], 0, a.rows) + tid; i < a.rows; i += kThreads) a.out[i] = -1;
-        if (a.starts != nullptr && r == 0)
-            for (int i = tid; i < start; i += kThreads) a.out[i] = -1;
+        if (r == a.requests - 1)
+            for (int i = clampi(a.starts[a.requests], 0, a.rows) + tid; i < a.rows; i += kWide) a.out[i] = -1;
+        if (r == 0)
+            for (int i = tid; i < start; i += kWide) a.out[i] = -1;
     }
     if (n <= 0) {
         if (chunk == 0 && tid == 0) {
-            if (a.accepted != nullptr) a.accepted[r] = 0;
-            w.spots[r].kind = 0;
+            a.accepted[r] = 0;
+            w.spots[r] = Spot{};  // pick_kernel reads a row's sums before it looks at the kind
         }
         return;
     }
     const double inv_heat = inv_heat_of(a, r);
-    const Part* const parts = w.parts + (int64_t)start * c.count;
-    const Part* const draft_parts = w.parts + ((int64_t)a.rows + start) * c.count;
-
-    // the first draft that falls: a wave to a row
-    int first = n - 1;
-    for (int i = wave; i < n - 1 && i < first; i += kWaves) {
-        const int token = a.tokens[start + i + 1];
-        const Total p = join(parts + (int64_t)i * c.count, c.count, a.target.cap, inv_heat);
-        const double p_at = chance(a.target, start + i, token, a.vocab, p, inv_heat);
-        double q_at = 1.0;
-        if (a.draft.x != nullptr) {
-            const Total q = join(draft_parts + (int64_t)i * c.count, c.count, a.draft.cap, inv_heat);
-            q_at = chance(a.draft, start + i, token, a.vocab, q, inv_heat);
-        }
-        if (!((double)a.uniforms[2 * (start + i)] * q_at < p_at)) first = i;
-    }
-    if (lane == 0) firsts[wave] = first;
+    const Part* const own = w.parts + (int64_t)start * parts;
+    const Part* const drafts = w.parts + ((int64_t)a.rows + start) * parts;
+    const bool drafter = a.draft.x != nullptr;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) first = firsts[i] < first ? firsts[i] : first;
 
-    if (wave == 0) {
-        Spot s{};
-        s.row = start + first;
-        const Total p = join(parts + (int64_t)first * c.count, c.count, a.target.cap, inv_heat);
-        s.kind = inv_heat > 0.0 && p.sum > 0.0 ? (first < n - 1 ? 2 : 1) : 0;
-        s.p_top = p.top;
-        s.p_scale = p.sum > 0.0 ? 1.0 / p.sum : 0.0;
-        s.token = -1;
+    // The first draft that falls: a wave to each join, so many rows at a time.
+    const int per = drafter ? kWaves / 2 : kWaves;
+    int first = n - 1;
+    Total p_first{}, q_first{};
+    for (int base = 0;; base += per) {
+        const int i = base + wave % per;
+        const bool of_q = wave >= per;
+        if (i < n - of_q) totals[of_q][wave % per] = of_q ? join<CAP, kHeld>(drafts + (int64_t)i * parts, parts, a.draft.cap, inv_heat, exp)
+                                                  : join<CAP, kHeld>(own + (int64_t)i * parts, parts, a.target.cap, inv_heat, exp);
+        __syncthreads();
+        if (!of_q) {
+            int fall = kNowhere;
+            if (i < n - 1) {
+                const int token = a.tokens[start + i + 1];
+                const bool greedy = !(inv_heat > 0.0);
+                const Total p = totals[0][wave], q = totals[1][wave];
+                const double p_at = weight_at<F32, CAP>(a.target, start + i, token, a.vocab, p, inv_heat, exp);
+                const double q_at = drafter ? weight_at<F32, CAP>(a.draft, start + i, token, a.vocab, q, inv_heat, exp) : 1.0;
+                // u q < p, times both sums (a drafter's row without any weight has q = 0)
+                const double p_sum = greedy ? 1.0 : p.sum, q_sum = greedy || !drafter || !(q.sum > 0.0) ? 1.0 : q.sum;
+                if (!((double)a.uniforms[2 * (start + i)] * q_at * p_sum < p_at * q_sum)) fall = i;
+            } else if (i == n - 1) {
+                fall = i;  // the last row has no draft
+            }
+            if (lane == 0) falls[wave] = fall;
+        }
+        __syncthreads();
+        int least = kNowhere;
+        for (int j = 0; j < per; ++j) least = falls[j] < least ? falls[j] : least;
+        if (least != kNowhere) {
+            first = least;
+            p_first = totals[0][least - base];
+            if (drafter) q_first = totals[1][least - base];
+            break;
+        }
+        __syncthreads();  // the totals are read
+    }
+
+    if (tid == 0) {
+        Spot s = spot_of(p_first, start + first, inv_heat, first < n - 1 ? 2 : 1);
         if (s.kind == 2) {
-            if (a.draft.x != nullptr) {
-                const Total q = join(draft_parts + (int64_t)first * c.count, c.count, a.draft.cap, inv_heat);
-                s.q_top = q.top;
-                s.q_scale = q.sum > 0.0 ? 1.0 / q.sum : 0.0;
+            if (drafter) {
+                s.q_top = q_first.top;
+                s.q_scale = q_first.sum > 0.0 ? 1.0 / q_first.sum : 0.0;
             } else {
                 s.token = a.tokens[s.row + 1];
             }
         }
-        if (lane == 0) {
-            spot = s;
-            if (chunk == 0) {
-                w.spots[r] = s;
-                if (a.accepted != nullptr) a.accepted[r] = first;
-                // greedy, or nothing has a weight: the first largest logit, or none
-                if (s.kind == 0) a.out[s.row] = !(inv_heat > 0.0) && p.at < a.vocab ? p.at : -1;
-            }
+        spot = s;
+        if (chunk == 0) {
+            w.spots[r] = s;
+            a.accepted[r] = first;
+            if (s.kind == 0) a.out[s.row] = greedy_token(p_first, inv_heat);
         }
     }
     __syncthreads();
     if (chunk == 0)
-        for (int i = tid; i < n; i += kThreads)
+        for (int i = tid; i < n; i += kWide)
             if (i != first) a.out[start + i] = i < first ? a.tokens[start + i + 1] : -1;
     const Spot s = spot;
-    if (s.kind != 2) return;  // p's sums are those of its chunks
+    if (s.kind != 2) return;  // p's sums are those of its parts
 
-    const double p_z = capped(s.p_top, a.target.cap), q_z = capped(s.q_top, a.draft.cap);
-    const int begin = chunk * c.size, end = begin + c.size < a.vocab ? begin + c.size : a.vocab;
-    double sum = 0.0;
-    for (int i0 = begin + 8 * tid; i0 < end; i0 += kSweep) {
-        float x[8], y[8] = {};
-        load8<F32>(a.target, s.row, i0, end, x);
-        if (a.draft.x != nullptr) load8<F32>(a.draft, s.row, i0, end, y);
+    const Rest<CAP> rest(a, s, inv_heat, exp);
+    for (int part = first_part(chunk, wave); part < parts; part += part_step(groups)) {
+        const int begin = part * 512 * S;
+        double sum = 0.0;
+        if (rest.plain) {
+            constexpr int kAtOnce = F32 && S > 2 ? 2 : S;  // four sweeps of both in fp32 are more than 128 registers
+#pragma unroll 1
+            for (int from = begin; from < begin + 512 * S; from += 512 * kAtOnce) {
+                Held<F32, kAtOnce> x, y{};
+                x.load(a.target, s.row, from, a.vocab);
+                if (drafter) y.load(a.draft, s.row, from, a.vocab);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += rest_weight(a, s, i0 + i, x[i], y[i], p_z, q_z, inv_heat);
+                for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum += rest.term_of(from + 512 * j + 8 * lane + i, x.at(j, i), y.at(j, i), exp);
+            }
+        } else {
+            const int end = begin + 512 * S < a.vocab ? begin + 512 * S : a.vocab;
+            for (int i = begin + lane; i < end; i += 64)
+                sum += rest.of(i, load1<F32>(a.target, s.row, i), drafter ? load1<F32>(a.draft, s.row, i) : -kInf, exp);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) w.rest[(int64_t)r * parts + part] = sum;
     }
-    sum = group_sum(sum, sums);
-    if (tid == 0) w.rest[(int64_t)r * c.count + chunk] = sum;
 }
 
-// Inclusive sums over the workgroup's threads; `total` of all of them.
+// Inclusive sums over the workgroup's threads, `total` of all; sums: scratch of a value per wave.
 __device__ __forceinline__ double group_scan(double v, double* sums, double* total) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double up = __shfl_up(v, d);
-        v += lane >= d ? up : 0.0;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = v;
+    const int wave = (int)threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();  // the scan before is read
+    if ((threadIdx.x & 63) == 63) sums[wave] = v;
     __syncthreads();
     double before = 0.0, all = 0.0;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < kWide / 64; ++i) {
         before += i < wave ? sums[i] : 0.0;
         all += sums[i];
     }
     *total = all;
     return v + before;
 }
+// Least and largest of the workgroup's `first` and `last`; in every thread.
+__device__ __forceinline__ void group_ends(int& first, int& last, int (*ends)[2]) {
+    first = wave_least(first);
+    last = -wave_least(-last);
+    if ((threadIdx.x & 63) == 0) {
+        ends[threadIdx.x >> 6][0] = first;
+        ends[threadIdx.x >> 6][1] = last;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWide / 64; ++i) {
+        first = ends[i][0] < first ? ends[i][0] : first;
+        last = ends[i][1] > last ? ends[i][1] : last;
+    }
+}
 
-template <bool F32>
-__global__ __launch_bounds__(kThreads) void pick_kernel(Args a, Work w, Chunks c) {
-    __shared__ double sums[kWaves];
-    __shared__ int found, last;
-    __shared__ double found_before;
-    const int tid = (int)threadIdx.x, r = (int)blockIdx.x;
-    Spot s = w.spots[r];
-    if (s.kind == 0) return;
+// DRAFTS: spots and sums are rest_kernel's; else each row is a request and is joined here.
+template <bool F32, bool CAP, bool DRAFTS>
+__global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) {
+    __shared__ U2 table[kSteps];
+    __shared__ double sums[kWide / 64];
+    __shared__ int ends[2][kWide / 64][2];
+    __shared__ float tops[kWide / 64];
+    __shared__ double before_found;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = (int)blockIdx.x;
+    const int parts = plan.parts;
+    Spot s{};
+    s.row = r;
+    if (DRAFTS) s = w.spots[r];
+    const Part* const own = w.parts + (int64_t)s.row * parts;
+    const Part none{0.0, -kInf, kNowhere};
+    const Part mine = tid < parts ? own[tid] : none;
+    const double* const rest = w.rest + (int64_t)r * parts;
+    const double my_rest = DRAFTS && s.kind == 2 && tid < parts ? rest[tid] : 0.0;
+    const double u = (double)(DRAFTS ? a.uniforms[2 * s.row + 1] : a.uniforms[s.row]);
     const double inv_heat = inv_heat_of(a, r);
-    const double u = (double)(a.starts == nullptr ? a.uniforms[s.row] : a.uniforms[2 * s.row + 1]);
-    const double* const rest = w.rest + (int64_t)r * c.count;
-    const Part* const parts = w.parts + (int64_t)s.row * c.count;
-    const double p_z = capped(s.p_top, a.target.cap), q_z = s.kind == 2 ? capped(s.q_top, a.draft.cap) : 0.0;
-    const auto chunk_weight = [&](int i) {
-        if (i >= c.count) return 0.0;
-        return s.kind == 2 ? rest[i] : parts[i].sum * weight(parts[i].top, s.p_top, p_z, a.target.cap, inv_heat) * s.p_scale;
+    take_exp2<kWide>(table);
+    const Exp exp(table);
+    if constexpr (DRAFTS) {
+        if (s.kind == 0) return;
+        __syncthreads();
+    } else {
+        s.kind = 1;
+        s.token = -1;
+        float top = mine.top;
+        for (int i = tid + kWide; i < parts; i += kWide) top = fmaxf(top, own[i].top);
+        top = wave_top(top);
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWide / 64; ++i) top = fmaxf(top, tops[i]);
+        s.p_top = top;
+        s.p_scale = 1.0;  // weights need not add to one
+        if (!(inv_heat > 0.0)) {
+            int at = mine.top == top ? mine.at : kNowhere, last = -1;
+            for (int i = tid + kWide; i < parts; i += kWide)
+                if (own[i].top == top) at = own[i].at < at ? own[i].at : at;
+            group_ends(at, last, ends[0]);
+            if (tid == 0) a.out[r] = at != kNowhere ? at : -1;
+            return;
+        }
+    }
+
+    // The part: the first whose sum with those before it exceeds the goal, else (rounding, or u >= 1)
+    // the last with any weight.
+    const Scale scale = scale_of<CAP>(s.p_top, a.target.cap, inv_heat, exp);
+    const auto part_weight = [&](int i) {
+        if (i >= parts) return 0.0;
+        if (DRAFTS && s.kind == 2) return i == tid ? my_rest : rest[i];
+        const Part p = i == tid ? mine : own[i];
+        return p.sum * weight<CAP>(p.top, scale, exp) * s.p_scale;
     };
-    double total = 0.0;
+    double first_weight, upto, total;
     const auto sum_all = [&]() {
-        total = 0.0;
-        for (int base = 0; base < c.count; base += kThreads) total += group_sum(chunk_weight(base + tid), sums);
+        first_weight = part_weight(tid);
+        upto = group_scan(first_weight, sums, &total);
+        for (int base = kWide; base < parts; base += kWide) {
+            double here;
+            (void)group_scan(part_weight(base + tid), sums, &here);
+            total += here;
+        }
     };
     sum_all();
-    if (s.kind == 2 && !(total > 0.0)) {
+    if (DRAFTS && s.kind == 2 && !(total > 0.0)) {
         s.kind = 1;  // p and q are equal to the last bit
+        s.token = -1;
         sum_all();
     }
     const double goal = u * total;
-    // the chunk: the first whose sum with those before it exceeds the goal, else the last with any weight
-    if (tid == 0) {
-        found = 0x7fffffff;
-        last = -1;
-        found_before = 0.0;
+    double before = 0.0, v = first_weight;
+    int part = kNowhere, last = -1;
+    for (int base = 0;;) {
+        int found = v > 0.0 && before + upto > goal ? base + tid : kNowhere, held = v > 0.0 ? base + tid : -1;
+        const int asked = found;
+        __syncthreads();
+        group_ends(found, held, ends[0]);
+        last = held > last ? held : last;
+        if (found != kNowhere) {
+            if (asked == found) before_found = before + upto - v;
+            part = found;
+            break;
+        }
+        base += kWide;
+        if (base >= parts) break;
+        double here;
+        (void)group_scan(v, sums, &here);
+        before += here;
+        v = part_weight(base + tid);
+        upto = group_scan(v, sums, &here);
     }
     __syncthreads();
-    double before = 0.0;
-    for (int base = 0; base < c.count; base += kThreads) {
-        const double v = chunk_weight(base + tid);
-        double here;
-        const double upto = before + group_scan(v, sums, &here);
-        if (v > 0.0) atomicMax(&last, base + tid);
-        if (v > 0.0 && upto > goal) atomicMin(&found, base + tid);
-        __syncthreads();
-        if (found == base + tid) found_before = upto - v;
-        __syncthreads();
-        if (found != 0x7fffffff) break;
-        before += here;
-    }
-    const bool past = found == 0x7fffffff;  // rounding, or u >= 1: the last place with any weight
-    const int chunk = past ? last : found;
-    if (chunk < 0) {  // no weight at all: logits that are no numbers
+    const bool past = part == kNowhere;
+    if (past) part = last;
+    if (part < 0) {  // no weight at all
         if (tid == 0) a.out[s.row] = -1;
         return;
     }
-    const double before_chunk = found_before;
-    __syncthreads();
-    if (tid == 0) {
-        found = 0x7fffffff;
-        last = -1;
-    }
-    __syncthreads();
-    const int begin = chunk * c.size, end = begin + c.size < a.vocab ? begin + c.size : a.vocab;
-    before = past ? 0.0 : before_chunk;
-    for (int base = begin; base < end; base += kSweep) {
-        const int i0 = base + 8 * tid;
-        float x[8], y[8] = {};
-        double v[8], sum = 0.0;
-        load8<F32>(a.target, s.row, i0, end, x);
-        if (s.kind == 2 && a.draft.x != nullptr) load8<F32>(a.draft, s.row, i0, end, y);
+
+    // The place in it, likewise.
+    const Rest<CAP> of(a, s, inv_heat, exp);
+    const int i0 = part * plan.size() + 2 * tid;
+    const bool within = 2 * tid < plan.size();
+    double each[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] = i0 + i < end ? rest_weight(a, s, i0 + i, x[i], y[i], p_z, q_z, inv_heat) : 0.0;
-            sum += v[i];
-        }
-        double here;
-        double upto = before + group_scan(sum, sums, &here) - sum;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            upto += v[i];
-            if (v[i] > 0.0) {
-                atomicMax(&last, i0 + i);
-                if (!past && upto > goal) atomicMin(&found, i0 + i);
-            }
-        }
-        __syncthreads();
-        if (found != 0x7fffffff) break;
-        before += here;
+    for (int i = 0; i < 2; ++i) {
+        const bool live = within && i0 + i < a.vocab;
+        const float x = live ? load1<F32>(a.target, s.row, i0 + i) : -kInf;
+        const float y = live && of.minus_q ? load1<F32>(a.draft, s.row, i0 + i) : -kInf;
+        each[i] = of.of(i0 + i, x, y, exp);
     }
-    if (tid == 0) a.out[s.row] = found != 0x7fffffff ? found : last;
+    upto = group_scan(each[0] + each[1], sums, &total) + (past ? 0.0 : before_found);
+    int found = kNowhere, held = -1;
+    if (each[1] > 0.0) {
+        held = i0 + 1;
+        if (!past && upto > goal) found = i0 + 1;
+    }
+    if (each[0] > 0.0) {
+        held = held < 0 ? i0 : held;
+        if (!past && upto - each[1] > goal) found = i0;
+    }
+    group_ends(found, held, ends[1]);
+    if (tid == 0) a.out[s.row] = found != kNowhere ? found : held;
 }
 
-// Chunks of whole sweeps: about as many as fill the card twice, of 2048 to 8192 places.
-Chunks chunks_of(const Args& a) {
-    const int rows = a.rows * (a.draft.x != nullptr ? 2 : 1);
-    const int sweeps = ceil_div(a.vocab, kSweep);
-    int per = 1;
-    while (per < 4 && (int64_t)ceil_div(sweeps, 2 * per) * rows >= 1024) per *= 2;
-    return Chunks{per * kSweep, ceil_div(sweeps, per)};
+int stats_rows(const Args& a) { return a.rows * (a.draft.x != nullptr ? 2 : 1); }
+Plan plan_of(const Args& a) { return verify::plan_of(stats_rows(a), a.vocab); }
+
+// A launch counts its threads in 32 bits.
+constexpr int64_t kMostThreads = 0xFFFFFFFFll;
+
+size_t part_bytes(const Plan& p) { return (size_t)p.rows * p.parts * sizeof(Part); }
+size_t rest_bytes(const Args& a, const Plan& p) {
+    return a.starts == nullptr ? 0 : (((size_t)a.requests * p.parts * sizeof(double)) + 15) & ~(size_t)15;
 }
+size_t spot_bytes(const Args& a) { return a.starts == nullptr ? 0 : (size_t)a.requests * sizeof(Spot); }
 
-// Workgroups of a launch, which counts its threads in 32 bits.
-constexpr int64_t kMostGroups = 0xFFFFFFFFll / kThreads;
-
-size_t part_bytes(const Args& a, const Chunks& c) { return (size_t)a.rows * (a.draft.x != nullptr ? 2 : 1) * c.count * sizeof(Part); }
-size_t rest_bytes(const Args& a, const Chunks& c) { return (((size_t)a.requests * c.count * sizeof(double)) + 15) & ~(size_t)15; }
-
-template <bool F32>
-hipError_t launch_of(const Args& a, const Work& w, const Chunks& c, hipStream_t stream) {
-    const unsigned rows = (unsigned)(a.rows * (a.draft.x != nullptr ? 2 : 1)) * (unsigned)c.count;
-    switch (c.size / kSweep) {
-        case 1: stats_kernel<F32, 1><<<rows, kThreads, 0, stream>>>(a, w, c); break;
-        case 2: stats_kernel<F32, 2><<<rows, kThreads, 0, stream>>>(a, w, c); break;
-        case 4: stats_kernel<F32, 4><<<rows, kThreads, 0, stream>>>(a, w, c); break;
-        default: return hipErrorInvalidValue;
-    }
+template <bool F32, bool CAP, int S>
+hipError_t launch_of(const Args& a, const Work& w, const Plan& p, hipStream_t stream) {
+    stats_kernel<F32, CAP, S><<<(unsigned)p.groups(), kStatsThreads, 0, stream>>>(a, w, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    rest_kernel<F32><<<(unsigned)a.requests * (unsigned)c.count, kThreads, 0, stream>>>(a, w, c);
+    if (a.starts == nullptr) {
+        pick_kernel<F32, CAP, false><<<(unsigned)a.requests, kWide, 0, stream>>>(a, w, p);
+        return hipGetLastError();
+    }
+    const int groups = rest_groups(a.requests, p.parts);
+    rest_kernel<F32, CAP, S><<<(unsigned)a.requests * (unsigned)groups, kWide, 0, stream>>>(a, w, p.parts, groups);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    pick_kernel<F32><<<(unsigned)a.requests, kThreads, 0, stream>>>(a, w, c);
+    pick_kernel<F32, CAP, true><<<(unsigned)a.requests, kWide, 0, stream>>>(a, w, p);
     return hipGetLastError();
+}
+template <bool F32, bool CAP>
+hipError_t launch_of(const Args& a, const Work& w, const Plan& p, hipStream_t stream) {
+    return p.sweeps == 1 ? launch_of<F32, CAP, 1>(a, w, p, stream) : launch_of<F32, CAP, 4>(a, w, p, stream);
 }
 
 }  // namespace
 
 bool fits(const Args& a) {
-    const Chunks c = chunks_of(a);
-    const int64_t rows = (int64_t)a.rows * (a.draft.x != nullptr ? 2 : 1);
-    return rows * c.count <= kMostGroups && (int64_t)a.requests * c.count <= kMostGroups;
+    const Plan p = plan_of(a);
+    return p.groups() * kStatsThreads <= kMostThreads && (int64_t)a.requests * rest_groups(a.requests, p.parts) * kWide <= kMostThreads;
 }
 
 size_t scratch_bytes(const Args& a) {
-    const Chunks c = chunks_of(a);
-    return part_bytes(a, c) + rest_bytes(a, c) + (size_t)a.requests * sizeof(Spot);
+    const Plan p = plan_of(a);
+    return part_bytes(p) + rest_bytes(a, p) + spot_bytes(a);
 }
 
 hipError_t launch(const Args& a, void* scratch, hipStream_t stream) {
-    const Chunks c = chunks_of(a);
+    const Plan p = plan_of(a);
     char* at = static_cast<char*>(scratch);
     Work w;
     w.parts = reinterpret_cast<Part*>(at);
-    w.rest = reinterpret_cast<double*>(at + part_bytes(a, c));
-    w.spots = reinterpret_cast<Spot*>(at + part_bytes(a, c) + rest_bytes(a, c));
-    return a.target.f32 ? launch_of<true>(a, w, c, stream) : launch_of<false>(a, w, c, stream);
+    w.rest = reinterpret_cast<double*>(at + part_bytes(p));
+    w.spots = reinterpret_cast<Spot*>(at + part_bytes(p) + rest_bytes(a, p));
+    const bool cap = a.target.cap > 0.0f || a.draft.cap > 0.0f;
+    if (a.target.f32) return cap ? launch_of<true, true>(a, w, p, stream) : launch_of<true, false>(a, w, p, stream);
+    return cap ? launch_of<false, true>(a, w, p, stream) : launch_of<false, false>(a, w, p, stream);
 }
 
 }  // namespace verify

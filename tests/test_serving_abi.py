@@ -287,3 +287,30 @@ def test_python_refuses_what_is_not_on_the_gpu():
         sampling.verify_drafts(floats, ints[:2], ints[:2], floats[:, :2])
     with pytest.raises(qmm.Gemma4Error, match="block scales"):
         A._block_scales(torch.zeros(1, 1, 1, dtype=torch.uint8), 1.0, torch.zeros(1, 1, 16, 64), 1, 2)
+
+
+# ------------------------------------------------------------------ the sampling kernels' shares
+
+@pytest.fixture(scope="module")
+def shares():
+    so = os.path.join(HERE, "_build", "libverifyindex.so")
+    src, dep = os.path.join(HERE, "verify_index_host.cpp"), os.path.join(hbuild.CSRC, "verify_index.h")
+    if not os.path.exists(so) or any(os.path.getmtime(d) > os.path.getmtime(so) for d in (src, dep)):
+        os.makedirs(os.path.dirname(so), exist_ok=True)
+        subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                        "-I", hbuild.CSRC, src, "-o", so], check=True, capture_output=True)
+    return ctypes.CDLL(so)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 31, 64, 240, 513, 4097])
+@pytest.mark.parametrize("vocab", [1, 7, 2048, 2049, 6001, 50001, 262144])
+def test_every_part_is_taken_once(shares, rows, vocab):
+    """Of each row and of each request; waves past the last row take none."""
+    import numpy as np
+
+    parts = shares.verify_stats(rows, vocab, None)
+    assert parts in (-(-vocab // 2048), -(-vocab // 512))
+    seen = np.zeros((rows, parts), np.int32)
+    assert shares.verify_stats(rows, vocab, ctypes.c_void_p(seen.ctypes.data)) == parts and (seen == 1).all()
+    seen[:] = 0
+    assert 1 <= shares.verify_rest(rows, parts, ctypes.c_void_p(seen.ctypes.data)) <= max(1, -(-256 // rows)) and (seen == 1).all()
