@@ -208,7 +208,7 @@ Items plan_items(const AttnArgs& a, const Shape& sh, int tiles, int fill, int le
 
 }  // namespace
 
-AttnPlan plan_attention(const AttnArgs& a) {
+AttnPlan plan_attention(const AttnArgs& a, bool scaled) {
     AttnPlan p{};
     const int group = a.q_heads / a.pages.kv_heads;
     const int64_t tokens = a.batch.tokens, requests = a.batch.requests;
@@ -221,11 +221,17 @@ AttnPlan plan_attention(const AttnArgs& a) {
     // (5e8) 33 / 39, eight of 128 rows (2e9) 60 / 48; 256 dims, window 1024, one of 128 tokens
     // (6e8) 26.8 / 27.5; 64 dims, eight of 64 rows (5e8) 22 / 27, of 128 (1.1e9) 32 / 28.
     const int from = ceil_div(a.pages.head_dim == 64 ? 96 : 64, wide.heads);
+    // Over pages of e4m3 with block scales, half the bytes for the 16-row tiles, further on (us, 16-row
+    // / 128-row): 512 dims, one of 64 tokens over 4096 keys (2e9) 41 / 52, sixteen of 8 (4.3e9) 64 / 75,
+    // twenty (5.4e9) 104 / 82; 256 dims, window 1024, one of 512 tokens (2.3e9) 28 / 41, of 1024 (4.6e9)
+    // 53 / 56, of 1400 (6.2e9) 75 / 63; 128 dims, one of 128 over 16384 (2.1e9) 35 / 39, of 200 (3.4e9)
+    // 55 / 45; 64 dims, one of 64 over 16384 (2.1e9) 38 / 39, of 128 (4.3e9) 64 / 56.
     const double work = (double)tokens * a.q_heads * (double)most_keys(a, wide.tokens) * a.pages.head_dim;
+    const double little = !scaled ? 8e8 : (a.pages.head_dim >= 256 ? 4.6e9 : 2.2e9);
     // One request: its kernel is known.  Several with a row each at least: none reaches
     // `from` rows if the sum stays under this (were some of them empty, the 16-row kernel
     // would still be right).
-    if (a.kernel == 2 || (a.kernel == 0 && work < 8e8))
+    if (a.kernel == 2 || (a.kernel == 0 && work < little))
         p.tile_from = kNoTiles;
     else if (requests == 1)
         p.tile_from = tokens >= from ? 1 : kNoTiles;

@@ -125,7 +125,7 @@ struct AttnPlan {
     }
 };
 constexpr int kThinRows = 16, kWideRows = 128;
-AttnPlan plan_attention(const AttnArgs& a);
+AttnPlan plan_attention(const AttnArgs& a, bool scaled);  // scaled: the pages have block scales
 hipError_t launch_tiles(const AttnArgs& a, const Items& it, hipStream_t stream);  // kv_tile.hip
 hipError_t launch_scaled_tiles(const AttnArgs& a, const Items& it, const BlockScales& sc, hipStream_t stream);  // kv_scaled.hip
 hipError_t launch_scaled_rows16(const AttnArgs& a, const Items& it, const BlockScales& sc, hipStream_t stream);

@@ -226,7 +226,7 @@ Gemma4Status attend(const char* name, const Gemma4KvPages* pages, const Gemma4Kv
     // a launch's workgroups are counted in 31 bits
     if (((uint64_t)batch->tokens + batch->requests + 1) * q_heads > 0x7FFFFFFFull)
         return unsupported(name, "tokens * q_heads exceeds 2^31");
-    kv::AttnPlan plan = kv::plan_attention(a);
+    kv::AttnPlan plan = kv::plan_attention(a, scaled);
     a.tile_from = plan.tile_from;
     // a launch's threads are counted in 32 bits, 512 to a workgroup at most
     for (const kv::Items* it : {&plan.tiles, &plan.rows})
