@@ -82,57 +82,113 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
     const uint32_t k_lane = (uint32_t)n * row_bytes + 16u * g;
     const uint32_t v_lane = 4u * g * row_bytes + (uint32_t)(n * C::kEpl * C::kElt);
 
-    int pages[NG];
-    uint32_t scales[NG];  // of those tiles' groups (kScaled)
-    for (int i = 0, ti = range.first + wave; ti < range.last; ++i, ti += kWaves) {
-        if ((i & 63) == 0) {
-            // the table entries of this wave's next 64 tiles, one per lane
-            const int tl = ti + lane * kWaves;
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const int at = (lo + tl * kTileKeys + j * kGroupKeys) >> a.pages.page_shift;
-                pages[j] = tl < range.last ? page_at(table, at, a.batch.width, a.pages.num_pages) : -1;
-            }
-            if constexpr (kScaled)
-#pragma unroll
-                for (int j = 0; j < NG; ++j)
-                    scales[j] = scale_bytes(scales_of(from...), pages[j], kv_head,
-                                            (uint32_t)(lo + tl * kTileKeys + j * kGroupKeys) & ((1u << a.pages.page_shift) - 1u));
-        }
-        u32x4 kf[NG][C::kChunks];
-        uint32_t vf[NG][4][C::kBlocks][C::kVWords];
+    // A tile of this wave's: its groups' first keys, whether they have pages, their scales (kScaled)
+    // and where they lie.
+    struct Groups {
         int first_key[NG];
         bool there[NG];
+        float k_by[NG], v_by[NG];
+        int64_t off[NG];
+    };
+    int pages[NG];
+    uint32_t scales[NG];
+    const auto fetch_pages = [&](int ti) {
+        // the table entries of this wave's next 64 tiles, one per lane
+        const int tl = ti + lane * kWaves;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            const int at = (lo + tl * kTileKeys + j * kGroupKeys) >> a.pages.page_shift;
+            pages[j] = tl < range.last ? page_at(table, at, a.batch.width, a.pages.num_pages) : -1;
+        }
+        if constexpr (kScaled)
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+                scales[j] = scale_bytes(scales_of(from...), pages[j], kv_head,
+                                        (uint32_t)(lo + tl * kTileKeys + j * kGroupKeys) & ((1u << a.pages.page_shift) - 1u));
+    };
+    const auto find = [&](int i, int ti, Groups& at) {
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
             const int key = lo + ti * kTileKeys + j * kGroupKeys;
             const int page = __builtin_amdgcn_readlane(pages[j], i & 63);
-            first_key[j] = key;
-            there[j] = page >= 0;
-            const int64_t off = ((int64_t)(there[j] ? page : 0) * a.pages.page_stride +
-                                 (int64_t)kv_head * a.pages.head_stride +
-                                 (int64_t)(key & ((1 << a.pages.page_shift) - 1)) * a.pages.token_stride) * C::kElt;
-            const char* kp = a.pages.k + off;
-            const char* vp = a.pages.v + off;
+            at.first_key[j] = key;
+            at.there[j] = page >= 0;
+            at.off[j] = ((int64_t)(at.there[j] ? page : 0) * a.pages.page_stride + (int64_t)kv_head * a.pages.head_stride +
+                         (int64_t)(key & ((1 << a.pages.page_shift) - 1)) * a.pages.token_stride) * C::kElt;
+        }
+    };
+    const auto find_scales = [&](int i, Groups& at) {
 #pragma unroll
-            for (int s = 0; s < C::kChunks; ++s)
-                kf[j][s] = *reinterpret_cast<const u32x4*>(kp + k_lane + 64u * s);
+        for (int j = 0; j < NG; ++j) {
+            const int both = kScaled ? __builtin_amdgcn_readlane((int)scales[j], i & 63) : 0;
+            at.k_by[j] = kScaled ? scale_value(both & 0xFF) : 1.0f;
+            at.v_by[j] = kScaled ? scale_value(both >> 8) : 1.0f;
+        }
+    };
+    u32x4 kf[NG][C::kChunks];
+    uint32_t vf[NG][4][C::kBlocks][C::kVWords];
+    const auto load_k = [&](const Groups& at, int j) {
+        const char* kp = a.pages.k + at.off[j];
+#pragma unroll
+        for (int s = 0; s < C::kChunks; ++s)
+            kf[j][s] = *reinterpret_cast<const u32x4*>(kp + k_lane + 64u * s);
+    };
+    const auto load_v = [&](const Groups& at, int j) {
+        const char* vp = a.pages.v + at.off[j];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int b = 0; b < C::kBlocks; ++b)
+#pragma unroll
+                for (int w = 0; w < C::kVWords; ++w)
+                    vf[j][k][b][w] = reinterpret_cast<const uint32_t*>(
+                        vp + v_lane + (uint32_t)k * row_bytes + (uint32_t)(b * 16 * C::kEpl * C::kElt))[w];
+    };
+    // Infinities and NaN of group j's V, where some row does not see all of it.
+    const auto clear_v = [&](int j) {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int b = 0; b < C::kBlocks; ++b)
+#pragma unroll
+                for (int w = 0; w < C::kVWords; ++w) bad |= any_nonfinite<FP8>(vf[j][k][b][w]);
+        if (__any(bad)) {
+            nonfinite = true;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int b = 0; b < C::kBlocks; ++b)
 #pragma unroll
-                    for (int w = 0; w < C::kVWords; ++w)
-                        vf[j][k][b][w] = reinterpret_cast<const uint32_t*>(
-                            vp + v_lane + (uint32_t)k * row_bytes + (uint32_t)(b * 16 * C::kEpl * C::kElt))[w];
+                    for (int w = 0; w < C::kVWords; ++w) vf[j][k][b][w] = finite_only<FP8>(vf[j][k][b][w]);
         }
+    };
 
-        float k_by[NG], v_by[NG];
+    Groups cur, nxt;
+    if (kScaled && range.first + wave < range.last) {
+        // The next tile's K loads go out when this one's have been used, its V loads likewise, so that
+        // a wave always has some on their way (32 single tokens over up to 16000 keys of 512 dims: 49.5
+        // us -> 45.8; 64 over 1024 keys of 256, where a workgroup has 8 tiles a wave, 49 either way).
+        // Two groups a tile at 512 dims: 47.8.
+        fetch_pages(range.first + wave);
+        find(0, range.first + wave, cur);
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            const int both = kScaled ? __builtin_amdgcn_readlane((int)scales[j], i & 63) : 0;
-            k_by[j] = kScaled ? scale_value(both & 0xFF) : 1.0f;
-            v_by[j] = kScaled ? scale_value(both >> 8) : 1.0f;
+        for (int j = 0; j < NG; ++j) load_k(cur, j);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) load_v(cur, j);
+        find_scales(0, cur);
+    }
+    for (int i = 0, ti = range.first + wave; ti < range.last; ++i, ti += kWaves) {
+        const bool more = ti + kWaves < range.last;
+        if constexpr (!kScaled) {
+            if ((i & 63) == 0) fetch_pages(ti);
+            find(i, ti, cur);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                load_k(cur, j);
+                load_v(cur, j);
+            }
+            find_scales(i, cur);
         }
 
         float x[NG][4];
@@ -146,42 +202,39 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
                 if (FP8) {
                     const u32x4 raw = kf[j][st / 2];
                     const uint32_t w0 = (st & 1) ? raw.z : raw.x, w1 = (st & 1) ? raw.w : raw.y;
-                    kk = u32x4{e4m3_to_bf16<false>(w0, k_by[j]), e4m3_to_bf16<true>(w0, k_by[j]), e4m3_to_bf16<false>(w1, k_by[j]),
-                               e4m3_to_bf16<true>(w1, k_by[j])};
+                    kk = u32x4{e4m3_to_bf16<false>(w0, cur.k_by[j]), e4m3_to_bf16<true>(w0, cur.k_by[j]), e4m3_to_bf16<false>(w1, cur.k_by[j]),
+                               e4m3_to_bf16<true>(w1, cur.k_by[j])};
                 } else {
                     kk = kf[j][st];
                 }
                 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), __builtin_bit_cast(bf16x8, q[st]), s, 0, 0, 0);
             }
-            const bool masked = !there[j] || !all_visible(first_key[j], kGroupKeys, t.pos0, t.n, a.window);
+            const bool masked = !cur.there[j] || !all_visible(cur.first_key[j], kGroupKeys, t.pos0, t.n, a.window);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[j][r] = s[r] * c;
             if (masked) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int key = first_key[j] + 4 * g + r;
-                    x[j][r] = there[j] && key <= pos && key > above ? x[j][r] : kNegInf;
+                    const int key = cur.first_key[j] + 4 * g + r;
+                    x[j][r] = cur.there[j] && key <= pos && key > above ? x[j][r] : kNegInf;
                 }
-                bool bad = false;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int b = 0; b < C::kBlocks; ++b)
-#pragma unroll
-                        for (int w = 0; w < C::kVWords; ++w) bad |= any_nonfinite<FP8>(vf[j][k][b][w]);
-                if (__any(bad)) {
-                    nonfinite = true;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int b = 0; b < C::kBlocks; ++b)
-#pragma unroll
-                            for (int w = 0; w < C::kVWords; ++w) vf[j][k][b][w] = finite_only<FP8>(vf[j][k][b][w]);
-                }
+                if (!kScaled) clear_v(j);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, x[j][r]);
         }
+        if (kScaled && more) {
+            if ((i & 63) == 63) fetch_pages(ti + kWaves);
+            find(i + 1, ti + kWaves, nxt);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) load_k(nxt, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (kScaled)
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+                if (!cur.there[j] || !all_visible(cur.first_key[j], kGroupKeys, t.pos0, t.n, a.window)) clear_v(j);
         top = col_max(top);
         if (__any(top > m)) {
             const float next = fmaxf(m, top);
@@ -216,7 +269,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
                             const uint32_t four = e < 2 ? __builtin_amdgcn_perm(lo23, lo01, sel) : __builtin_amdgcn_perm(hi23, hi01, sel);
-                            const u32x2 av = {e4m3_to_bf16<false>(four, v_by[j]), e4m3_to_bf16<true>(four, v_by[j])};
+                            const u32x2 av = {e4m3_to_bf16<false>(four, cur.v_by[j]), e4m3_to_bf16<true>(four, cur.v_by[j])};
                             o[b][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, av), bop, o[b][4 * w + e], 0, 0, 0);
                         }
                     } else {
@@ -228,6 +281,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 512 ? 1 : 2) void rows16_kernel(A
                         }
                     }
                 }
+        }
+        if (kScaled && more) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) load_v(nxt, j);
+            find_scales(i + 1, nxt);
+            cur = nxt;
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
