@@ -26,7 +26,8 @@ struct Reserve {
     int* positions;
     int64_t* slots;
 };
-hipError_t launch_reserve(const Pool& p, const Reserve& a, int rows, hipStream_t stream);  // kv_pool.hip
+size_t reserve_scratch(const Pool& p, int rows);  // bytes of launch_reserve's needs; 0: null
+hipError_t launch_reserve(const Pool& p, const Reserve& a, int rows, int* needs, hipStream_t stream);  // kv_pool.hip
 size_t release_scratch(const Pool& p);  // bytes of launch_release's counts; 0: null
 hipError_t launch_release(const Pool& p, const int* lens, int window, int* counts, hipStream_t stream);
 
@@ -82,9 +83,7 @@ struct HeadArgs {
 };
 
 hipError_t launch_heads(const HeadArgs& a, hipStream_t stream);
-// Workgroups of a launch, which counts its threads (256 to a workgroup) in 32 bits.
-constexpr uint32_t kMostGroups = (1u << 24) - 1;
-int64_t scaled_append_groups(const HeadArgs& a, const BlockScales& sc);
+bool scaled_append_fits(const HeadArgs& a, const BlockScales& sc);  // whether the launch can count its threads
 hipError_t launch_scaled_append(const HeadArgs& a, const BlockScales& sc, hipStream_t stream);  // kv_scaled_append.hip
 
 struct AttnArgs {

@@ -187,7 +187,7 @@ Gemma4Status append(const char* name, const Gemma4KvPages* pages, const Gemma4Kv
     a.rows = (int)batch->tokens;
     a.head_dim = (int)pages->head_dim;
     a.append = 1;
-    if (scaled && kv::scaled_append_groups(a, sc) > (int64_t)kv::kMostGroups)
+    if (scaled && !kv::scaled_append_fits(a, sc))
         return unsupported(name, "tokens * heads is too large for one launch");
     const hipError_t e = scaled ? kv::launch_scaled_append(a, sc, static_cast<hipStream_t>(stream))
                                 : kv::launch_heads(a, static_cast<hipStream_t>(stream));
@@ -344,8 +344,18 @@ Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_toke
             return bad(name, "arrays must be aligned to their type");
         if (rows >= (1u << 24)) return unsupported(name, "rows must be under 2^24");
         const kv::Reserve a{new_tokens_dev, query_starts_dev, kv_lens_dev, granted_dev, positions_dev, slots_dev};
-        const hipError_t e = kv::launch_reserve(p, a, (int)rows, static_cast<hipStream_t>(stream));
+        Scratch sc;
+        sc.stream = static_cast<hipStream_t>(stream);
+        hipError_t e = hipGetDevice(&sc.device);
+        if (e != hipSuccess) return hip_fail("gemma4_kv_reserve: hipGetDevice", e);
+        void* needs = nullptr;
+        e = sc.take(kv::reserve_scratch(p, (int)rows), &needs);
+        if (e != hipSuccess)
+            return fail(GEMMA4_ERR_MEMORY_GUARD, std::string(name) + ": workspace allocation failed: " + hipGetErrorString(e));
+        e = kv::launch_reserve(p, a, (int)rows, static_cast<int*>(needs), sc.stream);
+        const hipError_t er = sc.release();
         if (e != hipSuccess) return hip_fail("gemma4_kv_reserve: launch", e);
+        if (er != hipSuccess) return hip_fail("gemma4_kv_reserve: workspace release", er);
         return ok();
     } catch (...) {
         return fail_nothrow(GEMMA4_ERR_RUNTIME, "gemma4_kv_reserve: unexpected native exception");

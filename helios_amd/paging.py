@@ -63,6 +63,7 @@ class PagePool:
         self._c = _Pool(free_pages.data_ptr(), free_count.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), self.num_pages,
                         self.page_size, self.requests, width, stride)
         self._ref = ctypes.byref(self._c)
+        self._outs = (self.batch.query_starts.data_ptr(), self.batch.kv_lens.data_ptr(), self.granted.data_ptr())
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, requests: int, pages_per_request: int, device="cuda"):
@@ -89,8 +90,7 @@ class PagePool:
             positions = _new(self.lens, (rows,), torch.int32, stream)
             slots = _new(self.lens, (rows,), torch.int64, stream)
         _on(self._device, (new_tokens,), ())
-        status = self._lib.gemma4_kv_reserve(self._ref, new_tokens.data_ptr(), self.batch.query_starts.data_ptr(),
-                                             self.batch.kv_lens.data_ptr(), self.granted.data_ptr(), rows or 0,
+        status = self._lib.gemma4_kv_reserve(self._ref, new_tokens.data_ptr(), *self._outs, rows or 0,
                                              positions.data_ptr() if rows else None, slots.data_ptr() if rows else None,
                                              qmm._stream_ptr(stream))
         if status != 0:

@@ -489,7 +489,8 @@ typedef struct Gemma4KvPool {
  *   positions_dev    int32 [rows], slots_dev int64 [rows]; each NULL to skip: position of each of
  *                    the batch's rows in its request, and page * page_size + slot (-1 where there
  *                    is no page); rows past the last start get 0 and -1
- * lens are not changed: gemma4_kv_release sets them once it is known what is kept. */
+ * lens are not changed: gemma4_kv_release sets them once it is known what is kept.  More than
+ * 4096 rows or 1024 requests take scratch of 4 bytes a request. */
 Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_tokens_dev, int32_t* query_starts_dev, int32_t* kv_lens_dev,
                                int32_t* granted_dev, uint32_t rows, int32_t* positions_dev, int64_t* slots_dev, void* stream);
 
@@ -516,7 +517,7 @@ typedef struct Gemma4Logits {
  *   uniforms_dev     float [rows] in [0, 1)
  *   temperatures_dev float [rows] (0 or less: greedy), or NULL: `temperature` for all
  *   out_tokens_dev   int32 [rows]; -1 where no logit has a probability
- * Weights and sums are fp64.  Scratch: 16 bytes a row and chunk of 2048 to 8192 logits. */
+ * Weights and sums are fp64.  Scratch: 16 bytes a row and 2048 logits (512 of few rows). */
 Gemma4Status gemma4_sample(const Gemma4Logits* logits, uint32_t rows, uint32_t vocab, const float* uniforms_dev, float temperature,
                            const float* temperatures_dev, int32_t* out_tokens_dev, void* stream);
 

@@ -129,7 +129,9 @@ def test_append(gpu_lib, d, hk, page, block, layout):
 
 @pytest.mark.parametrize("d,pairs,distance", [(64, 32, 32), (128, 64, 1), (256, 128, 128), (256, 8, 64), (512, 64, 256), (512, 256, 1)])
 def test_append_rotates_as_the_norms_do(gpu_lib, d, pairs, distance):
-    """The q that the append writes and the q that qk_norm_rope writes are the same bits."""
+    """The q that the append writes is the q that qk_norm_rope writes, but for a product of the
+    rotation that is fused into the sum in one and rounded in the other: two fp32 values within
+    3 * 2^-24 of the head's largest, whose bf16 values are the same or neighbours (2^-7 apart)."""
     import torch
 
     from helios_amd import attention as A
@@ -145,7 +147,10 @@ def test_append_rotates_as_the_norms_do(gpu_lib, d, pairs, distance):
         pos[i] = p
     want, _ = A.qk_norm_rope(q, None, dev(pos), rope, q_norm=norm)
     live = int(b["starts"][-1])
-    assert torch.equal(got[:live], want[:live]) and bool((got[live:] == 0).all())
+    g, w = got[:live].float(), want[:live].float()
+    most = 2 * 3 * 2.0 ** -24 * w.abs().amax(-1, keepdim=True)  # a pair's norm is within sqrt(2) of its larger one
+    assert bool(((g - w).abs() <= 2.0 ** -7 * torch.maximum(g.abs(), w.abs()) + most).all())
+    assert int((g != w).sum()) <= g.numel() // 200 and bool((got[live:] == 0).all())
     inplace = q.clone()
     assert cache.append(k, k, O.device_batch(b), rope=rope, k_norm=norm, q=inplace, q_norm=norm, out_q=inplace) is inplace
     assert torch.equal(inplace, got)
