@@ -98,6 +98,13 @@ struct Exp {
     }
 };
 
+// The larger; b where a is NaN (the compiler's own form takes two operations).
+__device__ __forceinline__ double at_least(double a, double b) {
+    double v;
+    asm("v_max_f64 %0, %1, %2" : "=v"(v) : "v"(a), "s"(b));
+    return v;
+}
+
 // A distribution over a row's places: z = cap tanh(x / cap) / T, relative to that of `top`.
 struct Scale {
     double inv_heat, top_z;     // 1 / T, z of the top
@@ -134,12 +141,25 @@ __device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp
     return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
 }
 // The same as a term of a sum, where e^-700 is nothing; the top finite, or capped and not -inf.
-template <bool CAP>
+template <bool CAPPED>
 __device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) {
-    if (CAP && s.inv_cap2 > 0.0) return weight<CAP>(x, s, exp);
-    double z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
-    asm("v_max_f64 %0, %1, %2" : "=v"(z) : "v"(z), "s"(kLeast));  // NaN too; the compiler's form takes two
-    return exp(z);
+    double z;
+    if (CAPPED) {
+        // tanh(a) = 2 / (1 + e^-2a) - 1 of a = |x / cap|; the hardware's estimate is 2^-24 off, a step squares that
+        const double e = exp(at_least(__builtin_fabs((double)x) * -s.inv_cap2, kLeast)), d = 1.0 + e;
+        double y = __builtin_amdgcn_rcp(d);
+        y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+        z = __builtin_fma(__builtin_copysign(__builtin_fma(2.0, y, -1.0), (double)x), s.cap_heat, -s.top_z);
+        z = __builtin_fma((double)fminf(x, 0.0f), 1e-300, z);  // -inf where x is; else what it was
+    } else {
+        z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
+    }
+    return exp(at_least(z, kLeast));
+}
+
+template <bool CAP>
+__device__ __forceinline__ double any_term(float x, const Scale& s, const Exp& exp) {
+    return CAP && s.inv_cap2 > 0.0 ? term<true>(x, s, exp) : term<false>(x, s, exp);
 }
 
 // Eight logits from place i0 on, as they are; -inf from `end` on.
@@ -253,7 +273,7 @@ struct Held {
 };
 
 template <bool F32, bool CAP, int S>
-__global__ __launch_bounds__(kStatsThreads, CAP ? 4 : 8) void stats_kernel(Args a, Work w, Plan plan) {
+__global__ __launch_bounds__(kStatsThreads, 8) void stats_kernel(Args a, Work w, Plan plan) {
     __shared__ U2 table[kSteps];
     const int lane = (int)threadIdx.x & 63;
     const Place place = place_of(plan, __builtin_amdgcn_readfirstlane((int)blockIdx.x * (kStatsThreads / 64) + ((int)threadIdx.x >> 6)));
@@ -281,11 +301,20 @@ __global__ __launch_bounds__(kStatsThreads, CAP ? 4 : 8) void stats_kernel(Args 
     int at = kNowhere;
     if (inv_heat > 0.0) {
         const Scale scale = scale_of<CAP>(top, l.cap, inv_heat, exp);
-        if (top > -kInf && (top < kInf || (CAP && scale.inv_cap2 > 0.0))) {
+        const bool capped = CAP && scale.inv_cap2 > 0.0;
+        if (capped && top > -kInf) {
 #pragma unroll
             for (int j = 0; j < S; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += term<CAP>(x.at(j, i), scale, exp);
+                for (int i = 0; i < 8; ++i) {
+                    sum += term<true>(x.at(j, i), scale, exp);
+                    if (i == 7) __builtin_amdgcn_sched_barrier(0);  // more at once do not fit the registers
+                }
+        } else if (!capped && top > -kInf && top < kInf) {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += term<false>(x.at(j, i), scale, exp);
         } else {
 #pragma unroll
             for (int j = 0; j < S; ++j)
@@ -340,12 +369,13 @@ __device__ __forceinline__ Total join(const Part* parts, int count, double cap, 
     return t;
 }
 
-// The weight of place `at` of a row of that total; greedy: 1 at its first largest logit.
-template <bool F32, bool CAP>
-__device__ __forceinline__ double weight_at(const Logits& l, int64_t row, int at, int vocab, const Total& t, double inv_heat, const Exp& exp) {
-    if (at < 0 || at >= vocab) return 0.0;
+// The weight of place `at` (-1: none), whose logit is x, in a row of that total; greedy: 1 at its first
+// largest logit.
+template <bool CAP>
+__device__ __forceinline__ double weight_at(const Logits& l, int at, float x, const Total& t, double inv_heat, const Exp& exp) {
+    if (at < 0) return 0.0;
     if (!(inv_heat > 0.0)) return at == t.at ? 1.0 : 0.0;
-    return weight<CAP>(load1<F32>(l, row, at), scale_of<CAP>(t.top, l.cap, inv_heat, exp), exp);
+    return weight<CAP>(x, scale_of<CAP>(t.top, l.cap, inv_heat, exp), exp);
 }
 
 // The weights of a request's row to sample from.
@@ -364,8 +394,8 @@ struct Rest {
     // what of() gives, as a term of a sum; not where the top is infinite (`plain` says so)
     bool plain;
     __device__ __forceinline__ double term_of(int at, float x, float y, const Exp& exp) const {
-        const double v = term<CAP>(x, p, exp) * p_scale;
-        if (minus_q) return __builtin_fmax(v - term<CAP>(y, q, exp) * q_scale, 0.0);
+        const double v = any_term<CAP>(x, p, exp) * p_scale;
+        if (minus_q) return __builtin_fmax(v - any_term<CAP>(y, q, exp) * q_scale, 0.0);
         return at == token ? 0.0 : v;
     }
     // place `at`, whose logit is x and the drafter's y
@@ -398,7 +428,6 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
     __shared__ U2 table[kSteps];
     __shared__ Total totals[2][kWaves];  // of the rows in hand, and of the drafter's
     __shared__ int falls[kWaves];
-    __shared__ Spot spot;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = (int)blockIdx.x / groups, chunk = (int)blockIdx.x - r * groups;
     take_exp2<kWide>(table);
@@ -431,20 +460,32 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
     for (int base = 0;; base += per) {
         const int i = base + wave % per;
         const bool of_q = wave >= per;
+        // what does not wait for the joins goes out before them
+        int token = -1;
+        float u = 0.0f, x_at = 0.0f, y_at = 0.0f;
+        if (!of_q && i < n - 1) {
+            token = a.tokens[start + i + 1];
+            u = a.uniforms[2 * (start + i)];
+            if (token >= 0 && token < a.vocab) {
+                x_at = load1<F32>(a.target, start + i, token);
+                if (drafter) y_at = load1<F32>(a.draft, start + i, token);
+            } else {
+                token = -1;
+            }
+        }
         if (i < n - of_q) totals[of_q][wave % per] = of_q ? join<CAP, kHeld>(drafts + (int64_t)i * parts, parts, a.draft.cap, inv_heat, exp)
                                                   : join<CAP, kHeld>(own + (int64_t)i * parts, parts, a.target.cap, inv_heat, exp);
         __syncthreads();
         if (!of_q) {
             int fall = kNowhere;
             if (i < n - 1) {
-                const int token = a.tokens[start + i + 1];
                 const bool greedy = !(inv_heat > 0.0);
                 const Total p = totals[0][wave], q = totals[1][wave];
-                const double p_at = weight_at<F32, CAP>(a.target, start + i, token, a.vocab, p, inv_heat, exp);
-                const double q_at = drafter ? weight_at<F32, CAP>(a.draft, start + i, token, a.vocab, q, inv_heat, exp) : 1.0;
+                const double p_at = weight_at<CAP>(a.target, token, x_at, p, inv_heat, exp);
+                const double q_at = drafter ? weight_at<CAP>(a.draft, token, y_at, q, inv_heat, exp) : 1.0;
                 // u q < p, times both sums (a drafter's row without any weight has q = 0)
                 const double p_sum = greedy ? 1.0 : p.sum, q_sum = greedy || !drafter || !(q.sum > 0.0) ? 1.0 : q.sum;
-                if (!((double)a.uniforms[2 * (start + i)] * q_at * p_sum < p_at * q_sum)) fall = i;
+                if (!((double)u * q_at * p_sum < p_at * q_sum)) fall = i;
             } else if (i == n - 1) {
                 fall = i;  // the last row has no draft
             }
@@ -462,28 +503,24 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
         __syncthreads();  // the totals are read
     }
 
-    if (tid == 0) {
-        Spot s = spot_of(p_first, start + first, inv_heat, first < n - 1 ? 2 : 1);
-        if (s.kind == 2) {
-            if (drafter) {
-                s.q_top = q_first.top;
-                s.q_scale = q_first.sum > 0.0 ? 1.0 / q_first.sum : 0.0;
-            } else {
-                s.token = a.tokens[s.row + 1];
-            }
+    Spot s = spot_of(p_first, start + first, inv_heat, first < n - 1 ? 2 : 1);
+    if (s.kind == 2) {
+        if (drafter) {
+            s.q_top = q_first.top;
+            s.q_scale = q_first.sum > 0.0 ? 1.0 / q_first.sum : 0.0;
+        } else {
+            s.token = a.tokens[s.row + 1];
         }
-        spot = s;
-        if (chunk == 0) {
+    }
+    if (chunk == 0) {
+        if (tid == 0) {
             w.spots[r] = s;
             a.accepted[r] = first;
             if (s.kind == 0) a.out[s.row] = greedy_token(p_first, inv_heat);
         }
-    }
-    __syncthreads();
-    if (chunk == 0)
         for (int i = tid; i < n; i += kWide)
             if (i != first) a.out[start + i] = i < first ? a.tokens[start + i + 1] : -1;
-    const Spot s = spot;
+    }
     if (s.kind != 2) return;  // p's sums are those of its parts
 
     const Rest<CAP> rest(a, s, inv_heat, exp);
@@ -528,20 +565,23 @@ __device__ __forceinline__ double group_scan(double v, double* sums, double* tot
     *total = all;
     return v + before;
 }
-// Least and largest of the workgroup's `first` and `last`; in every thread.
-__device__ __forceinline__ void group_ends(int& first, int& last, int (*ends)[2]) {
-    first = wave_least(first);
-    last = -wave_least(-last);
-    if ((threadIdx.x & 63) == 0) {
-        ends[threadIdx.x >> 6][0] = first;
-        ends[threadIdx.x >> 6][1] = last;
-    }
+// The first of the workgroup's threads that is `hit`, the last that has `any`; -1 for none.
+struct Ends {
+    int first, last;
+};
+__device__ __forceinline__ Ends group_ends(bool hit, bool any, Ends* ends) {
+    const int wave = (int)threadIdx.x >> 6;
+    const unsigned long long hits = __ballot(hit), anys = __ballot(any);
+    if ((threadIdx.x & 63) == 0)
+        ends[wave] = Ends{hits != 0 ? 64 * wave + __ffsll(hits) - 1 : -1, anys != 0 ? 64 * wave + 63 - __clzll(anys) : -1};
     __syncthreads();
+    Ends e{-1, -1};
 #pragma unroll
     for (int i = 0; i < kWide / 64; ++i) {
-        first = ends[i][0] < first ? ends[i][0] : first;
-        last = ends[i][1] > last ? ends[i][1] : last;
+        e.first = e.first < 0 ? ends[i].first : e.first;
+        e.last = ends[i].last > e.last ? ends[i].last : e.last;
     }
+    return e;
 }
 
 // DRAFTS: spots and sums are rest_kernel's; else each row is a request and is joined here.
@@ -549,7 +589,8 @@ template <bool F32, bool CAP, bool DRAFTS>
 __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) {
     __shared__ U2 table[kSteps];
     __shared__ double sums[kWide / 64];
-    __shared__ int ends[2][kWide / 64][2];
+    __shared__ Ends ends[2][kWide / 64];
+    __shared__ int ats[kWide / 64];
     __shared__ float tops[kWide / 64];
     __shared__ double before_found;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = (int)blockIdx.x;
@@ -582,11 +623,16 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         s.p_top = top;
         s.p_scale = 1.0;  // weights need not add to one
         if (!(inv_heat > 0.0)) {
-            int at = mine.top == top ? mine.at : kNowhere, last = -1;
+            int at = mine.top == top ? mine.at : kNowhere;
             for (int i = tid + kWide; i < parts; i += kWide)
                 if (own[i].top == top) at = own[i].at < at ? own[i].at : at;
-            group_ends(at, last, ends[0]);
-            if (tid == 0) a.out[r] = at != kNowhere ? at : -1;
+            at = wave_least(at);
+            if (lane == 0) ats[wave] = at;
+            __syncthreads();
+            if (tid == 0) {
+                for (int i = 0; i < kWide / 64; ++i) at = ats[i] < at ? ats[i] : at;
+                a.out[r] = at != kNowhere ? at : -1;
+            }
             return;
         }
     }
@@ -618,18 +664,18 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
     }
     const double goal = u * total;
     double before = 0.0, v = first_weight;
-    int part = kNowhere, last = -1;
+    int part = -1, last = -1;
+    bool past = true;
     for (int base = 0;;) {
-        int found = v > 0.0 && before + upto > goal ? base + tid : kNowhere, held = v > 0.0 ? base + tid : -1;
-        const int asked = found;
-        __syncthreads();
-        group_ends(found, held, ends[0]);
-        last = held > last ? held : last;
-        if (found != kNowhere) {
-            if (asked == found) before_found = before + upto - v;
-            part = found;
+        __syncthreads();  // the round before has read the ends
+        const Ends e = group_ends(v > 0.0 && before + upto > goal, v > 0.0, ends[0]);
+        if (e.first >= 0) {
+            if (tid == e.first) before_found = before + upto - v;
+            part = base + e.first;
+            past = false;
             break;
         }
+        if (e.last >= 0) last = base + e.last;
         base += kWide;
         if (base >= parts) break;
         double here;
@@ -639,7 +685,6 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         upto = group_scan(v, sums, &here);
     }
     __syncthreads();
-    const bool past = part == kNowhere;
     if (past) part = last;
     if (part < 0) {  // no weight at all
         if (tid == 0) a.out[s.row] = -1;
@@ -659,17 +704,11 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         each[i] = of.of(i0 + i, x, y, exp);
     }
     upto = group_scan(each[0] + each[1], sums, &total) + (past ? 0.0 : before_found);
-    int found = kNowhere, held = -1;
-    if (each[1] > 0.0) {
-        held = i0 + 1;
-        if (!past && upto > goal) found = i0 + 1;
-    }
-    if (each[0] > 0.0) {
-        held = held < 0 ? i0 : held;
-        if (!past && upto - each[1] > goal) found = i0;
-    }
-    group_ends(found, held, ends[1]);
-    if (tid == 0) a.out[s.row] = found != kNowhere ? found : held;
+    const bool first_hit = !past && each[0] > 0.0 && upto - each[1] > goal;
+    const bool hit = first_hit || (!past && each[1] > 0.0 && upto > goal);
+    const Ends e = group_ends(hit, each[0] > 0.0 || each[1] > 0.0, ends[1]);
+    if (tid == e.first) a.out[s.row] = first_hit ? i0 : i0 + 1;
+    if (e.first < 0 && tid == (e.last < 0 ? 0 : e.last)) a.out[s.row] = e.last < 0 ? -1 : (each[1] > 0.0 ? i0 + 1 : i0);
 }
 
 int stats_rows(const Args& a) { return a.rows * (a.draft.x != nullptr ? 2 : 1); }
