@@ -11,7 +11,7 @@
 //     freed page i to free[count + F - 1 - i]
 //
 // So a release right after a reserve restores the free pages in their order, and nothing
-// depends on timing: there are no atomics, orders are those of prefix sums.
+// depends on timing: orders are those of prefix sums, and there are no atomics on the pool.
 //
 // A few hundred bytes for a decoding batch and a megabyte for prompts: what counts is the chain
 // of dependent loads, and the launches.  A batch of few rows is one workgroup's, a thread to a

@@ -167,6 +167,8 @@ Gemma4Status check_pool(const Gemma4KvPool* p, const char* name, kv::Pool* out) 
     return GEMMA4_OK;
 }
 
+uint64_t table_bytes(const kv::Pool& p) { return 4 * ((uint64_t)(p.requests - 1) * (uint64_t)p.stride + (uint64_t)p.width); }
+
 // scales: null, or those of the pages' blocks
 Gemma4Status append(const char* name, const Gemma4KvPages* pages, const Gemma4KvScales* scales, bool scaled, const Gemma4KvBatch* batch,
                     const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream) {
@@ -343,6 +345,12 @@ Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_toke
             !aligned(positions_dev, 4) || !aligned(slots_dev, 8))
             return bad(name, "arrays must be aligned to their type");
         if (rows >= (1u << 24)) return unsupported(name, "rows must be under 2^24");
+        const uint64_t of_requests = 4ull * p.requests;
+        if (clash({{p.free_pages, 4ull * p.num_pages, false}, {p.free_count, 4, true}, {p.lens, of_requests, false},
+                   {p.tables, table_bytes(p), true}, {new_tokens_dev, of_requests, false}, {query_starts_dev, of_requests + 4, true},
+                   {kv_lens_dev, of_requests, true}, {granted_dev, of_requests, true}, {positions_dev, 4ull * rows, true},
+                   {slots_dev, 8ull * rows, true}}))
+            return bad(name, "an array that is written must not overlap another");
         const kv::Reserve a{new_tokens_dev, query_starts_dev, kv_lens_dev, granted_dev, positions_dev, slots_dev};
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
@@ -370,6 +378,10 @@ Gemma4Status gemma4_kv_release(const Gemma4KvPool* pool, const int32_t* lens_dev
         if (st != GEMMA4_OK) return st;
         if (lens_dev == nullptr || !aligned(lens_dev, 4)) return bad(name, "requires non-null lens, 4-byte aligned");
         if (window > (1u << 30)) return unsupported(name, "window exceeds 2^30 (0: none)");
+        const uint64_t of_requests = 4ull * p.requests;
+        if (clash({{p.free_pages, 4ull * p.num_pages, true}, {p.free_count, 4, true}, {p.lens, of_requests, true},
+                   {p.tables, table_bytes(p), true}, {lens_dev == p.lens ? nullptr : lens_dev, of_requests, false}}))
+            return bad(name, "the pool's arrays must not overlap, nor lens any of them (it may be the pool's own)");
         Scratch sc;
         sc.stream = static_cast<hipStream_t>(stream);
         hipError_t e = hipGetDevice(&sc.device);

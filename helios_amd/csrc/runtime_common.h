@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -42,6 +43,22 @@ inline Gemma4Status ok() {
 inline Gemma4Status hip_fail(const char* where, hipError_t e) {
     return fail(GEMMA4_ERR_RUNTIME, std::string(where) + ": " + hipGetErrorName(e) + " (" +
                                         hipGetErrorString(e) + ")");
+}
+
+// Arrays of a call, some of them written.
+struct Span {
+    const void* at;  // may be null
+    uint64_t bytes;
+    bool written;
+};
+// Whether an array that is written shares a byte with another.
+inline bool clash(std::initializer_list<Span> spans) {
+    for (const Span* a = spans.begin(); a != spans.end(); ++a)
+        for (const Span* b = a + 1; b != spans.end(); ++b) {
+            const uintptr_t pa = reinterpret_cast<uintptr_t>(a->at), pb = reinterpret_cast<uintptr_t>(b->at);
+            if ((a->written || b->written) && pa != 0 && pb != 0 && pa < pb + b->bytes && pb < pa + a->bytes) return true;
+        }
+    return false;
 }
 
 // Per-device stream-ordered memory pool for per-call scratch (the GEMM's group sums

@@ -150,7 +150,11 @@ __device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) 
         double y = __builtin_amdgcn_rcp(d);
         y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
         z = __builtin_fma(__builtin_copysign(__builtin_fma(2.0, y, -1.0), (double)x), s.cap_heat, -s.top_z);
-        z = __builtin_fma((double)fminf(x, 0.0f), 1e-300, z);  // -inf where x is; else what it was
+        // of -inf and NaN kLeast's upper half, with any lower one
+        const U2 least = __builtin_bit_cast(U2, kLeast);
+        U2 bits = __builtin_bit_cast(U2, z);
+        bits.y = x > -kInf ? bits.y : least.y;
+        z = __builtin_bit_cast(double, bits);
     } else {
         z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
     }

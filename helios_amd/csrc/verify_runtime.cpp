@@ -43,8 +43,17 @@ Gemma4Status check_common(uint32_t rows, uint32_t vocab, const float* uniforms, 
     return GEMMA4_OK;
 }
 
+Span logits_span(const verify::Logits& l, const verify::Args& a) {
+    return Span{l.x, ((uint64_t)(a.rows - 1) * (uint64_t)l.stride + (uint64_t)a.vocab) * (l.f32 ? 4 : 2), false};
+}
+
 Gemma4Status run(const verify::Args& a, const char* name, void* stream) {
     if (!verify::fits(a)) return unsupported(name, "rows * vocab is too large for one launch");
+    const uint64_t rows = 4 * (uint64_t)a.rows, requests = 4 * (uint64_t)a.requests;
+    if (clash({logits_span(a.target, a), logits_span(a.draft, a), {a.tokens, rows, false}, {a.starts, requests + 4, false},
+               {a.uniforms, a.starts != nullptr ? 2 * rows : rows, false}, {a.heats, requests, false}, {a.out, rows, true},
+               {a.accepted, requests, true}}))
+        return bad(name, "an array that is written must not overlap another");
     Scratch sc;
     sc.stream = static_cast<hipStream_t>(stream);
     hipError_t e = hipGetDevice(&sc.device);

@@ -484,13 +484,13 @@ typedef struct Gemma4KvPool {
  *   query_starts_dev int32 [requests + 1], kv_lens_dev int32 [requests]: those of the batch
  *                    (exclusive sums of the new tokens; lens + new_tokens, also where pages were
  *                    not granted: the tokens then have absent pages, and nothing is stored for them
- *                    beyond the request's last page).  kv_lens_dev is not the pool's lens_dev
+ *                    beyond the request's last page)
  *   granted_dev      int32 [requests], 1 or 0; NULL to skip
  *   positions_dev    int32 [rows], slots_dev int64 [rows]; each NULL to skip: position of each of
  *                    the batch's rows in its request, and page * page_size + slot (-1 where there
  *                    is no page); rows past the last start get 0 and -1
- * lens are not changed: gemma4_kv_release sets them once it is known what is kept.  More than
- * 4096 rows or 1024 requests take scratch of 4 bytes a request. */
+ * lens are not changed: gemma4_kv_release sets them once it is known what is kept.  No array that is
+ * written may overlap another.  More than 4096 rows or 1024 requests take scratch of 4 bytes a request. */
 Gemma4Status gemma4_kv_reserve(const Gemma4KvPool* pool, const int32_t* new_tokens_dev, int32_t* query_starts_dev, int32_t* kv_lens_dev,
                                int32_t* granted_dev, uint32_t rows, int32_t* positions_dev, int64_t* slots_dev, void* stream);
 
@@ -537,7 +537,9 @@ Gemma4Status gemma4_sample(const Gemma4Logits* logits, uint32_t rows, uint32_t v
  *                    drawn token, then -1 (padding -1)
  *   accepted_dev     int32 [requests]: accepted drafts; accepted + 1 tokens are new (none where a
  *                    request has no rows)
- * draft_logits has the rows of logits; its last row of each request is not read for a result. */
+ * draft_logits has the rows of logits; its last row of each request is not read for a result.
+ * out_tokens and accepted overlap nothing.  Without rows nothing is written.  Scratch: that of
+ * gemma4_sample for the rows of both, 8 bytes a request and part of a row, and 48 a request. */
 Gemma4Status gemma4_verify_drafts(const Gemma4Logits* logits, const Gemma4Logits* draft_logits, const int32_t* tokens_dev,
                                   const int32_t* query_starts_dev, uint32_t requests, uint32_t rows, uint32_t vocab,
                                   const float* uniforms_dev, float temperature, const float* temperatures_dev, int32_t* out_tokens_dev,

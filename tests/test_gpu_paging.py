@@ -222,6 +222,45 @@ def test_captured_steps(gpu_lib, requests, width):
         torch.zeros(1000, device="cuda").sum().item()  # work of the program's own between replays
 
 
+@pytest.mark.parametrize("requests,width", [(5, 40), (90, 200)])
+def test_release_of_the_lens_held(gpu_lib, requests, width):
+    """pool.release(pool.lens) gives back what a reserve took, and with a window what is behind it."""
+    import torch
+
+    rng = np.random.default_rng(width)
+    host = Host(requests * width, 16, requests, width, rng)
+    pool = device(host)
+    stream = torch.cuda.Stream()
+    for window in (0, 40, 0):
+        n = rng.integers(1, 16 * width // 4, requests)
+        reserve_both(pool, host, n, 50)
+        release_both(pool, host, (host.lens + n).tolist())
+        reserve_both(pool, host, np.full(requests, 33), 50)
+        stream.wait_stream(torch.cuda.current_stream())
+        pool.release(pool.lens, window=window, stream=stream)
+        stream.synchronize()
+        host.release(host.lens.tolist(), window)
+        same(pool, host)
+
+
+def test_arrays_that_overlap(gpu_lib):
+    """A pool's own arrays as arguments: read where that is sound, else refused."""
+    import torch
+
+    from helios_amd import Gemma4Error, PagePool
+
+    pool = PagePool.allocate(9, 16, 2, 3)
+    pool.release(torch.tensor([5, 17], dtype=torch.int32, device="cuda"))
+    for bad in (pool.batch.kv_lens, pool.batch.query_starts[:2], pool.batch.query_starts[1:], pool.granted, pool.block_tables.view(-1)[2:4]):
+        with pytest.raises(Gemma4Error, match="overlap"):
+            pool.reserve(bad)
+    for bad in (pool.free_pages[3:5], pool.block_tables[1, :2]):
+        with pytest.raises(Gemma4Error, match="overlap"):
+            pool.release(bad)
+    pool.reserve(pool.lens, 4)  # as many again
+    assert pool.batch.kv_lens.tolist() == [10, 34] and pool.batch.query_starts.tolist() == [0, 5, 22]
+
+
 def test_refusals(gpu_lib):
     import torch
 

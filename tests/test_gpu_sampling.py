@@ -163,6 +163,118 @@ def test_rows_of_masks(gpu_lib):
     assert sample(t, dev(np.array([1.0, 7.0, -1.0, np.nan], np.float32))).tolist() == [4998, 4998, 0, 4998]
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(4, 5000), (260, 16385)])
+@pytest.mark.parametrize("cap,draft_cap", [(0.0, 0.0), (30.0, 30.0), (30.0, 0.0), (0.0, 20.0)])
+def test_masks_among_logits(gpu_lib, rows, vocab, kind, cap, draft_cap):
+    """NaN and -inf beside ordinary logits, of the target and of the drafter, have no part in the sums."""
+    from helios_amd import sample, verify_drafts
+
+    rng = np.random.default_rng(rows + vocab)
+    starts, heats = np.arange(0, rows + 1, 4), np.full(rows // 4, 0.8, np.float32)
+    t, x = logits(rng, rows, vocab, kinds()[kind])
+    y, tokens = drafts(rng, x, heats, starts, 0.3)
+    yt = dev(y.astype(np.float32), kinds()[kind])
+    for one in (t, yt):
+        for mask in (np.nan, -np.inf):
+            one[dev(rng.random((rows, vocab)) < 0.1)] = mask
+    x, y = (one.float().cpu().numpy().astype(np.float64) for one in (t, yt))
+    u = rng.random((rows, 2)).astype(np.float32)
+    assert sample(t, dev(u[:, 0]), 0.8, softcap=cap).tolist() == [pick(chances(x[r], np.float32(0.8), cap), u[r, 0]) for r in range(rows)]
+    got, count = verify_drafts(t, dev(tokens), dev(starts.astype(np.int32)), dev(u), dev(heats), draft_logits=yt, softcap=cap, draft_softcap=draft_cap)
+    want, accepted = verify(x, tokens, starts, u, heats, y, cap, draft_cap)
+    assert count.tolist() == accepted.tolist() and got.tolist() == want.tolist()
+
+
+def test_large_vocabularies(gpu_lib):
+    """More parts to a row than a workgroup has threads, and the largest vocabulary."""
+    from helios_amd import sample, verify_drafts
+
+    rng = np.random.default_rng(11)
+    for vocab in (1 << 21, (1 << 20) + 12345, 1 << 24):
+        x = (rng.standard_normal((3, vocab), np.float32) * 0.5).astype(np.float32)
+        x[:, -1] += 12.0
+        t, x = dev(x), x.astype(np.float64)
+        p = [chances(v, 1.0) for v in x]
+        for u in ([0.0, 0.31, 0.999], [0.5, 0.05, 0.77]):
+            u = np.array(u, np.float32)
+            assert sample(t, dev(u)).tolist() == [pick(p[r], u[r]) for r in range(3)]
+            assert sample(t, dev(u), 0.0).tolist() == x.argmax(1).tolist()
+        tokens, starts = np.array([1, vocab - 1, 5], np.int32), np.array([0, 3])
+        for u in ([[0.0, 0.3], [0.99, 0.6], [0.1, 0.2]], [[0.999, 0.4], [0.0, 0.0], [0.0, 0.0]]):
+            u = np.array(u, np.float32)
+            for y in (None, x[::-1].copy()):
+                got, count = verify_drafts(t, dev(tokens), dev(starts.astype(np.int32)), dev(u), 1.0,
+                                           draft_logits=None if y is None else t.flip(0).contiguous())
+                want, accepted = verify(x, tokens, starts, u, [1.0], y)
+                assert got.tolist() == want.tolist() and count.tolist() == accepted.tolist()
+
+
+def test_two_threads_two_streams(gpu_lib):
+    """Calls of two threads, each on a stream of its own, keep out of each other's scratch memory."""
+    import threading
+
+    import torch
+
+    from helios_amd import sample, verify_drafts
+
+    rng = np.random.default_rng(13)
+    work = []
+    for rows in (12, 64):
+        t, _ = logits(rng, rows, 60000, torch.bfloat16)
+        y, _ = logits(rng, rows, 60000, torch.bfloat16)
+        starts = dev(np.arange(0, rows + 1, 4).astype(np.int32))
+        tokens, u = dev(rng.integers(0, 60000, rows).astype(np.int32)), dev(rng.random((rows, 2)).astype(np.float32))
+        want = verify_drafts(t, tokens, starts, u, draft_logits=y) + (sample(t, u[:, 0].contiguous()),)
+        work.append((t, y, starts, tokens, u, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(t, y, starts, tokens, u, want, stream):
+        try:
+            for _ in range(50):
+                with torch.cuda.stream(stream):
+                    first = u[:, 0].contiguous()
+                got = verify_drafts(t, tokens, starts, u, draft_logits=y, stream=stream) + (sample(t, first, stream=stream),)
+                stream.synchronize()
+                assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_captured_sampling(gpu_lib):
+    """A captured call draws anew from what its inputs hold at the replay."""
+    import torch
+
+    from helios_amd import sample
+
+    rng = np.random.default_rng(17)
+    x, u, heats = torch.zeros(3, 40000, device="cuda"), torch.zeros(3, device="cuda"), torch.ones(3, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        sample(x, u, heats)  # takes the stream's scratch memory before the capture
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = sample(x, u, heats)
+    for _ in range(8):
+        x.copy_(torch.from_numpy(rng.standard_normal((3, 40000), np.float32)))
+        u.copy_(torch.from_numpy(rng.random(3, np.float32)))
+        heats.copy_(torch.from_numpy(rng.choice(np.array([0, 0.5, 1], np.float32), 3)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, sample(x, u, heats))
+        torch.rand(1000, device="cuda").sum().item()  # work of the program's own between replays
+
+
 def test_ties_and_saturated_softcap(gpu_lib):
     """Greedy: the first of equals, whatever the chunk; logits far past the softcap keep their order."""
     from helios_amd import sample

@@ -295,6 +295,41 @@ def test_prefill_tiles(gpu_lib, d, hq, hk, q_len, kv_len, window):
     attend_case(np.random.default_rng(q_len), d, hq, hk, [q_len], [kv_len], 64, 16, window=window)
 
 
+def test_pages_past_four_gigabytes(gpu_lib):
+    """The same tokens in near pages and in pages whose bytes lie past 32 bits, the same page twice in a
+    table: the same codes, scales and outputs."""
+    import torch
+
+    from helios_amd import attention as A
+
+    d, page, block, pages = 512, 64, 32, 140000
+    far = A.PagedKVCache.allocate(pages, page, 1, d, torch.float8_e4m3fn, scale_block=block)
+    near = A.PagedKVCache.allocate(8, page, 1, d, torch.float8_e4m3fn, scale_block=block)
+    assert far.k.numel() > 1 << 32
+    rng = np.random.default_rng(3)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    lens, results = [150, 300], []
+    x = randn(rng, sum(lens), 3, d) * 2
+    for cache, first in ((near, 0), (far, pages - 8)):
+        tables = np.array([[5, 1, 7, 7, 7], [0, 2, 3, 4, 6]]) + first
+        batch = A.KVBatch(ints([0, 150, 450]), ints(lens), ints(tables.tolist()))
+        cache.append(x[:, 1:2], x[:, 2:], batch)
+        outs = []
+        for starts, kv, window in (([0, 1, 2], lens, 0), ([0, 1, 2], lens, 100), ([0, 150, 450], lens, 0), ([0, 1, 2], [320, 300], 0)):
+            q = randn(np.random.default_rng(4), starts[-1], 16, d)
+            # the last: the first request reads its last page three times over
+            outs.append(cache.attend(q, A.KVBatch(ints(starts), ints(kv), ints(tables.tolist())), window=window))
+        at = slice(first, first + 8)
+        results.append(outs + [t[at].view(torch.uint8) for t in (cache.k_scale, cache.v_scale)] +
+                       [cache.k[at][tables[r, p // page] - first, 0, p % page].view(torch.uint8) for r in (0, 1) for p in (0, 63, 64, lens[r] - 1)])
+    unused = [5, 1, 0, 2, 3, 4]  # whose blocks are all written
+    for i, (a, b) in enumerate(zip(*results)):
+        a, b = (t[unused] if t.shape[:2] == (8, 1) and t.dtype == torch.uint8 else t for t in (a, b))
+        if i == 3:  # slots past the 150 tokens are whatever the pages held
+            a, b = a[1], b[1]
+        assert torch.equal(a, b), i
+
+
 def test_many_requests_and_absent_pages(gpu_lib):
     import torch
 

@@ -187,6 +187,19 @@ def test_release_is_checked(lib, kw, status, text):
     assert lib.gemma4_kv_release(None, P, 0, None) == BAD
 
 
+@pytest.mark.parametrize("kw", [dict(new=P + 4096), dict(new=P + 4096 + 8), dict(granted=P + 8192), dict(granted=P + 128), dict(positions=P + 4),
+                                dict(slots=P + 256 + 24), dict(starts=P + 64), dict(positions=P + 32768 - 12)])
+def test_reserve_writes_over_nothing(lib, kw):
+    apart = dict(new=P + 12288, starts=P + 4096, kv_lens=P + 8192, granted=P + 16384, positions=P + 24576, slots=P + 32768)
+    assert reserve(lib, **{**apart, **kw}) == BAD and "overlap" in qmm.last_error()
+
+
+def test_release_reads_its_own_lens_only(lib):
+    for lens in (P + 132, P + 124, P, P + 64, P + 256 + 28):
+        assert release(lib, lens=lens) == BAD and "overlap" in qmm.last_error()
+    assert release(lib, p=pool(free_count_dev=P + 36), lens=P + 4096) == BAD and "overlap" in qmm.last_error()
+
+
 # ------------------------------------------------------------------ sampling
 
 def logits(**kw):
@@ -250,6 +263,16 @@ def test_sampling_is_checked(lib, kw, status, text):
 def test_verification_is_checked(lib, kw, status, text):
     assert verify(lib, **kw) == status and text in qmm.last_error()
     assert lib.gemma4_verify_drafts(None, None, P, P, 1, 1, 10, P, 1.0, None, P, P, None) == BAD
+
+
+def test_tokens_are_written_over_nothing(lib):
+    apart = dict(u=P + (1 << 20), heats=P + (2 << 20), out=P + (3 << 20))
+    for kw in (dict(out=P + 3996), dict(out=P + (1 << 20) + 4), dict(out=P + (2 << 20) - 4)):
+        assert sample(lib, **{**apart, **kw}) == BAD and "overlap" in qmm.last_error()
+    apart.update(tokens=P + (4 << 20), starts=P + (5 << 20), accepted=P + (6 << 20), draft=logits(x_dev=P + (7 << 20)))
+    for kw in (dict(out=P + (4 << 20)), dict(out=P + (5 << 20) + 8), dict(accepted=P + (3 << 20) + 12), dict(accepted=P + (1 << 20) + 28),
+               dict(out=P + (7 << 20) + 7996), dict(accepted=P + (4 << 20) - 4)):
+        assert verify(lib, **{**apart, **kw}) == BAD and "overlap" in qmm.last_error()
 
 
 # ------------------------------------------------------------------ layout, Python's own checks
