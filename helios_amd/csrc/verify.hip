@@ -98,6 +98,12 @@ struct Exp {
     }
 };
 
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // The larger; b where a is NaN (the compiler's own form takes two operations).
 __device__ __forceinline__ double at_least(double a, double b) {
     double v;
@@ -161,6 +167,35 @@ __device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) 
     return exp(at_least(z, kLeast));
 }
 
+// Sums of uncapped terms with two operations less than term's, the same shape of e^z in x's own
+// units: x = (N + r) T ln2 / 256, N's share of the top taken off in t, r's at the end.
+struct Sum {
+    const U2* table;
+    double a, b, step, c1, c2, c3, least, sum;
+    // |top / T| under 2^40, so that N has room
+    __device__ __forceinline__ Sum(const Exp& exp, float top, double inv_heat, double heat)
+        : table(exp.table), a(inv_heat * exp.per_step), step(heat * exp.step), c1(inv_heat), c2(0.5 * inv_heat * inv_heat),
+          c3(inv_heat * inv_heat * inv_heat * exp.sixth), least(__builtin_fma(heat, kLeast, (double)top)), sum(0.0) {
+        b = exp.magic - (__builtin_fma((double)top, a, exp.magic) - exp.magic);
+        // the wave's own: to scalar registers, of which an operation takes one
+        a = lane_of(a, 0), step = lane_of(step, 0), c1 = lane_of(c1, 0), c3 = lane_of(c3, 0), least = lane_of(least, 0);
+    }
+    __device__ __forceinline__ double series(double r) const {
+        return __builtin_fma(__builtin_fma(__builtin_fma(r, c3, c2), r, c1), r, 1.0);
+    }
+    __device__ __forceinline__ void add(float logit) {
+        const double x = at_least((double)logit, least), t = __builtin_fma(x, a, b);
+        const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+        U2 two = table[n & (kSteps - 1)];
+        two.y += n << 12;
+        sum = __builtin_fma(__builtin_bit_cast(double, two), series(__builtin_fma(t - b, step, x)), sum);
+    }
+    __device__ __forceinline__ double relative_to(float top, const Exp& exp) const {
+        return sum * series(-__builtin_fma(exp.magic - b, step, (double)top));
+    }
+};
+constexpr double kRoomy = 0x1p40;
+
 template <bool CAP>
 __device__ __forceinline__ double any_term(float x, const Scale& s, const Exp& exp) {
     return CAP && s.inv_cap2 > 0.0 ? term<true>(x, s, exp) : term<false>(x, s, exp);
@@ -201,11 +236,6 @@ __device__ __forceinline__ double dpp_of(double v) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, DPP, ROWS, 0xf, ROWS == 0xf);
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), DPP, ROWS, 0xf, ROWS == 0xf);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double lane_of(double v, int lane) {
-    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // Inclusive sums over the lanes (row shifts of 1, 2, 4, 8, then the rows' last lanes to the rows after
@@ -253,11 +283,13 @@ __device__ __forceinline__ int request_of(const Args& a, int row) {
     return row < a.starts[0] ? a.requests : request;
 }
 __device__ __forceinline__ int start_of(const Args& a, int r) { return a.starts == nullptr ? r : clampi(a.starts[r], 0, a.rows); }
-// 0 where the request is greedy
-__device__ __forceinline__ double inv_heat_of(const Args& a, int r) {
+// The request's temperature; 0 where it is greedy, and past 1e30 all finite logits are equal.
+__device__ __forceinline__ double heat_of(const Args& a, int r) {
     const float t = a.heats != nullptr ? a.heats[r] : a.heat;
-    return t > 0.0f ? 1.0 / (double)fminf(t, 1e30f) : 0.0;  // past that all finite logits are equal
+    return t > 0.0f ? (double)fminf(t, 1e30f) : 0.0;
 }
+__device__ __forceinline__ double inv_of(double heat) { return heat > 0.0 ? 1.0 / heat : 0.0; }
+__device__ __forceinline__ double inv_heat_of(const Args& a, int r) { return inv_of(heat_of(a, r)); }
 
 constexpr int kNowhere = 0x7fffffff;
 
@@ -277,7 +309,7 @@ struct Held {
 };
 
 template <bool F32, bool CAP, int S>
-__global__ __launch_bounds__(kStatsThreads, 8) void stats_kernel(Args a, Work w, Plan plan) {
+__global__ __launch_bounds__(kStatsThreads, F32 && S > 1 ? 5 : 8) void stats_kernel(Args a, Work w, Plan plan) {
     __shared__ U2 table[kSteps];
     const int lane = (int)threadIdx.x & 63;
     const Place place = place_of(plan, __builtin_amdgcn_readfirstlane((int)blockIdx.x * (kStatsThreads / 64) + ((int)threadIdx.x >> 6)));
@@ -294,7 +326,7 @@ __global__ __launch_bounds__(kStatsThreads, 8) void stats_kernel(Args a, Work w,
     const int r = request_of(a, row);
     if (r >= a.requests) return;                                // padding
     if (of_draft && row + 1 >= start_of(a, r + 1)) return;      // no draft was drawn from it
-    const double inv_heat = inv_heat_of(a, r);
+    const double heat = heat_of(a, r), inv_heat = inv_of(heat);
     float top = -kInf;
 #pragma unroll
     for (int j = 0; j < S; ++j)
@@ -312,18 +344,21 @@ __global__ __launch_bounds__(kStatsThreads, 8) void stats_kernel(Args a, Work w,
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     sum += term<true>(x.at(j, i), scale, exp);
+                    if (i == 7) __builtin_amdgcn_sched_barrier(0);
+                }
+        } else if (!capped && __builtin_fabs((double)top * inv_heat) < kRoomy) {
+            Sum of(exp, top, inv_heat, heat);
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    of.add(x.at(j, i));
                     if (i == 7) __builtin_amdgcn_sched_barrier(0);  // more at once do not fit the registers
                 }
-        } else if (!capped && top > -kInf && top < kInf) {
-#pragma unroll
-            for (int j = 0; j < S; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += term<false>(x.at(j, i), scale, exp);
-        } else {
-#pragma unroll
-            for (int j = 0; j < S; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += x.at(j, i) == kInf;  // infinities share all there is; -inf has none
+            sum = of.relative_to(top, exp);
+        } else {  // nothing, infinities (which share all there is), or larger than Sum has room for
+            const int end = begin + 512 * S < a.vocab ? begin + 512 * S : a.vocab;
+            for (int i = begin + lane; i < end; i += 64) sum += weight<CAP>(load1<F32>(l, row, i), scale, exp);
         }
         sum = wave_sum(sum);
     } else if (top > -kInf) {

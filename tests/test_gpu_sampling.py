@@ -186,6 +186,25 @@ def test_masks_among_logits(gpu_lib, rows, vocab, kind, cap, draft_cap):
     assert count.tolist() == accepted.tolist() and got.tolist() == want.tolist()
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, 6000), (200, 30000)])
+def test_far_temperatures_and_logits(gpu_lib, rows, vocab):
+    """Quotients of 2^40 and more, temperatures near both ends of float32: ties alone, or all alike."""
+    import torch
+
+    from helios_amd import sample
+
+    places = [5, vocab // 2, vocab - 2]
+    for kind in kinds().values():
+        x = torch.zeros(rows, vocab, device="cuda", dtype=kind)
+        x[:, places] = 2.0 ** 41
+        for u, want in ((0.0, 0), (0.3, 0), (0.5, 1), (0.7, 2), (0.99, 2)):
+            uu = torch.full((rows,), u, device="cuda")
+            for t, heat in ((x, 1.0), (x, 4.0), (x, 1e-3), (x / 2 ** 41, 1e-42), (x / 2 ** 41, 1e-38), (x * 2.0 ** 80, 1e30)):
+                assert sample(t, uu, heat).tolist() == [places[want]] * rows, (u, heat)
+            # all weights are 1 to the last bit: the first place whose number of weights exceeds u n
+            assert sample(x / 2 ** 41, uu, 3e38).tolist() == [int(np.float64(np.float32(u)) * vocab)] * rows
+
+
 def test_large_vocabularies(gpu_lib):
     """More parts to a row than a workgroup has threads, and the largest vocabulary."""
     from helios_amd import sample, verify_drafts
