@@ -549,6 +549,7 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
             s.q_scale = q_first.sum > 0.0 ? 1.0 / q_first.sum : 0.0;
         } else {
             s.token = a.tokens[s.row + 1];
+            if (s.token < 0 || s.token >= a.vocab) s = Spot{s.p_scale, 0.0, s.p_top, 0.0f, s.row, -1, 1, 0};  // nothing to take off p
         }
     }
     if (chunk == 0) {
@@ -563,7 +564,11 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
     if (s.kind != 2) return;  // p's sums are those of its parts
 
     const Rest<CAP> rest(a, s, inv_heat, exp);
-    for (int part = first_part(chunk, wave); part < parts; part += part_step(groups)) {
+    // Without a drafter's logits only the part that has the token is other than p's (its sum without it is
+    // taken anew: a difference would lose what is left).
+    const int only = s.token / (512 * S);
+    for (int part = drafter ? first_part(chunk, wave) : (chunk == 0 && wave == 0 ? only : parts); part < parts;
+         part += drafter ? part_step(groups) : parts) {
         const int begin = part * 512 * S;
         double sum = 0.0;
         if (rest.plain) {
@@ -641,7 +646,9 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
     const Part none{0.0, -kInf, kNowhere};
     const Part mine = tid < parts ? own[tid] : none;
     const double* const rest = w.rest + (int64_t)r * parts;
-    const double my_rest = DRAFTS && s.kind == 2 && tid < parts ? rest[tid] : 0.0;
+    const int size = plan.size(), only = DRAFTS && s.kind == 2 && a.draft.x == nullptr ? s.token / size : -1;
+    const bool all_rest = DRAFTS && s.kind == 2 && a.draft.x != nullptr;
+    const double my_rest = (all_rest && tid < parts) || tid == only ? rest[tid] : 0.0;
     const double u = (double)(DRAFTS ? a.uniforms[2 * s.row + 1] : a.uniforms[s.row]);
     const double inv_heat = inv_heat_of(a, r);
     take_exp2<kWide>(table);
@@ -681,7 +688,7 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
     const Scale scale = scale_of<CAP>(s.p_top, a.target.cap, inv_heat, exp);
     const auto part_weight = [&](int i) {
         if (i >= parts) return 0.0;
-        if (DRAFTS && s.kind == 2) return i == tid ? my_rest : rest[i];
+        if (DRAFTS && s.kind == 2 && (all_rest || i == only)) return i == tid ? my_rest : rest[i];
         const Part p = i == tid ? mine : own[i];
         return p.sum * weight<CAP>(p.top, scale, exp) * s.p_scale;
     };
@@ -771,7 +778,7 @@ hipError_t launch_of(const Args& a, const Work& w, const Plan& p, hipStream_t st
         pick_kernel<F32, CAP, false><<<(unsigned)a.requests, kWide, 0, stream>>>(a, w, p);
         return hipGetLastError();
     }
-    const int groups = rest_groups(a.requests, p.parts);
+    const int groups = a.draft.x != nullptr ? rest_groups(a.requests, p.parts) : 1;
     rest_kernel<F32, CAP, S><<<(unsigned)a.requests * (unsigned)groups, kWide, 0, stream>>>(a, w, p.parts, groups);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
