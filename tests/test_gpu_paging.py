@@ -3,6 +3,8 @@
 import numpy as np
 import pytest
 
+from pooled_streams import streams  # noqa: F401
+
 pytestmark = pytest.mark.gpu
 
 
@@ -188,7 +190,7 @@ def test_lengths_and_counts_past_their_ends(gpu_lib):
 
 
 @pytest.mark.parametrize("requests,width", [(6, 40), (90, 200)])
-def test_captured_steps(gpu_lib, requests, width):
+def test_captured_steps(gpu_lib, requests, width, streams):
     """Replays of a captured reserve and release follow what the device arrays hold."""
     import torch
 
@@ -197,7 +199,7 @@ def test_captured_steps(gpu_lib, requests, width):
     pool = device(host)
     new, kept = (torch.zeros(requests, dtype=torch.int32, device="cuda") for _ in range(2))
     rows = 6000
-    stream = torch.cuda.Stream()
+    stream = streams()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         pool.reserve(new, rows)
@@ -223,14 +225,14 @@ def test_captured_steps(gpu_lib, requests, width):
 
 
 @pytest.mark.parametrize("requests,width", [(5, 40), (90, 200)])
-def test_release_of_the_lens_held(gpu_lib, requests, width):
+def test_release_of_the_lens_held(gpu_lib, requests, width, streams):
     """pool.release(pool.lens) gives back what a reserve took, and with a window what is behind it."""
     import torch
 
     rng = np.random.default_rng(width)
     host = Host(requests * width, 16, requests, width, rng)
     pool = device(host)
-    stream = torch.cuda.Stream()
+    stream = streams()
     for window in (0, 40, 0):
         n = rng.integers(1, 16 * width // 4, requests)
         reserve_both(pool, host, n, 50)

@@ -6,6 +6,8 @@ with a probability of some vocab * 1e-15 a draw."""
 import numpy as np
 import pytest
 
+from pooled_streams import streams  # noqa: F401
+
 pytestmark = pytest.mark.gpu
 
 
@@ -229,7 +231,7 @@ def test_large_vocabularies(gpu_lib):
                 assert got.tolist() == want.tolist() and count.tolist() == accepted.tolist()
 
 
-def test_two_threads_two_streams(gpu_lib):
+def test_two_threads_two_streams(gpu_lib, streams):
     """Calls of two threads, each on a stream of its own, keep out of each other's scratch memory."""
     import threading
 
@@ -245,7 +247,7 @@ def test_two_threads_two_streams(gpu_lib):
         starts = dev(np.arange(0, rows + 1, 4).astype(np.int32))
         tokens, u = dev(rng.integers(0, 60000, rows).astype(np.int32)), dev(rng.random((rows, 2)).astype(np.float32))
         want = verify_drafts(t, tokens, starts, u, draft_logits=y) + (sample(t, u[:, 0].contiguous()),)
-        work.append((t, y, starts, tokens, u, want, torch.cuda.Stream()))
+        work.append((t, y, starts, tokens, u, want, streams()))
     torch.cuda.synchronize()
     failed = []
 
@@ -268,7 +270,7 @@ def test_two_threads_two_streams(gpu_lib):
     assert not failed, failed
 
 
-def test_captured_sampling(gpu_lib):
+def test_captured_sampling(gpu_lib, streams):
     """A captured call draws anew from what its inputs hold at the replay."""
     import torch
 
@@ -276,7 +278,7 @@ def test_captured_sampling(gpu_lib):
 
     rng = np.random.default_rng(17)
     x, u, heats = torch.zeros(3, 40000, device="cuda"), torch.zeros(3, device="cuda"), torch.ones(3, device="cuda")
-    stream = torch.cuda.Stream()
+    stream = streams()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         sample(x, u, heats)  # takes the stream's scratch memory before the capture

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import attention_oracle as O
+from pooled_streams import streams  # noqa: F401
 from test_gpu_paging import Host
 from test_gpu_sampling import verify as verify_host
 
@@ -78,11 +79,11 @@ class Server:
                 "k_scale": c.k_scale.view(torch.uint8), "v_scale": c.v_scale.view(torch.uint8)}
 
 
-def test_captured_steps_replay_as_eager_ones(gpu_lib):
+def test_captured_steps_replay_as_eager_ones(gpu_lib, streams):
     import torch
 
     eager, captured = Server(1), Server(1)
-    stream = torch.cuda.Stream()
+    stream = streams()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         captured.step()  # takes the stream's scratch memory before the capture; no tokens are new
