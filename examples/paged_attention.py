@@ -6,7 +6,7 @@ Prompts of several requests go in together, a chunk at a time; then every reques
 one token a step, the whole block captured in a graph whose replays follow the batch's
 device arrays.
 
-    python examples/paged_attention.py [--layer sliding|full] [--requests 8] [--prompt 2000]
+    python examples/paged_attention.py [--layer sliding|full] [--requests 8] [--prompt 2000] [--e4m3 [--block 64]]
 
 Weights are random, in the shapes of the decoder that bench.py runs.
 """
@@ -73,6 +73,7 @@ def main():
     p.add_argument("--steps", type=int, default=64, help="tokens decoded per request")
     p.add_argument("--page", type=int, default=64)
     p.add_argument("--e4m3", action="store_true", help="keep the cache in 8-bit floats")
+    p.add_argument("--block", type=int, default=0, help="with --e4m3: a scale for each so many tokens, found from the values")
     a = p.parse_args()
     g = torch.Generator(device="cuda").manual_seed(1)
     q_heads, kv_heads, head_dim, window, base, pairs = LAYERS[a.layer]
@@ -81,8 +82,8 @@ def main():
     prompts = [max(1, a.prompt * (a.requests - i) // a.requests) for i in range(a.requests)]
     width = -(-(a.prompt + a.steps) // a.page)
     tables = torch.randperm(a.requests * width, device="cuda", generator=g).to(torch.int32).view(a.requests, width)
-    kind, scale = (torch.float8_e4m3fn, 1 / 16) if a.e4m3 else (torch.bfloat16, 1.0)
-    cache = PagedKVCache.allocate(a.requests * width, a.page, kv_heads, head_dim, kind, scale, scale)
+    kind, scale = (torch.float8_e4m3fn, 1.0 if a.block else 1 / 16) if a.e4m3 else (torch.bfloat16, 1.0)
+    cache = PagedKVCache.allocate(a.requests * width, a.page, kv_heads, head_dim, kind, scale, scale, scale_block=a.block)
 
     def timed(what, tokens, call):
         begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)

@@ -1,6 +1,5 @@
 // Launch interface of the paged-cache kernels (kv_heads.hip, kv_scaled_append.hip, kv_attention.hip,
-// kv_tile.hip, kv_scaled.hip);
-// arguments are checked by kv_runtime.cpp.
+// kv_tile.hip, kv_scaled.hip, kv_pool.hip); arguments are checked by kv_runtime.cpp.
 #pragma once
 
 #include <hip/hip_runtime.h>

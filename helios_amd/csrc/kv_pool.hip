@@ -17,9 +17,9 @@
 // of dependent loads, and the launches.  A batch of few rows is one workgroup's, a thread to a
 // request (what a decoding step needs) and a wave to each that needs many pages; larger ones take
 // two launches: what each request needs, then a workgroup to a request.  release likewise.
-// us: a token for each of 8 requests, reserve 3.5 and release 3.1 (6.2 and 7.4 with scans through LDS and
-// entries one after another); 96 requests of 200 tokens in pages of 16 and tables of 2048, 2.9 + 3.7 and
-// 3.0 + 4.3.
+// us: a token for each of 8 requests, reserve 3.1 and release 3.0 (6.2 and 7.4 with scans through LDS and
+// entries one after another); 96 requests' mixed prompts in tables of 2048, 84000 rows, 2.6 + 3.7 + 4.1 (the
+// map) and 2.8 + 4.5.
 #include "kv_device.h"
 
 namespace kv {

@@ -15,8 +15,8 @@
 // Every (block, KV head) of k and of v is a workgroup's, so the maximum needs no other; the
 // block's codes are rewritten only where its scale rises.  q's rows have workgroups of their own
 // in the same launch.  Bound by the chain of loads for few tokens (32 of one token, 16 query and 8
-// KV heads of 256: 6.5 us) and by memory and the angles for many: five prompts of up to 777 tokens, 16
-// and one of 512, 39 MB, 14.6 us, 2.7 TB/s, where a large copy moves 4.9 (26.6 with 256 threads, two
+// KV heads of 256: 6.4 us) and by memory and the angles for many: five prompts of up to 777 tokens, 16
+// and one of 512, 39 MB, 14.2 us, 2.7 TB/s, where a large copy moves 4.9 (26.6 with 256 threads, two
 // passes over a block's tokens and a row of q to four workgroups).
 #include "kv_heads_device.h"
 

@@ -28,11 +28,6 @@ struct Args {
     int* accepted;           // [requests]; may be null
 };
 
-// How a row is cut: `count` chunks of `size` places.
-struct Chunks {
-    int size, count;
-};
-
 bool fits(const Args& a);  // whether the launches can count their threads
 size_t scratch_bytes(const Args& a);
 hipError_t launch(const Args& a, void* scratch, hipStream_t stream);
