@@ -92,7 +92,7 @@ class PagePool:
         _on(self._device, (new_tokens,), ())
         status = self._lib.gemma4_kv_reserve(self._ref, new_tokens.data_ptr(), *self._outs, rows or 0,
                                              positions.data_ptr() if rows else None, slots.data_ptr() if rows else None,
-                                             qmm._stream_ptr(stream))
+                                             qmm._stream_ptr(stream, self._device))
         if status != 0:
             qmm.check(status, self._lib)
         return positions, slots
@@ -106,7 +106,7 @@ class PagePool:
         if window > 1 << 30:  # the library's limit, checked here: a larger one does not reach it whole
             raise Gemma4Error(Status.UNSUPPORTED_CONFIG, "window exceeds 2^30 (0: none)")
         _on(self._device, (lens,), ())
-        status = self._lib.gemma4_kv_release(self._ref, lens.data_ptr(), window, qmm._stream_ptr(stream))
+        status = self._lib.gemma4_kv_release(self._ref, lens.data_ptr(), window, qmm._stream_ptr(stream, self._device))
         if status != 0:
             qmm.check(status, self._lib)
 

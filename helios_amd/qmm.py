@@ -233,14 +233,14 @@ def gemm_min_rows(rows: int):
         set_gemm_min_rows(prev)
 
 
-def _stream_ptr(stream) -> int:
-    """The raw stream (default: torch's current one on the current device).  Read without
-    building a torch Stream object, which costs about as much as a launch; plain integers
+def _stream_ptr(stream, device: int | None = None) -> int:
+    """The raw stream (default: torch's current one on the current device, which is `device`
+    where that is known already).  Read without building a torch Stream object, which costs about as much as a launch; plain integers
     here and in _dev_ptr: ctypes converts them to the declared void pointers itself."""
     import torch
 
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
     return stream.cuda_stream
 
 

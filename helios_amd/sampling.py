@@ -28,8 +28,8 @@ class _Logits(ctypes.Structure):
 def _logits(t, what: str, softcap):
     import torch
 
-    kinds = {torch.bfloat16: 0, torch.float32: 1}
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_cuda or t.dtype not in kinds:
+    kind = {torch.bfloat16: 0, torch.float32: 1}.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if kind is None or t.dim() != 2 or not t.is_cuda:
         raise _invalid(f"{what} must be a bfloat16 or float32 tensor [rows, vocab] on the GPU")
     rows, vocab = t.shape
     if vocab > 1 and t.stride(1) != 1:
@@ -38,7 +38,7 @@ def _logits(t, what: str, softcap):
     if not 0.0 <= softcap < math.inf:
         raise _invalid(f"{what}' softcap must be finite and >= 0 (0: none)")
     # a single row's stride says nothing
-    return _Logits(t.data_ptr(), t.stride(0) if rows > 1 else vocab, kinds[t.dtype], softcap)
+    return _Logits(t.data_ptr(), t.stride(0) if rows > 1 else vocab, kind, softcap)
 
 
 def _floats(t, what: str, shape):
@@ -78,9 +78,10 @@ def sample(logits, uniforms, temperature=1.0, softcap: float = 0.0, stream=None)
     rows, vocab = logits.shape
     _floats(uniforms, "uniforms", (rows,))
     heat, heats = _temperature(temperature, rows)
-    _on(logits.get_device(), (uniforms, heats), ())
+    device = logits.get_device()
+    _on(device, (uniforms, heats), ())
     out = _new(logits, (rows,), torch.int32, stream)
-    status = lib.gemma4_sample(ctypes.byref(of), rows, vocab, uniforms.data_ptr(), heat, _ptr(heats), out.data_ptr(), qmm._stream_ptr(stream))
+    status = lib.gemma4_sample(ctypes.byref(of), rows, vocab, uniforms.data_ptr(), heat, _ptr(heats), out.data_ptr(), qmm._stream_ptr(stream, device))
     if status != 0:
         qmm.check(status, lib)
     return out
@@ -117,7 +118,8 @@ def verify_drafts(logits, tokens, query_starts, uniforms, temperature=1.0, draft
         raise _invalid("query_starts must have an entry more than there are requests, one at least")
     _floats(uniforms, "uniforms", (rows, 2))
     heat, heats = _temperature(temperature, requests)
-    _on(logits.get_device(), (draft_logits, tokens, query_starts, uniforms, heats), ())
+    device = logits.get_device()
+    _on(device, (draft_logits, tokens, query_starts, uniforms, heats), ())
     out = _new(logits, (rows,), torch.int32, stream)
     accepted = _new(logits, (requests,), torch.int32, stream)
     if rows == 0:
@@ -125,7 +127,7 @@ def verify_drafts(logits, tokens, query_starts, uniforms, temperature=1.0, draft
             return out, accepted.zero_()
     status = lib.gemma4_verify_drafts(ctypes.byref(of), None if draft is None else ctypes.byref(draft), tokens.data_ptr(),
                                       query_starts.data_ptr(), requests, rows, vocab, uniforms.data_ptr(), heat, _ptr(heats),
-                                      out.data_ptr(), accepted.data_ptr(), qmm._stream_ptr(stream))
+                                      out.data_ptr(), accepted.data_ptr(), qmm._stream_ptr(stream, device))
     if status != 0:
         qmm.check(status, lib)
     return out, accepted
