@@ -8,7 +8,7 @@
 //
 // 64 single tokens over 1024 keys, 8 KV heads of 256, 230 MB: 49 us, 4.7 TB/s; 32 over up to 16000
 // keys, one of 512, 201 MB: 46 us and a join of 7; 2048 tokens over 16384 keys, 16 heads of 512 over
-// one: 951-980 us, 1.05-1.08 PFLOP/s.  By one scale for all pages the same calls take 54.5, 45 + 7 and
+// one: 951-983 us, 1.05-1.08 PFLOP/s.  By one scale for all pages the same calls take 54.5, 45 + 7 and
 // (bf16) 959-1047.
 #include "kv_rows16.h"
 #include "kv_tile_kernel.h"

@@ -137,3 +137,16 @@ def test_steps_do_what_they_say(gpu_lib):
         assert server.pool.lens.tolist() == host.lens.tolist() and server.pool.free_pages[:len(host.free)].tolist() == host.free
         assert np.array_equal(server.pool.block_tables.cpu().numpy(), host.tables)
     assert int(host.lens.max()) > WINDOW  # pages went back behind the window
+
+
+@pytest.mark.parametrize("args", [["--block", "16"], ["--layer", "full", "--block", "64"]])
+def test_the_example_runs_over_block_scales(gpu_lib, args):
+    import os
+    import subprocess
+    import sys
+
+    example = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_attention.py")
+    run = subprocess.run([sys.executable, example, "--e4m3", "--requests", "3", "--prompt", "150", "--chunk", "64", "--steps", "5", *args],
+                         capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0, run.stderr
+    assert "prompts: 300 tokens" in run.stdout and "decoding: 12 tokens" in run.stdout
