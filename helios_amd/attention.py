@@ -365,7 +365,7 @@ class PagedKVCache:
             out_q = None
         _on(self._device, (k, v, q, out_q), (batch, rope, k_norm, v_norm, q_norm))
         args = (batch._struct(rows), of_q, _heads(k, shape, k_stride, k_norm, 0, 0), _heads(v, v_shape, v_stride, v_norm, 0, 0),
-                None if rope is None else rope._ref, qmm._stream_ptr(stream, self._device))
+                None if rope is None else rope._ref, qmm._stream_ptr(stream))
         if self._scales is None:
             status = self._lib.gemma4_kv_append(self._ref, *args)
         else:
@@ -392,7 +392,7 @@ class PagedKVCache:
         lse = _new(q, (rows, heads), torch.float32, stream) if return_lse else None
         _on(self._device, (q, out), (batch,))
         args = (batch._struct(rows), q.data_ptr(), q_stride, heads, self.head_dim ** -0.5 if scale is None else scale, window,
-                out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(), qmm._stream_ptr(stream, self._device))
+                out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(), qmm._stream_ptr(stream))
         if self._scales is None:
             status = self._lib.gemma4_kv_attention(self._ref, *args)
         else:
