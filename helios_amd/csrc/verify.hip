@@ -754,8 +754,10 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         const float y = live && of.minus_q ? load1<F32>(a.draft, s.row, i0 + i) : -kInf;
         each[i] = of.of(i0 + i, x, y, exp);
     }
-    upto = group_scan(each[0] + each[1], sums, &total) + (past ? 0.0 : before_found);
-    const bool first_hit = !past && each[0] > 0.0 && upto - each[1] > goal;
+    const double both = each[0] + each[1], scan = group_scan(both, sums, &total), found = past ? 0.0 : before_found;
+    upto = scan + found;
+    // of the places before this thread's (0 where none of them has any: then the least weight counts) and its first
+    const bool first_hit = !past && each[0] > 0.0 && (scan - both) + found + each[0] > goal;
     const bool hit = first_hit || (!past && each[1] > 0.0 && upto > goal);
     const Ends e = group_ends(hit, each[0] > 0.0 || each[1] > 0.0, ends[1]);
     if (tid == e.first) a.out[s.row] = first_hit ? i0 : i0 + 1;
