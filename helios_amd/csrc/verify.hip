@@ -25,6 +25,9 @@
 #include "verify_index.h"
 #include "verify_kernels.h"
 
+// rest_kernel and pick_kernel weigh the same places and have to agree on them to the last bit
+#pragma clang fp contract(off)
+
 namespace verify {
 namespace {
 
@@ -151,9 +154,9 @@ __device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp
     if (CAP && s.inv_cap2 > 0.0) return x > -kInf ? e : 0.0;
     return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
 }
-// The same as a term of a sum, where e^-700 is nothing; the top finite, or capped and not -inf.
+// Its exponent, kLeast or less (or NaN) for -inf and NaN; the top finite, or capped and not -inf.
 template <bool CAPPED>
-__device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) {
+__device__ __forceinline__ double exponent(float x, const Scale& s, const Exp& exp) {
     double z;
     if (CAPPED) {
         // tanh(a) = 2 / (1 + e^-2a) - 1 of a = |x / cap|; the hardware's estimate is 2^-24 off, a step squares that
@@ -169,7 +172,18 @@ __device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) 
     } else {
         z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
     }
-    return exp(at_least(z, kLeast));
+    return z;
+}
+// The weight as a term of a sum, where e^-700 is nothing.
+template <bool CAPPED>
+__device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) {
+    return exp(at_least(exponent<CAPPED>(x, s, exp), kLeast));
+}
+// The same, but 0 where there is none.
+template <bool CAPPED>
+__device__ __forceinline__ double term_or_none(float x, const Scale& s, const Exp& exp) {
+    const double z = exponent<CAPPED>(x, s, exp);
+    return z > kLeast ? exp(z) : 0.0;
 }
 
 // Sums of uncapped terms with two operations less than term's, the same shape of e^z in x's own
@@ -203,7 +217,7 @@ constexpr double kRoomy = 0x1p40;
 
 template <bool CAP>
 __device__ __forceinline__ double any_term(float x, const Scale& s, const Exp& exp) {
-    return CAP && s.inv_cap2 > 0.0 ? term<true>(x, s, exp) : term<false>(x, s, exp);
+    return CAP && s.inv_cap2 > 0.0 ? term_or_none<true>(x, s, exp) : term_or_none<false>(x, s, exp);
 }
 
 // Eight logits from place i0 on, as they are; -inf from `end` on.
@@ -435,17 +449,16 @@ struct Rest {
         q = minus_q ? scale_of<CAP>(s.q_top, a.draft.cap, inv_heat, exp) : p;
         plain = (s.p_top < kInf || p.inv_cap2 > 0.0) && (!minus_q || (fabsf(s.q_top) < kInf || (s.q_top > 0.0f && q.inv_cap2 > 0.0)));
     }
-    // what of() gives, as a term of a sum; not where the top is infinite (`plain` says so)
+    // Whether exponent() holds: no infinite top, but under a cap.
     bool plain;
-    __device__ __forceinline__ double term_of(int at, float x, float y, const Exp& exp) const {
-        const double v = any_term<CAP>(x, p, exp) * p_scale;
-        if (minus_q) return __builtin_fmax(v - any_term<CAP>(y, q, exp) * q_scale, 0.0);
-        return at == token ? 0.0 : v;
-    }
-    // place `at`, whose logit is x and the drafter's y
+    // Place `at`, whose logit is x and the drafter's y; PLAIN: with an operation or two less, 1e-13 from what
+    // the other gives.  A part summed by one of them is searched by the same one, so that its sum is over
+    // zero exactly where one of its places has a weight (p - q can be nothing but such differences).
+    template <bool PLAIN>
     __device__ __forceinline__ double of(int at, float x, float y, const Exp& exp) const {
-        double v = weight<CAP>(x, p, exp) * p_scale;
-        if (minus_q) v = __builtin_fmax(v - weight<CAP>(y, q, exp) * q_scale, 0.0);
+        const auto one = [&](float v, const Scale& s) { return PLAIN ? any_term<CAP>(v, s, exp) : weight<CAP>(v, s, exp); };
+        double v = one(x, p) * p_scale;
+        if (minus_q) v = __builtin_fmax(__builtin_fma(-one(y, q), q_scale, v), 0.0);
         return at == token ? 0.0 : v;
     }
 };
@@ -586,12 +599,12 @@ __global__ __launch_bounds__(kWide) void rest_kernel(Args a, Work w, int parts, 
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum += rest.term_of(from + 512 * j + 8 * lane + i, x.at(j, i), y.at(j, i), exp);
+                    for (int i = 0; i < 8; ++i) sum += rest.template of<true>(from + 512 * j + 8 * lane + i, x.at(j, i), y.at(j, i), exp);
             }
         } else {
             const int end = begin + 512 * S < a.vocab ? begin + 512 * S : a.vocab;
             for (int i = begin + lane; i < end; i += 64)
-                sum += rest.of(i, load1<F32>(a.target, s.row, i), drafter ? load1<F32>(a.draft, s.row, i) : -kInf, exp);
+                sum += rest.template of<false>(i, load1<F32>(a.target, s.row, i), drafter ? load1<F32>(a.draft, s.row, i) : -kInf, exp);
         }
         sum = wave_sum(sum);
         if (lane == 0) w.rest[(int64_t)r * parts + part] = sum;
@@ -742,8 +755,9 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         return;
     }
 
-    // The place in it, likewise.
+    // The place in it, likewise, by the weights that the part's sum is of.
     const Rest<CAP> of(a, s, inv_heat, exp);
+    const bool plain = DRAFTS && s.kind == 2 && (all_rest || part == only) && of.plain;
     const int i0 = part * plan.size() + 2 * tid;
     const bool within = 2 * tid < plan.size();
     double each[2];
@@ -752,7 +766,7 @@ __global__ __launch_bounds__(kWide) void pick_kernel(Args a, Work w, Plan plan) 
         const bool live = within && i0 + i < a.vocab;
         const float x = live ? load1<F32>(a.target, s.row, i0 + i) : -kInf;
         const float y = live && of.minus_q ? load1<F32>(a.draft, s.row, i0 + i) : -kInf;
-        each[i] = of.of(i0 + i, x, y, exp);
+        each[i] = plain ? of.template of<true>(i0 + i, x, y, exp) : of.template of<false>(i0 + i, x, y, exp);
     }
     const double both = each[0] + each[1], scan = group_scan(both, sums, &total), found = past ? 0.0 : before_found;
     upto = scan + found;

@@ -4,9 +4,13 @@ float64 on the host: uniforms of 0 and from 1 on beside places without weight.  
 import numpy as np
 import pytest
 
-from test_gpu_sampling import dev
+from test_gpu_sampling import dev, verify
 
 pytestmark = pytest.mark.gpu
+
+ONE_LESS = np.nextafter(np.float32(1), np.float32(0))
+# rows and vocabularies whose rows are cut into parts of 512, and of 2048
+SIZES = [(2, 3000, 512), (512, 8192, 2048)]
 
 
 def test_the_first_of_two_neighbours(gpu_lib):
@@ -21,3 +25,103 @@ def test_the_first_of_two_neighbours(gpu_lib):
             u = dev(np.zeros(1, np.float32))
             assert sample(dev(x), u, 1.0).tolist() == [at], at
             assert sample(dev(x), u, 1.0, softcap=100.0).tolist() == [at], at
+
+
+def blocks(rows):
+    """Requests of two rows: one draft each."""
+    return np.arange(0, rows + 1, 2)
+
+
+def check(x, tokens, starts, u, heats, y=None, cap=0.0):
+    """verify_drafts of float64 logits that are exact in float32, against the host's."""
+    from helios_amd import verify_drafts
+
+    on_gpu = lambda v: dev(v.astype(np.float32))  # noqa: E731
+    given = {} if y is None else dict(draft_logits=on_gpu(y), draft_softcap=cap)
+    got, count = verify_drafts(on_gpu(x), dev(tokens), dev(starts.astype(np.int32)), dev(u), dev(heats), softcap=cap, **given)
+    want, accepted = verify(x, tokens, starts, u, heats, y, cap, cap)
+    assert count.tolist() == accepted.tolist()
+    assert got.tolist() == want.tolist()
+    return got, count
+
+
+@pytest.mark.parametrize("rows,vocab,size", SIZES)
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_parts_of_nothing_with_a_drafter(gpu_lib, rows, vocab, size, cap, end):
+    """Parts that are masked in both, or far below, have no remainder, whatever u: the token comes
+    from the others (the first with any at 0, the last from 1 on)."""
+    rng = np.random.default_rng(rows + vocab)
+    x = np.round(rng.standard_normal((rows, vocab)) * 8) / 8
+    y = x * 0.5
+    here = slice(0, size) if end == "first" else slice(vocab - size, vocab)
+    kind = rng.integers(0, 3, size)
+    low = np.where(kind == 0, -np.inf, np.where(kind == 1, np.nan, -3000.0 if not cap else -np.inf))
+    x[:, here] = y[:, here] = low
+    middle = np.arange(size + 4, vocab - size)
+    tokens = rng.choice(middle, rows).astype(np.int32)
+    x[np.arange(rows - 1), tokens[1:]] = -5.0  # every draft falls
+    y[np.arange(rows - 1), tokens[1:]] = 9.0
+    x[:, size + 3] = 19.0  # the target is the more certain one
+    starts, heats = blocks(rows), np.full(rows // 2, 0.7, np.float32)
+    u = np.zeros((rows, 2), np.float32)
+    u[:, 0] = ONE_LESS
+    for v in (0.0, 1.0, 7.0, 0.5):
+        u[:, 1] = v
+        got, count = check(x, tokens, starts, u, heats, y, cap)
+        assert int(count.sum()) == 0 and bool((got[::2] >= 0).all())
+
+
+@pytest.mark.parametrize("rows,vocab,size", SIZES)
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("low", [-np.inf, -100.0])
+def test_a_part_of_nothing_but_the_draft(gpu_lib, rows, vocab, size, cap, low):
+    """Without a drafter's logits the fallen draft's part may hold nothing else: masked places, or
+    at a temperature of 0.05 ones 2000 below the top."""
+    if cap and low > -np.inf:
+        low = -20.0  # capped at -17.5, some 900 below the top at a temperature of 0.03
+    rng = np.random.default_rng(rows + vocab + 1)
+    x = np.round(rng.standard_normal((rows, vocab)) * 8) / 8
+    heats = np.full(rows // 2, 0.05 if not cap else 0.03, np.float32)
+    for end in ("first", "last"):
+        z = x.copy()
+        here = slice(0, size) if end == "first" else slice((vocab - 1) // size * size, vocab)
+        z[:, here] = low
+        z[:, size + 5] = 10.0
+        inside = np.arange(vocab)[here]
+        tokens = rng.choice(inside, rows).astype(np.int32)
+        u = np.zeros((rows, 2), np.float32)
+        u[:, 0] = ONE_LESS
+        for v in (0.0, 1.0, 0.3):
+            u[:, 1] = v
+            got, count = check(z, tokens, blocks(rows), u, heats, None, cap)
+            assert int(count.sum()) == 0 and bool((got[::2] >= 0).all())
+        # the draft has nearly all of the row's weight, and still falls
+        z[np.arange(rows - 1), tokens[1:]] = 10.5  # all but 4e-5 or 4e-7 of it
+        for v in (0.0, 1.0, 0.3):
+            u[:, 1] = v
+            got, count = check(z, tokens, blocks(rows), u, heats, None, cap)
+            assert int(count.sum()) == 0 and bool((got[::2] >= 0).all())
+
+
+@pytest.mark.parametrize("rows,vocab,size", SIZES)
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_remainders_of_roundings_alone(gpu_lib, rows, vocab, size, cap):
+    """p and q that differ by roundings alone in most parts: whatever u, a token that the target can give."""
+    import torch
+
+    from helios_amd import verify_drafts
+
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    y = np.roll(x, 1, axis=1)
+    y[:, :2 * size] = x[:, :2 * size]
+    y[:, 2 * size] = x[:, vocab - 1]  # the same values in another order
+    x[:, 7::16] = y[:, 7::16] = -np.inf
+    tokens = np.full(rows, 7, np.int32)
+    u = np.zeros((rows, 2), np.float32)
+    for v in (0.0, 1e-20, 1.0):
+        u[:, 1] = v
+        got, count = verify_drafts(dev(x), dev(tokens), dev(blocks(rows).astype(np.int32)), dev(u), 0.9, draft_logits=dev(y), softcap=cap, draft_softcap=cap)
+        assert int(count.sum()) == 0 and bool((got[::2] >= 0).all())
+        assert bool(torch.isfinite(dev(x)[::2].gather(1, got[::2, None].long())).all())
