@@ -121,9 +121,9 @@ __device__ __forceinline__ double at_least(double a, double b) {
 
 // A distribution over a row's places: z = cap tanh(x / cap) / T, relative to that of `top`.
 struct Scale {
-    double inv_heat, top_z;     // 1 / T, z of the top
+    double inv_heat, top_z;     // 1 / T, z of the top (of capped logits; of others z is of the difference to the top)
     double cap_heat, inv_cap2;  // cap / T and 2 / cap (0: no cap)
-    float top;
+    double top;
 };
 
 // tanh(x / cap) by e^(-2 |x / cap|): the quotient's Newton steps start from the hardware's estimate.
@@ -143,13 +143,14 @@ __device__ __forceinline__ double heated(float x, const Scale& s, const Exp& exp
 template <bool CAP>
 __device__ __forceinline__ Scale scale_of(float top, double cap, double inv_heat, const Exp& exp) {
     Scale s{inv_heat, 0.0, cap * inv_heat, CAP && cap > 0.0 ? 2.0 / cap : 0.0, top};
-    s.top_z = heated<CAP>(top, s, exp);
+    if (CAP) s.top_z = heated<CAP>(top, s, exp);
     return s;
 }
 // e^(z(x) - z(top)); 0 for -inf, NaN and less than e^-700.
 template <bool CAP>
 __device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp) {
-    const double z = CAP ? heated<CAP>(x, s, exp) - s.top_z : __builtin_fma((double)x, s.inv_heat, -s.top_z);
+    // x - top is exact, or off by 2^-53 of it; x / T - top / T would be off by that of a quotient without bound
+    const double z = CAP && s.inv_cap2 > 0.0 ? heated<CAP>(x, s, exp) - s.top_z : ((double)x - s.top) * s.inv_heat;
     const double e = z >= kLeast ? exp(z) : 0.0;
     if (CAP && s.inv_cap2 > 0.0) return x > -kInf ? e : 0.0;
     return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
@@ -170,7 +171,7 @@ __device__ __forceinline__ double exponent(float x, const Scale& s, const Exp& e
         bits.y = x > -kInf ? bits.y : least.y;
         z = __builtin_bit_cast(double, bits);
     } else {
-        z = __builtin_fma((double)x, s.inv_heat, -s.top_z);
+        z = ((double)x - s.top) * s.inv_heat;
     }
     return z;
 }

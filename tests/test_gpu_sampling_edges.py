@@ -4,7 +4,7 @@ float64 on the host: uniforms of 0 and from 1 on beside places without weight.  
 import numpy as np
 import pytest
 
-from test_gpu_sampling import dev, verify
+from test_gpu_sampling import chances, dev, drafts, pick, verify
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,82 @@ def test_remainders_of_roundings_alone(gpu_lib, rows, vocab, size, cap):
         got, count = verify_drafts(dev(x), dev(tokens), dev(blocks(rows).astype(np.int32)), dev(u), 0.9, draft_logits=dev(y), softcap=cap, draft_softcap=cap)
         assert int(count.sum()) == 0 and bool((got[::2] >= 0).all())
         assert bool(torch.isfinite(dev(x)[::2].gather(1, got[::2, None].long())).all())
+
+
+def random_uniforms(rng, n):
+    u = rng.random(n).astype(np.float32)
+    return np.minimum(u, ONE_LESS)
+
+
+def draw_all(x, u, heat, cap=0.0, kind=None):
+    """The same row for each uniform."""
+    from helios_amd import sample
+
+    t = dev(np.broadcast_to(x.astype(np.float32), (len(u), len(x))).copy(), kind)
+    return sample(t, dev(u), heat, softcap=cap).tolist()
+
+
+HEATS = [1e-3, 3e-7, 1e-10, 1e-11, 3e-12, 1e-13, 1e-16, 1e-18, 1e-20, 1e-27, 1e-37, 1e-42]
+
+
+@pytest.mark.parametrize("heat", HEATS)
+@pytest.mark.parametrize("cap", [0.0])
+@pytest.mark.parametrize("vocab", [3000, 40000])
+def test_small_temperatures(gpu_lib, heat, cap, vocab):
+    """What is equal to the largest logit has its weight; of the smaller ones those have one that a
+    temperature of 3e-7 and more leaves within e^-700."""
+    rng = np.random.default_rng(int(-np.log10(heat) * 10) + vocab)
+    for trial in range(6):
+        x = rng.uniform(5.0, 30.0, vocab).astype(np.float32)
+        top = np.float32(rng.uniform(30.5, 34.0))
+        places = np.sort(rng.choice(vocab, 3, replace=False))
+        x[places] = top
+        u = random_uniforms(rng, 20)
+        u[0] = 0.0
+        if heat >= 3e-7:
+            p = chances(x.astype(np.float64), np.float32(heat), cap)
+            want = [pick(np.where(p >= p.max() * np.exp(-700.0), p, 0.0), v) for v in u]
+        else:
+            want = [int(places[int(v * 3)]) for v in u.astype(np.float64)]
+        assert draw_all(x, u, heat, cap) == want, trial
+
+
+@pytest.mark.parametrize("step,over", [(1, 0.8), (1, 3.0), (3, 2.0)])
+def test_temperatures_of_a_step(gpu_lib, step, over):
+    """Logits one or some float32 steps under the top, and a temperature of that size."""
+    rng = np.random.default_rng(step)
+    for top in (0.7, 19.3, 5e-6, 3e20):
+        top = np.float32(top)
+        ulp = float(np.spacing(top))
+        heat = np.float32(ulp * over)
+        x = np.full(4000, 0.0, np.float32) - np.float32(top)
+        some = rng.choice(4000, 30, replace=False)
+        x[some] = (float(top) - rng.integers(0, 4, 30) * step * ulp).astype(np.float32)
+        u = random_uniforms(rng, 40)
+        z = (x.astype(np.float64) - float(x.max())) / float(heat)  # exact differences
+        e = np.exp(z)
+        p = e / e.sum()
+        assert draw_all(x, u, float(heat)) == [pick(p, v) for v in u], (top, heat)
+
+
+@pytest.mark.parametrize("cap,heat", [(30.0, 1e-6), (0.0, 1e-18)])
+def test_drafts_at_far_softcaps_and_temperatures(gpu_lib, cap, heat):
+    """The check of drafts by the same weights: a large cap is none, a small temperature the first largest."""
+    rng = np.random.default_rng(31)
+    for rows, vocab, _ in SIZES:
+        x = (np.round(rng.standard_normal((rows, vocab)) * 64) / 64).astype(np.float32).astype(np.float64)
+        x[np.arange(rows), rng.integers(0, vocab, rows)] = 9.0  # one largest logit
+        y = np.roll(x, 3, axis=1)
+        y[::4] = x[::4]
+        starts, heats = blocks(rows), np.full(rows // 2, heat, np.float32)
+        greedy = heat < 1e-3
+        _, tokens = drafts(rng, x, [0.0 if greedy else float(h) for h in heats], starts, 0.0)
+        from helios_amd import verify_drafts
+
+        u = random_uniforms(rng, 2 * rows).reshape(rows, 2)
+        on_gpu = lambda v: dev(v.astype(np.float32))  # noqa: E731
+        for drafter in (None, y):
+            given = {} if drafter is None else dict(draft_logits=on_gpu(y), draft_softcap=cap)
+            got, count = verify_drafts(on_gpu(x), dev(tokens), dev(starts.astype(np.int32)), dev(u), dev(heats), softcap=cap, **given)
+            want, accepted = verify(x, tokens, starts, u, heats * 0 if greedy else heats, drafter)
+            assert count.tolist() == accepted.tolist() and got.tolist() == want.tolist()
