@@ -121,59 +121,83 @@ __device__ __forceinline__ double at_least(double a, double b) {
 
 // A distribution over a row's places: z = cap tanh(x / cap) / T, relative to that of `top`.
 struct Scale {
-    double inv_heat, top_z;     // 1 / T, z of the top (of capped logits; of others z is of the difference to the top)
+    double inv_heat, top;       // 1 / T
     double cap_heat, inv_cap2;  // cap / T and 2 / cap (0: no cap)
-    double top;
+    double at_top;              // capped: z of the top or, where cap / T is over kSteep, its factor of z
 };
 
-// tanh(x / cap) by e^(-2 |x / cap|): the quotient's Newton steps start from the hardware's estimate.
-__device__ __forceinline__ double tanh_of(double x, double inv_cap2, const Exp& exp) {
-    const double z = -__builtin_fabs(x) * inv_cap2;
-    const double e = z >= kLeast ? exp(z) : 0.0, d = 1.0 + e;
+// cap / T up to which tanh itself is taken, 1e-13 off: z is off by cap / T * 2e-13, 6e-12 at a cap of 30 and T = 1, 3e-9 at
+// most.  256 rows of 262144 bf16: 84 us, and 224 past kSteep.
+constexpr double kSteep = 16384.0;
+
+__device__ __forceinline__ double reciprocal(double d) {
     double y = __builtin_amdgcn_rcp(d);
     y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+}
+// tanh(x / cap) by e^-2|a| of a = x / cap: 2 / (1 + e^-2|a|) - 1; the hardware's estimate is 2^-24 off, a step squares that
+__device__ __forceinline__ double tanh_of(float x, double inv_cap2, const Exp& exp) {
+    const double e = exp(at_least(__builtin_fabs((double)x) * -inv_cap2, kLeast)), d = 1.0 + e;
+    double y = __builtin_amdgcn_rcp(d);
     y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
-    return __builtin_copysign((1.0 - e) * y, x);
+    return __builtin_copysign(__builtin_fma(2.0, y, -1.0), (double)x);
 }
-// CAP: the target's or the drafter's logits are capped.
-template <bool CAP>
-__device__ __forceinline__ double heated(float x, const Scale& s, const Exp& exp) {
-    return CAP && s.inv_cap2 > 0.0 ? s.cap_heat * tanh_of(x, s.inv_cap2, exp) : (double)x * s.inv_heat;
+
+// Past kSteep, and with it for large caps, the difference of two tanh is formed as a product, some 5e-13 of itself off:
+//   tanh a - tanh b = 2 s(-2a) (e^(2 (a - b)) - 1) s(2b),  s(v) = 1 / (1 + e^-v)
+__device__ __forceinline__ double logistic(double v, const Exp& exp) {
+    const double size = -__builtin_fabs(v), e = size >= kLeast ? exp(size) : 0.0, y = reciprocal(1.0 + e);
+    return v < 0.0 ? e * y : y;
 }
+struct Inverses {
+    double v[15];
+};
+constexpr Inverses make_inverses() {
+    Inverses t{};
+    for (int k = 1; k < 15; ++k) t.v[k] = 1.0 / k;
+    return t;
+}
+__device__ const Inverses kInverse = make_inverses();
+// e^v - 1 of v <= 0: the series to the 14th power (4e-17) where e^v is near 1.
+__device__ __forceinline__ double exp_less_one(double v, const Exp& exp) {
+    if (v < -0.5) return v >= kLeast ? exp(v) - 1.0 : -1.0;
+    double sum = 1.0;
+#pragma unroll 1  // in line its constants take the registers of the paths beside it
+    for (int k = 14; k > 1; --k) sum = __builtin_fma(sum * v, kInverse.v[k], 1.0);
+    return sum * v;
+}
+
 template <bool CAP>
 __device__ __forceinline__ Scale scale_of(float top, double cap, double inv_heat, const Exp& exp) {
-    Scale s{inv_heat, 0.0, cap * inv_heat, CAP && cap > 0.0 ? 2.0 / cap : 0.0, top};
-    if (CAP) s.top_z = heated<CAP>(top, s, exp);
+    Scale s{inv_heat, (double)top, cap * inv_heat, CAP && cap > 0.0 ? 2.0 / cap : 0.0, 0.0};
+    if (CAP && s.inv_cap2 > 0.0)
+        s.at_top = s.cap_heat > kSteep ? 2.0 * s.cap_heat * logistic(s.top * s.inv_cap2, exp) : s.cap_heat * tanh_of(top, s.inv_cap2, exp);
     return s;
 }
-// e^(z(x) - z(top)); 0 for -inf, NaN and less than e^-700.
-template <bool CAP>
-__device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp) {
-    // x - top is exact, or off by 2^-53 of it; x / T - top / T would be off by that of a quotient without bound
-    const double z = CAP && s.inv_cap2 > 0.0 ? heated<CAP>(x, s, exp) - s.top_z : ((double)x - s.top) * s.inv_heat;
-    const double e = z >= kLeast ? exp(z) : 0.0;
-    if (CAP && s.inv_cap2 > 0.0) return x > -kInf ? e : 0.0;
-    return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
-}
-// Its exponent, kLeast or less (or NaN) for -inf and NaN; the top finite, or capped and not -inf.
+
+// z relative to the top's, kLeast or less (or NaN) for -inf and NaN; the top finite, or capped and not -inf.
 template <bool CAPPED>
 __device__ __forceinline__ double exponent(float x, const Scale& s, const Exp& exp) {
-    double z;
-    if (CAPPED) {
-        // tanh(a) = 2 / (1 + e^-2a) - 1 of a = |x / cap|; the hardware's estimate is 2^-24 off, a step squares that
-        const double e = exp(at_least(__builtin_fabs((double)x) * -s.inv_cap2, kLeast)), d = 1.0 + e;
-        double y = __builtin_amdgcn_rcp(d);
-        y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
-        z = __builtin_fma(__builtin_copysign(__builtin_fma(2.0, y, -1.0), (double)x), s.cap_heat, -s.top_z);
-        // of -inf and NaN kLeast's upper half, with any lower one
-        const U2 least = __builtin_bit_cast(U2, kLeast);
-        U2 bits = __builtin_bit_cast(U2, z);
-        bits.y = x > -kInf ? bits.y : least.y;
-        z = __builtin_bit_cast(double, bits);
-    } else {
-        z = ((double)x - s.top) * s.inv_heat;
+    // x - top is exact, or off by 2^-53 of it; x / T - top / T would be off by that of a quotient without bound
+    if (!CAPPED) return ((double)x - s.top) * s.inv_heat;
+    const double z = __builtin_fma(tanh_of(x, s.inv_cap2, exp), s.cap_heat, -s.at_top);
+    // of -inf and NaN kLeast's upper half, with any lower one
+    const U2 least = __builtin_bit_cast(U2, kLeast);
+    U2 bits = __builtin_bit_cast(U2, z);
+    bits.y = x > -kInf ? bits.y : least.y;
+    return __builtin_bit_cast(double, bits);
+}
+// e^(z(x) - z(top)); 0 for -inf, NaN and less than e^-700; x is not over the top.
+template <bool CAP>
+__device__ __forceinline__ double weight(float x, const Scale& s, const Exp& exp) {
+    if (CAP && s.inv_cap2 > 0.0) {
+        const double z = s.cap_heat > kSteep ? s.at_top * logistic((double)x * -s.inv_cap2, exp) * exp_less_one(((double)x - s.top) * s.inv_cap2, exp)
+                                             : exponent<true>(x, s, exp);
+        const double e = z >= kLeast ? exp(z) : 0.0;
+        return x == kInf ? 1.0 : (x > -kInf ? e : 0.0);
     }
-    return z;
+    const double z = exponent<false>(x, s, exp), e = z >= kLeast ? exp(z) : 0.0;
+    return x == kInf ? 1.0 : e;  // beside infinity nothing finite has a weight
 }
 // The weight as a term of a sum, where e^-700 is nothing.
 template <bool CAPPED>
@@ -358,7 +382,7 @@ __global__ __launch_bounds__(kStatsThreads, F32 && S > 1 ? 5 : 8) void stats_ker
     if (inv_heat > 0.0) {
         const Scale scale = scale_of<CAP>(top, l.cap, inv_heat, exp);
         const bool capped = CAP && scale.inv_cap2 > 0.0;
-        if (capped && top > -kInf) {
+        if (capped && top > -kInf && scale.cap_heat <= kSteep) {
 #pragma unroll
             for (int j = 0; j < S; ++j)
 #pragma unroll
@@ -376,7 +400,7 @@ __global__ __launch_bounds__(kStatsThreads, F32 && S > 1 ? 5 : 8) void stats_ker
                     if (i == 7) __builtin_amdgcn_sched_barrier(0);  // more at once do not fit the registers
                 }
             sum = of.relative_to(top, exp);
-        } else {  // nothing, infinities (which share all there is), or larger than Sum has room for
+        } else {  // nothing, infinities (which share all there is), larger than Sum has room for, or past kSteep
             const int end = begin + 512 * S < a.vocab ? begin + 512 * S : a.vocab;
             for (int i = begin + lane; i < end; i += 64) sum += weight<CAP>(load1<F32>(l, row, i), scale, exp);
         }
@@ -448,9 +472,10 @@ struct Rest {
         : p(scale_of<CAP>(s.p_top, a.target.cap, inv_heat, exp)), p_scale(s.p_scale), q_scale(s.q_scale), token(s.token),
           minus_q(s.kind == 2 && a.draft.x != nullptr) {
         q = minus_q ? scale_of<CAP>(s.q_top, a.draft.cap, inv_heat, exp) : p;
-        plain = (s.p_top < kInf || p.inv_cap2 > 0.0) && (!minus_q || (fabsf(s.q_top) < kInf || (s.q_top > 0.0f && q.inv_cap2 > 0.0)));
+        const auto holds = [](float top, const Scale& z) { return CAP && z.inv_cap2 > 0.0 ? top > -kInf && z.cap_heat <= kSteep : fabsf(top) < kInf; };
+        plain = holds(s.p_top, p) && (!minus_q || holds(s.q_top, q));
     }
-    // Whether exponent() holds: no infinite top, but under a cap.
+    // Whether exponent() holds of both.
     bool plain;
     // Place `at`, whose logit is x and the drafter's y; PLAIN: with an operation or two less, 1e-13 from what
     // the other gives.  A part summed by one of them is searched by the same one, so that its sum is over

@@ -1,5 +1,12 @@
 """Sampling and verification at the ends of what they take, on the GPU against the definitions in
-float64 on the host: uniforms of 0 and from 1 on beside places without weight.  Tokens have to be equal."""
+float64 (or in decimals of 60 digits) on the host: uniforms of 0 and from 1 on beside places without
+weight, temperatures and softcaps over float32's range.
+
+Tokens have to be equal: uniforms are drawn at random, and a token differs only where one lies within the
+kernels' error of a border (2e-13 of the sum, with a softcap up to 3e-9), which happens once in 10^5 runs
+with other numbers than these."""
+
+import decimal
 
 import numpy as np
 import pytest
@@ -144,7 +151,7 @@ HEATS = [1e-3, 3e-7, 1e-10, 1e-11, 3e-12, 1e-13, 1e-16, 1e-18, 1e-20, 1e-27, 1e-
 
 
 @pytest.mark.parametrize("heat", HEATS)
-@pytest.mark.parametrize("cap", [0.0])
+@pytest.mark.parametrize("cap", [0.0, 30.0, 5.0])
 @pytest.mark.parametrize("vocab", [3000, 40000])
 def test_small_temperatures(gpu_lib, heat, cap, vocab):
     """What is equal to the largest logit has its weight; of the smaller ones those have one that a
@@ -183,7 +190,7 @@ def test_temperatures_of_a_step(gpu_lib, step, over):
         assert draw_all(x, u, float(heat)) == [pick(p, v) for v in u], (top, heat)
 
 
-@pytest.mark.parametrize("cap,heat", [(30.0, 1e-6), (0.0, 1e-18)])
+@pytest.mark.parametrize("cap,heat", [(30.0, 1e-6), (0.0, 1e-18), (1e12, 1.0), (3.4e38, 0.7), (30.0, 1e-17)])
 def test_drafts_at_far_softcaps_and_temperatures(gpu_lib, cap, heat):
     """The check of drafts by the same weights: a large cap is none, a small temperature the first largest."""
     rng = np.random.default_rng(31)
@@ -204,3 +211,60 @@ def test_drafts_at_far_softcaps_and_temperatures(gpu_lib, cap, heat):
             got, count = verify_drafts(on_gpu(x), dev(tokens), dev(starts.astype(np.int32)), dev(u), dev(heats), softcap=cap, **given)
             want, accepted = verify(x, tokens, starts, u, heats * 0 if greedy else heats, drafter)
             assert count.tolist() == accepted.tolist() and got.tolist() == want.tolist()
+
+
+def exact_chances(x, heat, cap):
+    """softmax(cap tanh(x / cap) / heat) with 60 digits."""
+    with decimal.localcontext() as c:
+        c.prec, c.Emin, c.Emax = 60, -10 ** 9, 10 ** 9
+        D = decimal.Decimal
+        cap, heat = D(float(np.float32(cap))), D(float(np.float32(heat)))
+        cache = {}
+        for v in set(x.tolist()):
+            w = D(v) / cap
+            if abs(w) < D("1e-15"):
+                t = w - w ** 3 / 3
+            else:
+                e = (-2 * abs(w)).exp()
+                t = ((1 - e) / (1 + e)).copy_sign(w)
+            cache[v] = cap * t / heat
+        top = max(cache.values())
+        e = {v: (z - top).exp() for v, z in cache.items()}
+        weights = [e[v] for v in x.tolist()]
+        total = sum(weights)
+        return [w / total for w in weights]
+
+
+def exact_pick(p, u):
+    with decimal.localcontext() as c:
+        c.prec = 60
+        goal, at = decimal.Decimal(float(u)) * sum(p), decimal.Decimal(0)
+        for i, w in enumerate(p):
+            at += w
+            if at > goal:
+                return i
+        return max(i for i, w in enumerate(p) if w > 0)
+
+
+CAPS = [(1e3, 1.0), (1e6, 1.0), (1e9, 1.0), (1e12, 1.0), (1e15, 1.0), (1e17, 1.0), (1e30, 1.0), (3.4e38, 1.0),
+        (1e12, 1e10), (30.0, 0.3), (30.0, 0.03), (30.0, 0.02), (30.0, 1e-3), (30.0, 1e-6), (30.0, 1e-9), (30.0, 1e-13), (30.0, 1e-15),
+        (1.0, 1.0), (1e-3, 1e-3), (1e-3, 1e-6), (1e-20, 1e-20), (1e-38, 1e-38), (1e-38, 1.0), (1e-45, 1e-45), (1e-45, 1e-40)]
+
+
+@pytest.mark.parametrize("cap,heat", CAPS)
+def test_softcaps(gpu_lib, cap, heat):
+    """Any finite softcap and temperature: the logits lie where cap tanh(x / cap) / T spreads."""
+    rng = np.random.default_rng(int(np.log10(cap) * 7 - np.log10(heat) * 3) + 1000)
+    vocab = 1500
+    for low, high in ((0.0, 1.0), (-2.0, 2.0), (6.0, 8.0)):
+        # z over a range of about 12 below some largest logit
+        at = rng.uniform(low, high)
+        if cap > 1e4:
+            at *= heat / cap * 5
+        slope = 1 - np.tanh(at) ** 2
+        x = cap * at - rng.uniform(0, 12, vocab) * heat / max(slope, 1e-6)
+        x = np.clip(x, -3.4e38, 3.4e38).astype(np.float32)
+        u = random_uniforms(rng, 24)
+        p = exact_chances(x.astype(np.float64), heat, cap)
+        got = draw_all(x, u, heat, cap)
+        assert got == [exact_pick(p, v) for v in u], (low, high)
