@@ -204,12 +204,6 @@ template <bool CAPPED>
 __device__ __forceinline__ double term(float x, const Scale& s, const Exp& exp) {
     return exp(at_least(exponent<CAPPED>(x, s, exp), kLeast));
 }
-// The same, but 0 where there is none.
-template <bool CAPPED>
-__device__ __forceinline__ double term_or_none(float x, const Scale& s, const Exp& exp) {
-    const double z = exponent<CAPPED>(x, s, exp);
-    return z > kLeast ? exp(z) : 0.0;
-}
 
 // Sums of uncapped terms with two operations less than term's, the same shape of e^z in x's own
 // units: x = (N + r) T ln2 / 256, N's share of the top taken off in t, r's at the end.
@@ -242,7 +236,7 @@ constexpr double kRoomy = 0x1p40;
 
 template <bool CAP>
 __device__ __forceinline__ double any_term(float x, const Scale& s, const Exp& exp) {
-    return CAP && s.inv_cap2 > 0.0 ? term_or_none<true>(x, s, exp) : term_or_none<false>(x, s, exp);
+    return CAP && s.inv_cap2 > 0.0 ? term<true>(x, s, exp) : term<false>(x, s, exp);
 }
 
 // Eight logits from place i0 on, as they are; -inf from `end` on.
@@ -474,17 +468,24 @@ struct Rest {
         q = minus_q ? scale_of<CAP>(s.q_top, a.draft.cap, inv_heat, exp) : p;
         const auto holds = [](float top, const Scale& z) { return CAP && z.inv_cap2 > 0.0 ? top > -kInf && z.cap_heat <= kSteep : fabsf(top) < kInf; };
         plain = holds(s.p_top, p) && (!minus_q || holds(s.q_top, q));
+        nothing = exp(kLeast);
     }
     // Whether exponent() holds of both.
     bool plain;
+    double nothing;  // the term of a place without weight
     // Place `at`, whose logit is x and the drafter's y; PLAIN: with an operation or two less, 1e-13 from what
     // the other gives.  A part summed by one of them is searched by the same one, so that its sum is over
     // zero exactly where one of its places has a weight (p - q can be nothing but such differences).
     template <bool PLAIN>
     __device__ __forceinline__ double of(int at, float x, float y, const Exp& exp) const {
-        const auto one = [&](float v, const Scale& s) { return PLAIN ? any_term<CAP>(v, s, exp) : weight<CAP>(v, s, exp); };
-        double v = one(x, p) * p_scale;
-        if (minus_q) v = __builtin_fmax(__builtin_fma(-one(y, q), q_scale, v), 0.0);
+        double v;
+        if (PLAIN) {
+            v = (any_term<CAP>(x, p, exp) - nothing) * p_scale;  // changes no term over 1e-288; of q's it may stay
+            if (minus_q) v = __builtin_fmax(__builtin_fma(-any_term<CAP>(y, q, exp), q_scale, v), 0.0);
+        } else {
+            v = weight<CAP>(x, p, exp) * p_scale;
+            if (minus_q) v = __builtin_fmax(__builtin_fma(-weight<CAP>(y, q, exp), q_scale, v), 0.0);
+        }
         return at == token ? 0.0 : v;
     }
 };
