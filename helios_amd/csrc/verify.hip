@@ -321,10 +321,10 @@ __device__ __forceinline__ int request_of(const Args& a, int row) {
     return row < a.starts[0] ? a.requests : request;
 }
 __device__ __forceinline__ int start_of(const Args& a, int r) { return a.starts == nullptr ? r : clampi(a.starts[r], 0, a.rows); }
-// The request's temperature; 0 where it is greedy, and past 1e30 all finite logits are equal.
+// The request's temperature; 0 where it is greedy.  For infinity 1e60, over which all logits are equal.
 __device__ __forceinline__ double heat_of(const Args& a, int r) {
     const float t = a.heats != nullptr ? a.heats[r] : a.heat;
-    return t > 0.0f ? (double)fminf(t, 1e30f) : 0.0;
+    return t > 0.0f ? (t < kInf ? (double)t : 1e60) : 0.0;
 }
 __device__ __forceinline__ double inv_of(double heat) { return heat > 0.0 ? 1.0 / heat : 0.0; }
 __device__ __forceinline__ double inv_heat_of(const Args& a, int r) { return inv_of(heat_of(a, r)); }

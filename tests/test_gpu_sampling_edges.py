@@ -247,7 +247,7 @@ def exact_pick(p, u):
 
 
 CAPS = [(1e3, 1.0), (1e6, 1.0), (1e9, 1.0), (1e12, 1.0), (1e15, 1.0), (1e17, 1.0), (1e30, 1.0), (3.4e38, 1.0),
-        (1e12, 1e10), (30.0, 0.3), (30.0, 0.03), (30.0, 0.02), (30.0, 1e-3), (30.0, 1e-6), (30.0, 1e-9), (30.0, 1e-13), (30.0, 1e-15),
+        (1e12, 1e10), (3.4e38, 3e38), (30.0, 0.3), (30.0, 0.03), (30.0, 0.02), (30.0, 1e-3), (30.0, 1e-6), (30.0, 1e-9), (30.0, 1e-13), (30.0, 1e-15),
         (1.0, 1.0), (1e-3, 1e-3), (1e-3, 1e-6), (1e-20, 1e-20), (1e-38, 1e-38), (1e-38, 1.0), (1e-45, 1e-45), (1e-45, 1e-40)]
 
 
@@ -268,3 +268,25 @@ def test_softcaps(gpu_lib, cap, heat):
         p = exact_chances(x.astype(np.float64), heat, cap)
         got = draw_all(x, u, heat, cap)
         assert got == [exact_pick(p, v) for v in u], (low, high)
+
+
+@pytest.mark.parametrize("heat", [1e28, 1e30, 1e31, 1e37, 3e38])
+def test_large_temperatures(gpu_lib, heat):
+    """Logits of float32's largest values over temperatures of that size."""
+    rng = np.random.default_rng(int(np.log10(heat)))
+    for cap in (0.0, 3e38):
+        x = np.clip(rng.uniform(-12, 12, 3000) * heat, -3.4e38, 3.4e38).astype(np.float32)
+        u = random_uniforms(rng, 40)
+        p = chances(x.astype(np.float64), float(np.float32(heat)), float(np.float32(cap)))
+        assert draw_all(x, u, heat, cap) == [pick(p, v) for v in u], cap
+
+
+def test_an_infinite_temperature_is_uniform(gpu_lib):
+    """In the array of temperatures: every place that can be given is as likely as another."""
+    from helios_amd import sample
+
+    x = np.linspace(-3e38, 3e38, 3000).astype(np.float32)
+    x[::2] = -np.inf
+    u = np.array([0.0, 0.25, 0.5, 0.75, ONE_LESS], np.float32)
+    got = sample(dev(np.tile(x, (5, 1))), dev(u), dev(np.full(5, np.inf, np.float32))).tolist()
+    assert got == [2 * int(float(v) * 1500) + 1 for v in u]
