@@ -25,6 +25,16 @@ class _Logits(ctypes.Structure):
     _fields_ = [("x_dev", _vp), ("stride", _u64), ("dtype", _u32), ("softcap", _f32)]
 
 
+def _number(v, what: str, zero: str):
+    """A finite v >= 0 that is not 0 for the library, which takes float32, alone."""
+    v = float(v)
+    if not 0.0 <= v < math.inf:
+        raise _invalid(f"{what} must be finite and >= 0 (0: {zero})")
+    if 0.0 < v <= 2.0 ** -150:
+        raise _invalid(f"{what} must be 0 ({zero}) or over 2^-150: a smaller one is 0 in float32")
+    return v
+
+
 def _logits(t, what: str, softcap):
     import torch
 
@@ -34,9 +44,7 @@ def _logits(t, what: str, softcap):
     rows, vocab = t.shape
     if vocab > 1 and t.stride(1) != 1:
         raise _invalid(f"{what} must have each row contiguous")
-    softcap = float(softcap)
-    if not 0.0 <= softcap < math.inf:
-        raise _invalid(f"{what}' softcap must be finite and >= 0 (0: none)")
+    softcap = _number(softcap, f"{what}' softcap", "none")
     # a single row's stride says nothing
     return _Logits(t.data_ptr(), t.stride(0) if rows > 1 else vocab, kind, softcap)
 
@@ -55,10 +63,7 @@ def _temperature(t, requests: int):
 
     if isinstance(t, torch.Tensor):
         return 0.0, _floats(t, "temperature", (requests,))
-    t = float(t)
-    if not 0.0 <= t < math.inf:
-        raise _invalid("temperature must be finite and >= 0 (0: greedy)")
-    return t, None
+    return _number(t, "temperature", "greedy"), None
 
 
 def _ptr(t):
