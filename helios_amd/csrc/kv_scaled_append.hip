@@ -44,7 +44,7 @@ __device__ __forceinline__ Run find_run(const Batch& b, const Pages& pg, int blo
         if (r < b.requests) {
             start = run_bound(b.starts, r, b.requests, b.tokens);
             const int rows = run_bound(b.starts, r + 1, b.requests, b.tokens) - start;
-            const int len = clampi(b.kv_lens[r], 0, 0x40000000);
+            const int len = b.kv_lens[r] > 0 ? b.kv_lens[r] : 0;  // may be past the table: positions count from it
             if (rows > 0) {
                 pos = len - rows;  // of the first row; rows before position 0 or past the table go nowhere
                 lo = pos < 0 ? 0 : pos;
