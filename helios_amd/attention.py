@@ -348,7 +348,9 @@ class PagedKVCache:
                stream=None):
         """Stores the batch's k and v [rows, kv_heads, head_dim]: k normed and rotated, v
         normed, each where given.  k and v may be the same tensor.  With q [rows, heads,
-        head_dim] the same launch norms and rotates it; returns it (or None)."""
+        head_dim] the same launch norms and rotates it; returns it (or None), in a new tensor or in
+        ``out_q``, which may be q itself but not lie over k or v.  With block scales the cache's k and
+        v, and their scales, must not share memory."""
         shape, k_stride = _heads_tensor(k, "k", self.head_dim)
         v_shape, v_stride = (shape, k_stride) if v is k else _heads_tensor(v, "v", self.head_dim)
         rows = shape[0]

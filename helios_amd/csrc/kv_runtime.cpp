@@ -9,6 +9,7 @@
 
 #include "kv_index.h"
 #include "kv_kernels.h"
+#include "overlap.h"
 #include "runtime_common.h"
 
 namespace {
@@ -169,6 +170,26 @@ Gemma4Status check_pool(const Gemma4KvPool* p, const char* name, kv::Pool* out) 
 
 uint64_t table_bytes(const kv::Pool& p) { return 4 * ((uint64_t)(p.requests - 1) * (uint64_t)p.stride + (uint64_t)p.width); }
 
+// The scaled append's K and V, and its q, k and v, are workgroups of one launch in any order: null, or which of
+// the arrays written would take from another.
+const char* mixed(const kv::HeadArgs& a, const kv::BlockScales& sc) {
+    const kv::Pages& p = a.pages;
+    const uint64_t pages = (uint64_t)p.num_pages, heads = (uint64_t)p.kv_heads, slots = 1ull << p.page_shift, dim = (uint64_t)p.head_dim;
+    if (overlap(p.k, dim, p.v, dim, {{pages, (uint64_t)p.page_stride}, {slots, (uint64_t)p.token_stride}, {heads, (uint64_t)p.head_stride}}))
+        return "the k and v pages must not overlap";
+    const uint64_t per = slots >> sc.block_shift;
+    if (overlap(sc.k, per, sc.v, per, {{pages, (uint64_t)sc.page_stride}, {heads, (uint64_t)sc.head_stride}}))
+        return "the k and v scales must not overlap";
+    const kv::Heads& q = a.part[0];
+    if (q.count == 0) return nullptr;
+    const uint64_t rows = (uint64_t)a.rows;
+    const auto in = [&](const kv::Heads& h) { return Rows{h.x, 2 * (uint64_t)h.x_stride, 2 * (uint64_t)h.count * dim}; };
+    const Rows out{q.out, 2 * (uint64_t)q.out_stride, 2 * (uint64_t)q.count * dim};
+    if (overlap(out, in(a.part[1]), rows) || overlap(out, in(a.part[2]), rows)) return "q's out must not overlap k's or v's rows";
+    const bool in_place = q.out == q.x && (q.out_stride == q.x_stride || rows == 1);
+    return !in_place && overlap(out, in(q), rows) ? "q's out must be its x or not overlap it" : nullptr;
+}
+
 // scales: null, or those of the pages' blocks
 Gemma4Status append(const char* name, const Gemma4KvPages* pages, const Gemma4KvScales* scales, bool scaled, const Gemma4KvBatch* batch,
                     const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope, void* stream) {
@@ -191,6 +212,8 @@ Gemma4Status append(const char* name, const Gemma4KvPages* pages, const Gemma4Kv
     a.append = 1;
     if (scaled && !kv::scaled_append_fits(a, sc))
         return unsupported(name, "tokens * heads is too large for one launch");
+    if (scaled)
+        if (const char* const what = mixed(a, sc)) return bad(name, what);
     const hipError_t e = scaled ? kv::launch_scaled_append(a, sc, static_cast<hipStream_t>(stream))
                                 : kv::launch_heads(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail((std::string(name) + ": launch").c_str(), e);

@@ -447,7 +447,9 @@ typedef struct Gemma4KvScales {
  * where the block holds tokens before them (its first slot is not among the new ones) it never
  * falls, and where it rises the codes held are brought to the new scale and rounded again.
  * Infinities are stored as +-448 times the scale, NaN as NaN.  Slots after the new tokens are
- * left as they are.  A block must be stored to for one request only in a call. */
+ * left as they are.  A block must be stored to for one request only in a call.  The k and v pages,
+ * and the k and v scales, must not overlap, nor q's out k's or v's rows, nor other places of its own
+ * x (it may be x itself): refused.  No other array of the call may lie in what it writes. */
 Gemma4Status gemma4_kv_append_scaled(const Gemma4KvPages* pages, const Gemma4KvScales* scales, const Gemma4KvBatch* batch,
                                      const Gemma4Heads* q, const Gemma4Heads* k, const Gemma4Heads* v, const Gemma4Rope* rope,
                                      void* stream);

@@ -43,3 +43,44 @@ def test_tokens_past_a_table_of_2_30(gpu_lib, past, rows):
         want.append(x[:inside], y[:inside], KVBatch(ints(0, inside), ints(2 ** 30), tables))
     for a, b in ((got.k, want.k), (got.v, want.v), (got.k_scale, want.k_scale), (got.v_scale, want.v_scale)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_arrays_of_one_allocation(gpu_lib):
+    """K and V between each other, scales likewise, q normed in place within a fused projection's rows: as
+    from arrays apart; what shares bytes is refused and nothing is written."""
+    import torch
+
+    from helios_amd import Gemma4Error, HeadNorm, KVBatch, PagedKVCache
+
+    rng = np.random.default_rng(8)
+    pages, hk, page, d, rows = 6, 2, 32, 128, 40
+    batch = KVBatch(ints(0, 33, rows), ints(50, 7), ints(0, 1, 2, 3).view(2, 2))
+    x = randn(rng, rows, 8 * d)
+    norm = HeadNorm(None, 1e-6)
+    of = lambda t, a, b: t[:, a * d:b * d].unflatten(1, (b - a, d))  # noqa: E731
+    apart = filled(PagedKVCache.allocate(pages, page, hk, d, torch.float8_e4m3fn, scale_block=16))
+    want = apart.append(of(x, 4, 6), of(x, 6, 8), batch, k_norm=norm, v_norm=norm, q=of(x, 0, 4), q_norm=norm)
+    for axis in (0, 1, 2, 3):  # where K and V take turns
+        shape, small = [pages, hk, page, d], [pages, hk, page // 16]
+        both = torch.zeros(shape[:axis] + [2] + shape[axis:], device="cuda").to(torch.float8_e4m3fn)
+        scale = torch.zeros(small[:min(axis, 2)] + [2] + small[min(axis, 2):], dtype=torch.uint8, device="cuda")
+        cache = filled(PagedKVCache(both.select(axis, 0), both.select(axis, 1), scale.select(min(axis, 2), 0), scale.select(min(axis, 2), 1)))
+        y = x.clone()
+        got = cache.append(of(y, 4, 6), of(y, 6, 8), batch, k_norm=norm, v_norm=norm, q=of(y, 0, 4), q_norm=norm, out_q=of(y, 0, 4))
+        assert torch.equal(got, want) and torch.equal(y[:, :4 * d], want.flatten(1)) and torch.equal(y[:, 4 * d:], x[:, 4 * d:])
+        for a, b in ((cache.k, apart.k), (cache.v, apart.v), (cache.k_scale, apart.k_scale), (cache.v_scale, apart.v_scale)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), axis
+    before = [t.view(torch.uint8).clone() for t in (apart.k, apart.v, apart.k_scale, apart.v_scale, x)]
+    k, v, s, t = apart.k, apart.v, apart.k_scale, apart.v_scale
+    args = (of(x, 4, 6), of(x, 6, 8), batch)
+    for cache in (PagedKVCache(k, k, s, t), PagedKVCache(k, v, s, s), PagedKVCache(k[:-1], k[1:], s[:-1], t[:-1])):
+        with pytest.raises(Gemma4Error, match="must not overlap"):
+            cache.append(*args, k_norm=norm)
+        cache.attend(of(x, 0, 4), batch)  # reads alone
+    for out in (of(x, 2, 6), of(x, 4, 8)):
+        with pytest.raises(Gemma4Error, match="k's or v's rows"):
+            apart.append(*args, k_norm=norm, v_norm=norm, q=of(x, 0, 4), q_norm=norm, out_q=out)
+    with pytest.raises(Gemma4Error, match="be its x"):
+        apart.append(*args, q=of(x, 0, 3), q_norm=norm, out_q=of(x, 1, 4))
+    for was, t in zip(before, (apart.k, apart.v, apart.k_scale, apart.v_scale, x)):
+        assert torch.equal(was, t.view(torch.uint8))
