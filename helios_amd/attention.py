@@ -290,7 +290,9 @@ class PagedKVCache:
     or float8_e4m3fn, of equal strides.  e4m3 pages hold value / scale: one scale for all, or,
     with float8_e8m0fnu (or uint8) tensors [pages, kv_heads, page_size // block] of equal
     strides, a power of two for each ``block`` consecutive tokens (16 to 256) of a page and
-    KV head, which ``append`` sets from the values it stores.  The tensors are the caller's;
+    KV head, which ``append`` sets from the values it stores.  Tokens that are dropped again (drafts
+    that fell) leave a scale that they raised, and the tokens before them in the block rounded by
+    it.  The tensors are the caller's;
     ``PagedKVCache.allocate`` makes them."""
 
     def __init__(self, k, v, k_scale=1.0, v_scale=1.0, layout: str = "phsd"):

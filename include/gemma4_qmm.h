@@ -446,6 +446,10 @@ typedef struct Gemma4KvScales {
  * least whose scale times 448 holds the largest finite value among them (0 to 2^-100 take 27);
  * where the block holds tokens before them (its first slot is not among the new ones) it never
  * falls, and where it rises the codes held are brought to the new scale and rounded again.
+ * So a token that is dropped again (a draft that fell, one of a request that got no pages, stored
+ * behind its last ones) has a lasting effect on the tokens before it in its block: once it has raised
+ * the scale they are rounded once more, by at most half a step of a code at the raised scale (2^-4
+ * of the value, or 2^-10 of the scale), and the scale stays until the block's first slot is stored anew.
  * Infinities are stored as +-448 times the scale, NaN as NaN.  Slots after the new tokens are
  * left as they are.  A block must be stored to for one request only in a call.  The k and v pages,
  * and the k and v scales, must not overlap, nor q's out k's or v's rows, nor other places of its own
@@ -486,7 +490,8 @@ typedef struct Gemma4KvPool {
  *   query_starts_dev int32 [requests + 1], kv_lens_dev int32 [requests]: those of the batch
  *                    (exclusive sums of the new tokens; lens + new_tokens, also where pages were
  *                    not granted: the tokens then have absent pages, and nothing is stored for them
- *                    beyond the request's last page)
+ *                    beyond the request's last page; in block-scaled pages what is stored there may
+ *                    raise the scale of the tokens held.  A step keeps them out by new_tokens of 0)
  *   granted_dev      int32 [requests], 1 or 0; NULL to skip
  *   positions_dev    int32 [rows], slots_dev int64 [rows]; each NULL to skip: position of each of
  *                    the batch's rows in its request, and page * page_size + slot (-1 where there

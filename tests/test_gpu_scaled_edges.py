@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from test_gpu_attention import dev, randn
+from test_gpu_scaled_cache import codes64, e4m3, exponents, least
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +85,41 @@ def test_arrays_of_one_allocation(gpu_lib):
         apart.append(*args, q=of(x, 0, 3), q_norm=norm, out_q=of(x, 1, 4))
     for was, t in zip(before, (apart.k, apart.v, apart.k_scale, apart.v_scale, x)):
         assert torch.equal(was, t.view(torch.uint8))
+
+
+@pytest.mark.parametrize("d,block,kept,loud", [(64, 16, 5, 3), (256, 32, 20, 8), (512, 64, 1, 40), (128, 16, 15, 1)])
+def test_dropped_drafts_leave_their_scale(gpu_lib, d, block, kept, loud):
+    """Drafts 64 times as large as the tokens before them raise the block's scale for good: the
+    tokens before them are rounded twice, the second time to a step of the raised scale, and no
+    more than that; the block begun anew has a scale of its own again."""
+    import torch
+
+    from helios_amd import KVBatch, PagedKVCache
+
+    rng = np.random.default_rng(d)
+    page, hk = 64, 2
+    cache = filled(PagedKVCache.allocate(1, page, hk, d, torch.float8_e4m3fn, scale_block=block))
+    table = ints(0).view(1, 1)
+    batch = lambda n, length: KVBatch(ints(0, n), ints(length), table)  # noqa: E731
+    first, drafts, last = (randn(rng, n, hk, d) for n in (kept, loud, 1))
+    cache.append(first, first, batch(kept, kept))
+    before, low = codes64(cache.k), exponents(cache.k_scale)
+    cache.append(drafts * 64, drafts * 64, batch(loud, kept + loud))
+    cache.append(last, last, batch(1, kept + 1))  # in the first draft's place
+    after, high = codes64(cache.k), exponents(cache.k_scale)
+    in_block = min(loud, block - kept)
+    for h in range(hk):
+        y = first[:, h].double().cpu().numpy()
+        e0, e1 = int(low[0, h, 0]), int(high[0, h, 0])
+        assert e0 == least(np.abs(y).max())
+        assert e1 == least(np.abs(drafts[:in_block, h].double().cpu().numpy() * 64).max()) > e0
+        assert np.array_equal(after[0, h, :kept], e4m3(before[0, h, :kept] * 2.0 ** (e0 - e1)))
+        # half a step of each scale: 2^-4 of the value, 2^-10 of the scale under its least normal code
+        one = np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** (e0 - 10))
+        both = one + np.maximum(2.0 ** -4 * (np.abs(y) + one), 2.0 ** (e1 - 10))
+        assert (np.abs(after[0, h, :kept] * 2.0 ** e1 - y) <= both).all()
+        z = last[0, h].double().cpu().numpy()
+        assert (np.abs(after[0, h, kept] * 2.0 ** e1 - z) <= np.maximum(2.0 ** -4 * np.abs(z), 2.0 ** (e1 - 10))).all()
+    assert torch.equal(cache.k.view(torch.uint8), cache.v.view(torch.uint8)) and torch.equal(cache.k_scale, cache.v_scale)
+    cache.append(first, first, batch(kept, kept))
+    assert np.array_equal(codes64(cache.k)[0, :, :kept], before[0, :, :kept]) and np.array_equal(exponents(cache.k_scale)[0, :, 0], low[0, :, 0])
