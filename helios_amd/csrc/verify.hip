@@ -5,7 +5,8 @@
 //   the first that does not: a token from max(p - q, 0); all stand: one from the last row's p
 //   from weights w: the first i with w_0 + .. + w_i > u (w_0 + .. + w_(n-1))
 //   T = 0: p and q are 1 at the first largest logit, 0 elsewhere
-//   a logit of -inf or NaN has weight 0 whatever cap and T; a drafter that gives no logits is sure (q_d = 1)
+//   a logit of -inf or NaN, and a weight under e^-700 of the largest, is 0 whatever cap and T; a drafter that
+//   gives no logits is sure (q_d = 1)
 //
 // Sums and weights are fp64: a token is a place in a sum of some 2^18 terms, and an fp32 sum
 // (2^-24 of it off) would miss by one wherever the terms are smaller than that.
@@ -17,8 +18,8 @@
 // draft that falls and sum max(p - q, 0) over parts of that one row (rest_kernel); a workgroup per
 // request finds the part and the place in it (pick_kernel).  Orders are fixed: no atomics.
 //
-// us of the three, rows of 262144: 32 requests of 8 rows, bf16, with the drafter's rows (252 MB) 80 + 17 +
-// 8 (3.2 TB/s in the first, whose 31M operations are 53 us of issue); 256 rows without drafts (134 MB) 38 + 6;
+// us of the three, rows of 262144: 32 requests of 8 rows, bf16, with the drafter's rows (252 MB) 80 + 18 +
+// 7 (3.2 TB/s in the first, whose 31M operations are 53 us of issue); 256 rows without drafts (134 MB) 38 + 6, capped 84 in all;
 // 48 rows of fp32 (50 MB) 13 + 5 (3.8 TB/s); one row 3.7 + 6, two launches and a chain of loads.
 // Parts one after another in a wave, the next one's loads ahead of this one's sums: 84 for the 80.
 #include "q4_common.h"
@@ -473,8 +474,8 @@ struct Rest {
     // Whether exponent() holds of both.
     bool plain;
     double nothing;  // the term of a place without weight
-    // Place `at`, whose logit is x and the drafter's y; PLAIN: with an operation or two less, 1e-13 from what
-    // the other gives.  A part summed by one of them is searched by the same one, so that its sum is over
+    // Place `at`, whose logit is x and the drafter's y; PLAIN: with an operation or two less, within its error of
+    // what the other gives.  A part summed by one of them is searched by the same one, so that its sum is over
     // zero exactly where one of its places has a weight (p - q can be nothing but such differences).
     template <bool PLAIN>
     __device__ __forceinline__ double of(int at, float x, float y, const Exp& exp) const {

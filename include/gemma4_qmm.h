@@ -491,7 +491,8 @@ typedef struct Gemma4KvPool {
  *                    (exclusive sums of the new tokens; lens + new_tokens, also where pages were
  *                    not granted: the tokens then have absent pages, and nothing is stored for them
  *                    beyond the request's last page; in block-scaled pages what is stored there may
- *                    raise the scale of the tokens held.  A step keeps them out by new_tokens of 0)
+ *                    raise the scale of the tokens held.  A second call with new_tokens * granted makes
+ *                    the same step without those requests)
  *   granted_dev      int32 [requests], 1 or 0; NULL to skip
  *   positions_dev    int32 [rows], slots_dev int64 [rows]; each NULL to skip: position of each of
  *                    the batch's rows in its request, and page * page_size + slot (-1 where there
@@ -511,7 +512,9 @@ Gemma4Status gemma4_kv_release(const Gemma4KvPool* pool, const int32_t* lens_dev
 /* ---- Sampling, and drafted tokens ----
  * Rows of logits [rows, vocab], row r at x_dev + r * stride elements, BF16 or F32, aligned to their
  * type.  softcap > 0: cap * tanh(x / cap) in their place (native_model.cc:1794, unrounded).
- * Logits of -inf and NaN have no probability, whatever the softcap. */
+ * Logits of -inf and NaN have no probability, whatever the softcap, nor have those whose weight is
+ * under e^-700 of the largest's.  A weight is good to 4e-13 of itself; under a softcap to 2e-13 *
+ * softcap / temperature more, 3e-9 at most. */
 typedef struct Gemma4Logits {
     const void* x_dev;
     uint64_t stride;
@@ -522,7 +525,7 @@ typedef struct Gemma4Logits {
 /* A token from each row's p = softmax(logits / temperature): the first i with
  * p_0 + .. + p_i > uniforms[row]; the first largest logit where the temperature is 0.
  *   uniforms_dev     float [rows] in [0, 1)
- *   temperatures_dev float [rows] (0 or less: greedy), or NULL: `temperature` for all
+ *   temperatures_dev float [rows] (0 or less, or NaN: greedy; infinity: all alike), or NULL: `temperature` for all
  *   out_tokens_dev   int32 [rows]; -1 where no logit has a probability
  * Weights and sums are fp64.  Scratch: 16 bytes a row and 2048 logits (512 of few rows). */
 Gemma4Status gemma4_sample(const Gemma4Logits* logits, uint32_t rows, uint32_t vocab, const float* uniforms_dev, float temperature,

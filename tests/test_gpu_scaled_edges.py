@@ -123,3 +123,39 @@ def test_dropped_drafts_leave_their_scale(gpu_lib, d, block, kept, loud):
     assert torch.equal(cache.k.view(torch.uint8), cache.v.view(torch.uint8)) and torch.equal(cache.k_scale, cache.v_scale)
     cache.append(first, first, batch(kept, kept))
     assert np.array_equal(codes64(cache.k)[0, :, :kept], before[0, :, :kept]) and np.array_equal(exponents(cache.k_scale)[0, :, 0], low[0, :, 0])
+
+
+def test_requests_without_pages_left_out_of_a_step(gpu_lib):
+    """A second reserve of new_tokens * granted is the same step without the requests that got no
+    pages: the others keep what they were given, and nothing is stored for those."""
+    import torch
+
+    from helios_amd import PagedKVCache, PagePool
+
+    rng = np.random.default_rng(12)
+    for new, held, pages in (([5, 40, 3], [3, 10, 0], 3), ([9, 17, 17, 0, 30], [16, 16, 15, 4, 2], 6)):
+        n = len(new)
+        pool = PagePool.allocate(pages, 16, n, 6)
+        pool.reserve(ints(*held))
+        assert pool.granted.tolist() == [1] * n
+        pool.release(ints(*held))
+        first = ints(*new)
+        pool.reserve(first)
+        granted = pool.granted.tolist()
+        assert 0 in granted and 1 in granted
+        tables, count = pool.block_tables.clone(), int(pool.free_count)
+        _, slots = pool.reserve(first * pool.granted, sum(new))
+        assert pool.granted.tolist() == [1] * n and torch.equal(pool.block_tables, tables) and int(pool.free_count) == count
+        left = [a * g for a, g in zip(new, granted)]
+        assert pool.batch.query_starts.tolist() == [0] + np.cumsum(left).tolist()
+        assert pool.batch.kv_lens.tolist() == [a + b for a, b in zip(held, left)]
+        cache = filled(PagedKVCache.allocate(pages, 16, 1, 64, torch.float8_e4m3fn, scale_block=16))
+        x = randn(rng, sum(new), 1, 64)
+        cache.append(x, x, pool.batch)
+        stored = {int(s) for s in slots.tolist() if s >= 0}
+        assert len(stored) == sum(left)
+        # the places of the tokens held before, whose codes may have been lowered, and those of the new ones
+        pages_of = pool.block_tables.tolist()
+        before = {16 * pages_of[r][i // 16] + i % 16 for r in range(n) if granted[r] for i in range(held[r])}
+        changed = (cache.k.view(torch.uint8) != 0x38).any(-1).flatten().nonzero().flatten().tolist()
+        assert set(changed) <= stored | before and stored <= set(changed) | before
