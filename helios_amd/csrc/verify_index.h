@@ -20,9 +20,9 @@ struct Plan {
         return ((int64_t)rows * parts + kStatsThreads / 64 - 1) / (kStatsThreads / 64);
     }
 };
-// Parts of 2048 where that leaves two waves to a SIMD at least, else of 512.  stats_kernel in us, by
-// 512 and by 2048, rows of 262144 bf16: 3.2 / 4.1 for one, 4.5 / 4.5 for 8, 6.4 / 5.5 for 16, 10.6 / 8.9
-// for 32, 55 / 37 for 256; with a softcap 3.7 / 6.1, 6.5 / 7.4, 10.0 / 9.4, 17.1 / 16.0, 103 / 88.
+// Parts of 2048 where that leaves two waves to a SIMD at least, else of 512.  stats_kernel in us (under a
+// profiler), by 512 and by 2048, rows of 262144 bf16: 3.3 / 4.1 for one, 4.4 / 4.4 for 8, 6.1 / 5.3 for 16,
+// 11.3 / 8.7 for 32, 56 / 39 for 256; with a softcap 3.7 / 6.3, 6.2 / 7.1, 9.6 / 9.0, 16.4 / 15.5, 109 / 97.
 __host__ __device__ inline Plan plan_of(int rows, int vocab) {
     const int64_t large = (int64_t)rows * ceil_div(vocab, 2048);
     const int sweeps = large >= 2 * 4 * 256 ? 4 : 1;
